@@ -310,6 +310,68 @@ srx_status srx_layer_upsample2d(int32_t dtype, int32_t layout, const void* in, c
                                 uint32_t scale_x, uint32_t scale_y, int32_t interpolation, void* out, void* stream);
 srx_status srx_layer_add(int32_t dtype, const void* a, const void* b, void* out, size_t count, void* stream);
 
+/*
+ * Normalisation and 4-bit layers.  They have no counterparts in the reference: they are what a network of this kind
+ * needs that cannot fold its normalisation into the filters, or that runs its convolutions on 4-bit operands (a
+ * quarter of the bytes of fp16, four times its matrix rate).  All tensors are dense device tensors, channels last:
+ * sizes {N, C, H, W} held as [N][H][W][C].  dtype: 0 = fp16 storage, 1 = fp32 (arithmetic is fp32 either way).
+ *
+ *   - The first pointer of a call must be device memory; the call runs on the GPU that holds it, whichever is
+ *     current, and `stream` must belong to that GPU (NULL = its default stream).  All other pointers must be memory
+ *     that GPU can reach.  Tensors need the alignment of their element type only; sizes may be odd.
+ *   - Nothing is allocated and nothing is kept between calls: every call may be captured into a HIP graph, and calls
+ *     may overlap on different streams as long as their outputs and workspaces are different memory.
+ *   - Results do not depend on what runs beside a call: no atomics, fixed orders of summation.
+ *   - A call that is refused (SRX_ERR_INVALID) has launched nothing.  Sizes of zero are refused.
+ *   - At most 2^20 channels and filters; N*H*W at most 2^31 - 1 in srx_layer_conv2d_mx4.
+ *
+ * Activations: 0 = none, 1 = ReLU, 2 = SiLU, y / (1 + exp(-y)).
+ *
+ * The 4-bit block form (OCP microscaling format MXFP4).  The `columns` values of a row (the channels of a pixel, or of
+ * a filter tap) are taken in B = ceil(columns / 32) blocks of 32, the last one filled up with zeros.  Per row there are
+ * B scale bytes s, each standing for the factor 2^(s - 127) (255: NaN), and B times 16 bytes of codes, two to a byte,
+ * the first in the low half: bit 3 the sign, bits 0-2 one of the magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6.
+ */
+enum { SRX_ACT_NONE = 0, SRX_ACT_RELU = 1, SRX_ACT_SILU = 2 };
+
+/* Host-only: bytes of the codes and of the scales of rows x columns values.  Either output may be NULL. */
+srx_status srx_layer_mx4_sizes(uint64_t rows, uint64_t columns, uint64_t* code_bytes, uint64_t* scale_bytes);
+
+/* rows x columns values to the 4-bit block form.  A block whose largest magnitude is m gets the factor
+ * 2^max(-127, floor(log2 m) - 2) (m = 0: 2^-127); its values are divided by it, rounded to the nearest magnitude (ties
+ * to the even code) and limited to 6.  A block that holds an infinity or a NaN gets the scale 255 and codes of zero. */
+srx_status srx_layer_quantize_mx4(int32_t dtype, const void* in, uint64_t rows, uint64_t columns, void* codes,
+                                  void* scales, void* stream);
+/* And back: code times factor, exact in fp32, rounded to nearest in fp16. */
+srx_status srx_layer_dequantize_mx4(int32_t dtype, const void* codes, const void* scales, uint64_t rows,
+                                    uint64_t columns, void* out, void* stream);
+
+/* Bytes of device workspace that srx_layer_group_norm* need for these sizes (host-only). */
+srx_status srx_layer_group_norm_workspace(int32_t dtype, const uint32_t sizes[4], uint32_t groups, size_t* bytes);
+
+/* Group normalisation with an activation.  The channels are taken in `groups` groups of C / groups neighbours; with the
+ * mean and the (uncorrected) variance of an image's group over all its pixels,
+ *     out = act((in - mean) / sqrt(variance + epsilon) * scale[c] + bias[c]).
+ * scale and bias are C values of the tensor's type; NULL stands for 1 and 0.  `out` may be `in`.  The workspace may be
+ * reused by the next call on the same stream. */
+srx_status srx_layer_group_norm(int32_t dtype, const void* in, const uint32_t sizes[4], uint32_t groups,
+                                const void* scale, const void* bias, float epsilon, int32_t activation, void* out,
+                                void* workspace, size_t workspace_bytes, void* stream);
+/* The same with the fp32 result quantised as srx_layer_quantize_mx4 does, with one row per pixel: what
+ * srx_layer_conv2d_mx4 reads.  The normalised tensor is never stored. */
+srx_status srx_layer_group_norm_mx4(int32_t dtype, const void* in, const uint32_t sizes[4], uint32_t groups,
+                                    const void* scale, const void* bias, float epsilon, int32_t activation,
+                                    void* codes, void* scales, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Convolution of a 4-bit tensor (N*H*W rows of C values) with a 4-bit filter (O*kh*kw rows of C values, in that order:
+ * a filter {O, C, kh, kw} of the NHWC layout, quantised once with srx_layer_quantize_mx4): stride 1, zero padding as
+ * in srx_layer_conv2d, kh, kw <= 7; then out = act(sum + bias[o]) in the type `dtype`, bias (O values of that type) may
+ * be NULL.  A 1x1 filter is the product of a matrix of N*H*W rows with the transposed filter, so {1, C, 1, rows} are
+ * the sizes of a plain matrix product.  The sum is fp32.  A block with the scale 255 makes NaN of every sum it is in. */
+srx_status srx_layer_conv2d_mx4(int32_t dtype, const void* codes, const void* scales, const uint32_t sizes[4],
+                                const void* filter_codes, const void* filter_scales, const uint32_t filter_sizes[4],
+                                const void* bias, int32_t activation, void* out, void* stream);
+
 /* Message of the last failure on this thread (never NULL). */
 const char* srx_last_error(void);
 

@@ -23,7 +23,10 @@ SYMBOLS = ["srx_create", "srx_destroy", "srx_get_out_size", "srx_get_in_size", "
            "srx_launch_stage", "srx_frames_per_launch", "srx_device_info", "srx_last_error", "srx_upscale_frames",
            "srx_pipe_create", "srx_pipe_destroy", "srx_pipe_slots", "srx_pipe_input", "srx_pipe_submit",
            "srx_pipe_wait", "srx_layer_conv2d", "srx_layer_upsample2d", "srx_layer_add", "srx_fused_weights", "srx_pipe_set_channels", "srx_layer_plan", "srx_stage_issued_flops",
-           "srx_upscale_static", "srx_static_scratch_bytes"]
+           "srx_upscale_static", "srx_static_scratch_bytes", "srx_layer_mx4_sizes", "srx_layer_quantize_mx4",
+           "srx_layer_dequantize_mx4", "srx_layer_group_norm_workspace", "srx_layer_group_norm",
+           "srx_layer_group_norm_mx4", "srx_layer_conv2d_mx4"]
+ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2
 
 
 class SrxError(RuntimeError):
@@ -112,6 +115,14 @@ def load_library(path):
     L.srx_layer_upsample2d.argtypes = [i32, i32, vp, u32x4, u32, u32, i32, vp, vp]
     L.srx_layer_add.argtypes = [i32, vp, vp, vp, sz, vp]
     L.srx_layer_plan.argtypes = [i32, i32, u32x4, u32x4, u32x4, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]
+    u64, f32 = C.c_uint64, C.c_float
+    L.srx_layer_mx4_sizes.argtypes = [u64, u64, C.POINTER(u64), C.POINTER(u64)]
+    L.srx_layer_quantize_mx4.argtypes = [i32, vp, u64, u64, vp, vp, vp]
+    L.srx_layer_dequantize_mx4.argtypes = [i32, vp, vp, u64, u64, vp, vp]
+    L.srx_layer_group_norm_workspace.argtypes = [i32, u32x4, u32, C.POINTER(sz)]
+    L.srx_layer_group_norm.argtypes = [i32, vp, u32x4, u32, vp, vp, f32, i32, vp, vp, sz, vp]
+    L.srx_layer_group_norm_mx4.argtypes = [i32, vp, u32x4, u32, vp, vp, f32, i32, vp, vp, vp, sz, vp]
+    L.srx_layer_conv2d_mx4.argtypes = [i32, vp, vp, u32x4, vp, vp, u32x4, vp, i32, vp, vp]
     for name in SYMBOLS:
         if name not in ("srx_stage_name", "srx_last_error", "srx_frames_per_launch", "srx_pipe_slots", "srx_static_scratch_bytes"):
             getattr(L, name).restype = i32
@@ -331,6 +342,51 @@ def layer_upsample2d(dtype, layout, in_ptr, in_sizes, scale_x, scale_y, interpol
 
 def layer_add(dtype, a_ptr, b_ptr, out_ptr, count, stream=None):
     _check(lib().srx_layer_add(dtype, a_ptr, b_ptr, out_ptr, count, stream))
+
+
+def layer_mx4_sizes(rows, columns):
+    """Host-only: (code bytes, scale bytes) of rows x columns values in the 4-bit block form."""
+    c, s = C.c_uint64(), C.c_uint64()
+    _check(lib().srx_layer_mx4_sizes(rows, columns, C.byref(c), C.byref(s)))
+    return c.value, s.value
+
+
+def layer_quantize_mx4(dtype, in_ptr, rows, columns, codes_ptr, scales_ptr, stream=None):
+    """rows x columns values (dtype 0 fp16 / 1 fp32) to the 4-bit block form, on device pointers."""
+    _check(lib().srx_layer_quantize_mx4(dtype, in_ptr, rows, columns, codes_ptr, scales_ptr, stream))
+
+
+def layer_dequantize_mx4(dtype, codes_ptr, scales_ptr, rows, columns, out_ptr, stream=None):
+    """What the 4-bit block form of rows x columns values stands for."""
+    _check(lib().srx_layer_dequantize_mx4(dtype, codes_ptr, scales_ptr, rows, columns, out_ptr, stream))
+
+
+def layer_group_norm_workspace(dtype, sizes, groups):
+    """Host-only: bytes of device workspace of layer_group_norm and layer_group_norm_mx4 for sizes {N, C, H, W}."""
+    n = C.c_size_t()
+    _check(lib().srx_layer_group_norm_workspace(dtype, C.byref(_sizes(sizes)), groups, C.byref(n)))
+    return n.value
+
+
+def layer_group_norm(dtype, in_ptr, sizes, groups, scale_ptr, bias_ptr, epsilon, activation, out_ptr, workspace_ptr,
+                     workspace_bytes, stream=None):
+    """Group normalisation with an activation (ACT_*) of a channels-last tensor; scale and bias may be None."""
+    _check(lib().srx_layer_group_norm(dtype, in_ptr, C.byref(_sizes(sizes)), groups, scale_ptr, bias_ptr, epsilon, activation,
+                                      out_ptr, workspace_ptr, workspace_bytes, stream))
+
+
+def layer_group_norm_mx4(dtype, in_ptr, sizes, groups, scale_ptr, bias_ptr, epsilon, activation, codes_ptr, scales_ptr,
+                         workspace_ptr, workspace_bytes, stream=None):
+    """The same, with the result in the 4-bit block form (one row per pixel)."""
+    _check(lib().srx_layer_group_norm_mx4(dtype, in_ptr, C.byref(_sizes(sizes)), groups, scale_ptr, bias_ptr, epsilon,
+                                          activation, codes_ptr, scales_ptr, workspace_ptr, workspace_bytes, stream))
+
+
+def layer_conv2d_mx4(dtype, codes_ptr, scales_ptr, sizes, filter_codes_ptr, filter_scales_ptr, filter_sizes, bias_ptr,
+                     activation, out_ptr, stream=None):
+    """Convolution of a 4-bit tensor with a 4-bit filter (rows in the order O, kh, kw); a 1x1 filter is the matrix product."""
+    _check(lib().srx_layer_conv2d_mx4(dtype, codes_ptr, scales_ptr, C.byref(_sizes(sizes)), filter_codes_ptr, filter_scales_ptr,
+                                      C.byref(_sizes(filter_sizes)), bias_ptr, activation, out_ptr, stream))
 
 
 def fold_weights(layer, weights_path=None):

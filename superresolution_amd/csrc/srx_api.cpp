@@ -1096,6 +1096,160 @@ srx_status srx_layer_add(int32_t dtype, const void* a, const void* b, void* out,
 SRX_CATCH
 
 // ---------------------------------------------------------------------------
+// Normalisation and 4-bit layers.
+// ---------------------------------------------------------------------------
+namespace {
+// Makes the device that holds `p` current for as long as this lives.
+struct OnDeviceOf
+{
+    int before = 0, device = 0;
+    bool valid = false;
+    explicit OnDeviceOf(const void* p)
+    {
+        hipPointerAttribute_t at{};
+        if (hipPointerGetAttributes(&at, p) != hipSuccess)
+        {
+            (void)hipGetLastError();                       // the refusal is ours: leave no error behind
+            return;
+        }
+        if (at.type != hipMemoryTypeDevice && at.type != hipMemoryTypeManaged) return;
+        device = at.device;
+        if (hipGetDevice(&before) != hipSuccess || (before != device && hipSetDevice(device) != hipSuccess))
+        {
+            (void)hipGetLastError();
+            return;
+        }
+        valid = true;
+    }
+    ~OnDeviceOf() { if (valid && before != device) (void)hipSetDevice(before); }
+    OnDeviceOf(const OnDeviceOf&) = delete;
+    OnDeviceOf& operator=(const OnDeviceOf&) = delete;
+};
+
+constexpr const char* kNotOnDevice = ": the first pointer is not device memory of a GPU";
+
+bool aligned(const void* p, int32_t dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == 0 ? 1 : 3)) == 0; }
+
+// rows x columns values of the 4-bit block form that the kernels can count.
+bool validMx4(uint64_t rows, uint64_t columns)
+{
+    return rows && columns && columns <= (1u << 20) && rows < (uint64_t(1) << 40) && rows * ((columns + 31) / 32) < (uint64_t(1) << 38);
+}
+
+srx_status groupNorm(const char* who, int32_t dtype, const void* in, const uint32_t sizes[4], uint32_t groups, const void* scale,
+                     const void* bias, float epsilon, int32_t activation, void* out, void* codes, void* scales,
+                     void* workspace, size_t workspaceBytes, void* stream)
+{
+    srx::ML::Util util;
+    srx::ML::Operator op;
+    if (!in || !utilFor(dtype, 1, util) || !util.CreateGroupNormLayer(sizes, groups, epsilon, uint32_t(activation), op))
+        return fail(SRX_ERR_INVALID, std::string(who) + ": bad pointer, data type, sizes, groups (a divisor of the channels), epsilon (positive) or activation");
+    if (!aligned(in, dtype) || !aligned(scale, dtype) || !aligned(bias, dtype) || !aligned(out, dtype))
+        return fail(SRX_ERR_INVALID, std::string(who) + ": a tensor is not aligned to its element type");
+    if (reinterpret_cast<uintptr_t>(codes) & 3) return fail(SRX_ERR_INVALID, std::string(who) + ": codes must be a multiple of 4");
+    const size_t need = srx::GroupNormWorkspace(op);
+    if (need && (!workspace || workspaceBytes < need || (reinterpret_cast<uintptr_t>(workspace) & 7)))
+        return fail(SRX_ERR_INVALID, std::string(who) + ": the workspace must hold " + std::to_string(need) + " bytes (a multiple of 8)");
+    const OnDeviceOf scope(in);
+    if (!scope.valid) return fail(SRX_ERR_INVALID, std::string(who) + kNotOnDevice);
+    SRX_HIP(srx::LaunchGroupNorm(op, in, scale, bias, out, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales),
+                                 workspace, static_cast<hipStream_t>(stream)));
+    return SRX_OK;
+}
+}  // namespace
+
+srx_status srx_layer_mx4_sizes(uint64_t rows, uint64_t columns, uint64_t* codeBytes, uint64_t* scaleBytes) try
+{
+    if (!validMx4(rows, columns)) return fail(SRX_ERR_INVALID, "srx_layer_mx4_sizes: bad sizes");
+    const uint64_t blocks = rows * ((columns + 31) / 32);
+    if (codeBytes) *codeBytes = blocks * 16;
+    if (scaleBytes) *scaleBytes = blocks;
+    return SRX_OK;
+}
+SRX_CATCH
+
+srx_status srx_layer_quantize_mx4(int32_t dtype, const void* in, uint64_t rows, uint64_t columns, void* codes,
+                                  void* scales, void* stream) try
+{
+    srx::ML::Util util;
+    if (!in || !codes || !scales || !utilFor(dtype, 1, util) || !validMx4(rows, columns) || !aligned(in, dtype) ||
+        (reinterpret_cast<uintptr_t>(codes) & 3))
+        return fail(SRX_ERR_INVALID, "srx_layer_quantize_mx4: bad pointer (codes: a multiple of 4), data type or sizes");
+    const OnDeviceOf scope(in);
+    if (!scope.valid) return fail(SRX_ERR_INVALID, std::string("srx_layer_quantize_mx4") + kNotOnDevice);
+    SRX_HIP(srx::LaunchQuantizeMx4(util.GetDataType(), in, int64_t(rows), int64_t(columns), static_cast<uint8_t*>(codes),
+                                   static_cast<uint8_t*>(scales), static_cast<hipStream_t>(stream)));
+    return SRX_OK;
+}
+SRX_CATCH
+
+srx_status srx_layer_dequantize_mx4(int32_t dtype, const void* codes, const void* scales, uint64_t rows, uint64_t columns,
+                                    void* out, void* stream) try
+{
+    srx::ML::Util util;
+    if (!codes || !scales || !out || !utilFor(dtype, 1, util) || !validMx4(rows, columns) || !aligned(out, dtype) ||
+        (reinterpret_cast<uintptr_t>(codes) & 3))
+        return fail(SRX_ERR_INVALID, "srx_layer_dequantize_mx4: bad pointer (codes: a multiple of 4), data type or sizes");
+    const OnDeviceOf scope(codes);
+    if (!scope.valid) return fail(SRX_ERR_INVALID, std::string("srx_layer_dequantize_mx4") + kNotOnDevice);
+    SRX_HIP(srx::LaunchDequantizeMx4(util.GetDataType(), static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales),
+                                     int64_t(rows), int64_t(columns), out, static_cast<hipStream_t>(stream)));
+    return SRX_OK;
+}
+SRX_CATCH
+
+srx_status srx_layer_group_norm_workspace(int32_t dtype, const uint32_t sizes[4], uint32_t groups, size_t* bytes) try
+{
+    srx::ML::Util util;
+    srx::ML::Operator op;
+    if (!bytes || !utilFor(dtype, 1, util) || !util.CreateGroupNormLayer(sizes, groups, 1.0f, 0, op))
+        return fail(SRX_ERR_INVALID, "srx_layer_group_norm_workspace: bad pointer, data type, sizes or groups (a divisor of the channels)");
+    *bytes = srx::GroupNormWorkspace(op);
+    return SRX_OK;
+}
+SRX_CATCH
+
+srx_status srx_layer_group_norm(int32_t dtype, const void* in, const uint32_t sizes[4], uint32_t groups, const void* scale,
+                                const void* bias, float epsilon, int32_t activation, void* out, void* workspace,
+                                size_t workspaceBytes, void* stream) try
+{
+    if (!out) return fail(SRX_ERR_INVALID, "srx_layer_group_norm: bad output pointer");
+    return groupNorm("srx_layer_group_norm", dtype, in, sizes, groups, scale, bias, epsilon, activation, out, nullptr, nullptr,
+                     workspace, workspaceBytes, stream);
+}
+SRX_CATCH
+
+srx_status srx_layer_group_norm_mx4(int32_t dtype, const void* in, const uint32_t sizes[4], uint32_t groups, const void* scale,
+                                    const void* bias, float epsilon, int32_t activation, void* codes, void* scales,
+                                    void* workspace, size_t workspaceBytes, void* stream) try
+{
+    if (!codes || !scales) return fail(SRX_ERR_INVALID, "srx_layer_group_norm_mx4: bad output pointer");
+    return groupNorm("srx_layer_group_norm_mx4", dtype, in, sizes, groups, scale, bias, epsilon, activation, nullptr, codes, scales,
+                     workspace, workspaceBytes, stream);
+}
+SRX_CATCH
+
+srx_status srx_layer_conv2d_mx4(int32_t dtype, const void* codes, const void* scales, const uint32_t sizes[4],
+                                const void* filterCodes, const void* filterScales, const uint32_t filterSizes[4],
+                                const void* bias, int32_t activation, void* out, void* stream) try
+{
+    srx::ML::Util util;
+    srx::ML::Operator op;
+    if (!codes || !scales || !sizes || !filterCodes || !filterScales || !filterSizes || !out || !utilFor(dtype, 1, util) ||
+        !util.CreateConvolutionMx4Layer(sizes, filterSizes, uint32_t(activation), op))
+        return fail(SRX_ERR_INVALID, "srx_layer_conv2d_mx4: bad pointer, data type, activation or sizes (filter depth must equal the input channels, sides <= 7)");
+    if (!aligned(out, dtype) || !aligned(bias, dtype) || (reinterpret_cast<uintptr_t>(codes) & 3) || (reinterpret_cast<uintptr_t>(filterCodes) & 3))
+        return fail(SRX_ERR_INVALID, "srx_layer_conv2d_mx4: a tensor is not aligned to its element type (codes: a multiple of 4)");
+    const OnDeviceOf scope(codes);
+    if (!scope.valid) return fail(SRX_ERR_INVALID, std::string("srx_layer_conv2d_mx4") + kNotOnDevice);
+    SRX_HIP(srx::LaunchConvMx4(op, static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales),
+                               static_cast<const uint8_t*>(filterCodes), static_cast<const uint8_t*>(filterScales), bias, out,
+                               static_cast<hipStream_t>(stream)));
+    return SRX_OK;
+}
+SRX_CATCH
+
+// ---------------------------------------------------------------------------
 // Frame pipe: pinned staging buffers and three streams around srx_upscale_frames.
 // ---------------------------------------------------------------------------
 struct srx_pipe

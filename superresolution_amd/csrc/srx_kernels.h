@@ -128,6 +128,20 @@ hipError_t LaunchImageToTensor(const Image& src, void* tensor, ML::TensorDataTyp
 hipError_t LaunchTensorToImage(const void* tensor, const Image& dst, ML::TensorDataType t, ML::TensorLayout layout,
                                int width, int height, int batch, hipStream_t s);
 
+// Group normalisation (srx_norm.hip): out (or codes and scales, the 4-bit block form) from dense channels-last tensors.
+// scale and bias may be null; the workspace holds GroupNormWorkspace(op) bytes.
+size_t GroupNormWorkspace(const ML::Operator& op);
+hipError_t LaunchGroupNorm(const ML::Operator& op, const void* in, const void* scale, const void* bias, void* out,
+                           uint8_t* codes, uint8_t* scales, void* workspace, hipStream_t s);
+// Rows of `columns` values to and from the 4-bit block form (srx_norm.hip).
+hipError_t LaunchQuantizeMx4(ML::TensorDataType t, const void* in, int64_t rows, int64_t columns, uint8_t* codes,
+                             uint8_t* scales, hipStream_t s);
+hipError_t LaunchDequantizeMx4(ML::TensorDataType t, const uint8_t* codes, const uint8_t* scales, int64_t rows,
+                               int64_t columns, void* out, hipStream_t s);
+// Convolution of an input and a filter in the 4-bit block form (srx_conv_mx4.hip); bias may be null.
+hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uint8_t* scales, const uint8_t* filterCodes,
+                         const uint8_t* filterScales, const void* bias, void* out, hipStream_t s);
+
 constexpr int kTileW = 32;   // output pixels per MFMA column tile
 constexpr int kTileH = 8;    // output rows per workgroup tile
 

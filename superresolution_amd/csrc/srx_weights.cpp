@@ -86,6 +86,9 @@ bool validSizes(const uint32_t sizes[4])
            uint64_t(sizes[0]) * sizes[1] * sizes[2] * sizes[3] < (uint64_t(1) << 40);
 }
 
+// Channels of the normalisation and 4-bit layers: their kernels count channels and blocks in 32 bits.
+constexpr uint32_t kMaxChannels = 1u << 20;
+
 }  // namespace
 
 bool Util::CreateUpsampleLayer(const uint32_t inputSizes[4], uint64_t& inputBufferRequiredSize,
@@ -153,6 +156,38 @@ bool Util::CreateAdditionLayer(const uint32_t inputSizes[4], Operator& opOut) co
     opOut.dataType = m_dataType;
     opOut.layout = m_layout;
     for (int i = 0; i < 4; ++i) opOut.inputSizes[i] = opOut.outputSizes[i] = inputSizes[i];
+    return true;
+}
+
+bool Util::CreateGroupNormLayer(const uint32_t inputSizes[4], uint32_t groups, float epsilon, uint32_t activation,
+                                Operator& opOut) const
+{
+    if (!validSizes(inputSizes) || m_dataType == TensorDataType::UNKNOWN || m_layout != TensorLayout::NHWC) return false;
+    if (groups == 0 || inputSizes[1] % groups != 0 || inputSizes[1] > kMaxChannels) return false;
+    if (!(epsilon > 0.0f) || !std::isfinite(epsilon) || activation > uint32_t(Activation::SILU)) return false;
+    opOut = Operator{};
+    opOut.kind = Operator::Kind::GROUP_NORM;
+    opOut.dataType = m_dataType;
+    opOut.layout = m_layout;
+    opOut.groups = groups;
+    opOut.epsilon = epsilon;
+    opOut.activation = Activation(activation);
+    for (int i = 0; i < 4; ++i) opOut.inputSizes[i] = opOut.outputSizes[i] = inputSizes[i];
+    return true;
+}
+
+bool Util::CreateConvolutionMx4Layer(const uint32_t inputSizes[4], const uint32_t* filterSizes, uint32_t activation,
+                                     Operator& opOut) const
+{
+    uint64_t ib = 0, ob = 0;
+    uint32_t os[4];
+    if (m_layout != TensorLayout::NHWC || activation > uint32_t(Activation::SILU)) return false;
+    if (!CreateConvolutionLayer(inputSizes, filterSizes, false, ib, ob, os, opOut)) return false;
+    if (filterSizes[2] > 7 || filterSizes[3] > 7 || inputSizes[1] > kMaxChannels || filterSizes[0] > kMaxChannels) return false;
+    if (uint64_t(inputSizes[0]) * inputSizes[2] * inputSizes[3] > uint64_t(INT32_MAX)) return false;
+    if (!validSizes(os)) return false;
+    opOut.kind = Operator::Kind::CONVOLUTION_MX4;
+    opOut.activation = Activation(activation);
     return true;
 }
 

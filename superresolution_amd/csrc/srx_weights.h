@@ -32,12 +32,13 @@ float Float16ToFloat32(uint16_t h);
 uint16_t Float32ToFloat16(float v);
 
 enum class InterpolationType : uint32_t { NEAREST_NEIGHBOR, LINEAR };   // XUSGMachineLearning.h:177-181
+enum class Activation : uint32_t { NONE, RELU, SILU };
 
 // What a layer factory returns: the counterpart of the reference's compiled DirectML operator
 // (XUSG::ML::Operator), reduced to the description a kernel launch needs.  Sizes are {N, C, H, W}.
 struct Operator
 {
-    enum class Kind : uint32_t { NONE, UPSAMPLE_2D, CONVOLUTION, ELEMENT_WISE_ADD };
+    enum class Kind : uint32_t { NONE, UPSAMPLE_2D, CONVOLUTION, ELEMENT_WISE_ADD, GROUP_NORM, CONVOLUTION_MX4 };
     Kind kind = Kind::NONE;
     TensorDataType dataType = TensorDataType::FLOAT16;
     TensorLayout layout = TensorLayout::DEFAULT;
@@ -47,6 +48,9 @@ struct Operator
     bool useBiasAndActivation = false;             // bias + fused ReLU
     uint32_t scaleX = 1, scaleY = 1;
     InterpolationType interpolation = InterpolationType::NEAREST_NEIGHBOR;
+    Activation activation = Activation::NONE;      // GROUP_NORM, CONVOLUTION_MX4
+    uint32_t groups = 1;                           // GROUP_NORM
+    float epsilon = 0.0f;
 };
 
 class Util
@@ -80,6 +84,14 @@ public:
                                 uint64_t& inputBufferRequiredSize, uint64_t& outputBufferRequiredSize,
                                 uint32_t outputSizes[4], Operator& opOut) const;
     bool CreateAdditionLayer(const uint32_t inputSizes[4], Operator& opOut) const;
+    // No counterparts in the reference.  Both take channels-last tensors only (the NHWC layout).  Group normalisation:
+    // `groups` must divide the channels, epsilon must be positive and finite.  Convolution of an input and a filter in
+    // the 4-bit block form: sizes and padding as in CreateConvolutionLayer, filter sides up to 7, the output in the
+    // tensor data type; at most 2^31 - 1 pixels in all.
+    bool CreateGroupNormLayer(const uint32_t inputSizes[4], uint32_t groups, float epsilon, uint32_t activation,
+                              Operator& opOut) const;
+    bool CreateConvolutionMx4Layer(const uint32_t inputSizes[4], const uint32_t* filterSizes, uint32_t activation,
+                                   Operator& opOut) const;
 
     TensorDataType GetDataType() const { return m_dataType; }
     TensorLayout GetLayout() const { return m_layout; }
