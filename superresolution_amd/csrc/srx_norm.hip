@@ -17,21 +17,48 @@ namespace {
 
 constexpr int kVec = 8;               // channels of one thread
 constexpr int kTileC = kThreads * kVec;
+constexpr int kJoin = 16;             // parts of an image that every workgroup of NormApplyKernel joins by itself
 
 struct NormArgs
 {
     const void *in, *scale, *bias;
     void* out;
     uint8_t *codes, *scales;
-    float2* partial;                  // [N][chunks][G] (mean, M2)
+    float2* partial;                  // [N][G][chunks] (mean, M2)
+    float2* joined;                   // [N][G] (mean, 1 / deviation), where chunks > kJoin
     int64_t pixels;                   // H * W
     int C, G, groupC;                 // channels, groups, channels of a group
     int chunks, chunkPixels;          // statistics: parts of an image
-    int tileGroups, tiles;            // statistics: whole groups per workgroup
+    int tileGroups, tiles;            // whole groups per workgroup (statistics, slabs)
     int applyChunks, applyPixels, applyTiles;
+    int groupsInAll;                  // N * G
     float epsilon;
     int activation;
 };
+
+// Eight values as they are held in memory: registers that wait for the statistics take half the room in fp16.
+template <typename T> struct Held;
+template <> struct Held<f16>
+{
+    f16x8 v;
+    __device__ void load(const f16* p) { __builtin_memcpy(&v, p, 16); }
+    __device__ void set(int i, float x) { v[i] = (f16)x; }
+    __device__ float get(int i) const { return (float)v[i]; }
+};
+template <> struct Held<float>
+{
+    f32x4 a, b;
+    __device__ void load(const float* p) { __builtin_memcpy(&a, p, 16); __builtin_memcpy(&b, p + 4, 16); }
+    __device__ void set(int i, float x) { if (i < 4) a[i & 3] = x; else b[i & 3] = x; }
+    __device__ float get(int i) const { return i < 4 ? a[i & 3] : b[i & 3]; }
+};
+template <typename T>
+__device__ __forceinline__ void loadHeld(const T* p, int count, Held<T>& v)
+{
+    if (count >= kVec) { v.load(p); return; }
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) v.set(i, i < count ? (float)p[i] : 0.0f);
+}
 
 // Sum over the `lanes` (a power of two up to 64) lanes of an aligned part of a wave.
 __device__ __forceinline__ float sumLanes(float v, int lanes)
@@ -40,12 +67,175 @@ __device__ __forceinline__ float sumLanes(float v, int lanes)
     return v;
 }
 
-// Threads that share one group's reduction when a workgroup reduces `groups` of them.
-__device__ __forceinline__ int lanesPerGroup(int groups)
+// Sum of squared deviations from sums about another point: rounding may leave it below zero, a NaN stays one.
+__device__ __forceinline__ float spread(float squares, float sum, float inverseCount)
+{
+    const float m2 = squares - sum * sum * inverseCount;
+    return m2 < 0.0f ? 0.0f : m2;
+}
+
+// Threads that share one group's reduction when `threads` of them reduce `groups` groups.
+__device__ __forceinline__ int lanesPerGroup(int groups, int threads)
 {
     int lanes = 64;
-    while (lanes > 1 && lanes * groups > kThreads) lanes >>= 1;
+    while (lanes > 1 && lanes * groups > threads) lanes >>= 1;
     return lanes;
+}
+
+// What a thread needs to finish its eight channels, and the finish.
+template <typename T>
+struct Finish
+{
+    float mean[kVec], mul[kVec], add[kVec];
+    // channels c ..; stat: (mean, 1 / deviation) of group g0 and the following ones
+    __device__ __forceinline__ void prepare(const NormArgs& a, const float2* stat, int g0, int c)
+    {
+        int g = min(c, a.C - 1) / a.groupC, left = (g + 1) * a.groupC - c;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i)
+        {
+            const int ci = min(c + i, a.C - 1);
+            if (i == left && c + i < a.C) { ++g; left += a.groupC; }
+            const float2 st = stat[g - g0];
+            mean[i] = st.x;
+            mul[i] = st.y * (a.scale ? (float)static_cast<const T*>(a.scale)[ci] : 1.0f);
+            add[i] = a.bias ? (float)static_cast<const T*>(a.bias)[ci] : 0.0f;
+        }
+    }
+    // m channels exist; `pixel` counts over all images, `column` is the thread's place among the pixel's eighths of blocks
+    template <bool MX4>
+    __device__ __forceinline__ void store(const NormArgs& a, const Held<T>& x, int m, int c, int64_t pixel) const
+    {
+        float v[kVec];
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) v[i] = activate(fmaf(x.get(i) - mean[i], mul[i], add[i]), a.activation);
+        if (MX4)
+        {
+            if (m < kVec)
+            {
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) v[i] = i < m ? v[i] : 0.0f;
+            }
+            unsigned scale;
+            const unsigned codes = mxQuantise(v, scale);
+            const int64_t block = pixel * mxBlocks(a.C) + (c >> 5);
+            *reinterpret_cast<unsigned*>(a.codes + block * kMxBytes + ((c >> 1) & 12)) = codes;
+            if ((c & 24) == 0) a.scales[block] = uint8_t(scale);
+        }
+        else storeUpTo8(static_cast<T*>(a.out) + pixel * a.C + c, m, v);
+    }
+};
+
+// Threads of a row of `channels` channels; whole blocks of 32 take four threads each.
+template <bool MX4>
+__host__ __device__ __forceinline__ int vecsFor(int channels)
+{
+    return MX4 ? ((channels + 31) >> 5) << 2 : (channels + kVec - 1) / kVec;
+}
+
+// Small images: one workgroup holds a slab, all pixels of a range of whole groups of one image, in registers (R eighths
+// a thread), takes mean and variance one after the other, and stores.  One launch, one trip to memory.
+template <typename T, bool MX4, int THREADS, int R>
+__global__ __launch_bounds__(THREADS) void NormSlabKernel(const NormArgs a)
+{
+    __shared__ float sPart[THREADS * kVec];
+    __shared__ float2 sStat[THREADS * kVec];
+    const int tid = threadIdx.x, tile = blockIdx.x % a.tiles, n = blockIdx.x / a.tiles;
+    const int g0 = tile * a.tileGroups, groups = min(a.tileGroups, a.G - g0);
+    const int c0 = g0 * a.groupC, tileC = groups * a.groupC;
+    const int vecs = vecsFor<MX4>(tileC), rows = THREADS / vecs, row = tid / vecs, col = tid - row * vecs;
+    const int m = row < rows ? max(0, min(kVec, tileC - col * kVec)) : 0;
+    const int c = c0 + col * kVec, pixels = int(a.pixels);
+    const T* in = static_cast<const T*>(a.in) + int64_t(n) * pixels * a.C + c;
+    Held<T> x[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+        if (row + i * rows < pixels) loadHeld(in + int64_t(row + i * rows) * a.C, m, x[i]);
+
+    const int lanes = lanesPerGroup(groups, THREADS), lane = tid & (lanes - 1);
+    const float inv = 1.0f / (float(pixels) * float(a.groupC));
+    // Where a group is whole eighths, a thread adds up its eight channels first.
+    const int per = a.groupC % kVec == 0 ? 1 : kVec;
+    const int rowValues = vecs * per, groupValues = per == 1 ? a.groupC / kVec : a.groupC;
+    const auto reduce = [&](int g) -> float {
+        // every thread's values are in sPart; this thread's lane group adds up those of group g
+        float sum = 0.0f;
+        int r = lane / groupValues, k = lane - r * groupValues;
+        const int dr = lanes / groupValues, dk = lanes - dr * groupValues;
+        while (r < rows)
+        {
+            sum += sPart[r * rowValues + g * groupValues + k];
+            k += dk;
+            r += dr;
+            if (k >= groupValues) { k -= groupValues; ++r; }
+        }
+        return sumLanes(sum, lanes);
+    };
+    const auto publish = [&](const float (&v)[kVec]) {
+        if (row >= rows) return;
+        if (per == 1)
+            sPart[tid] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        else
+        {
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) sPart[tid * kVec + i] = v[i];
+        }
+    };
+    float s[kVec];
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) s[k] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+        if (row + i * rows < pixels)
+        {
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) s[k] += k < m ? x[i].get(k) : 0.0f;
+        }
+    publish(s);
+    __syncthreads();
+    for (int g = tid / lanes; g < groups; g += THREADS / lanes)
+    {
+        const float sum = reduce(g);
+        if (lane == 0) sStat[g].x = sum * inv;
+    }
+    __syncthreads();
+    Finish<T> f;
+    if (m > 0)
+    {
+        int g = (col * kVec) / a.groupC, left = (g + 1) * a.groupC - col * kVec;
+#pragma unroll
+        for (int k = 0; k < kVec; ++k)
+        {
+            if (k == left && k < m) { ++g; left += a.groupC; }
+            f.mean[k] = sStat[g].x;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) s[k] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+        if (row + i * rows < pixels)
+        {
+#pragma unroll
+            for (int k = 0; k < kVec; ++k)
+            {
+                const float d = k < m ? x[i].get(k) - f.mean[k] : 0.0f;
+                s[k] = fmaf(d, d, s[k]);
+            }
+        }
+    publish(s);
+    __syncthreads();
+    for (int g = tid / lanes; g < groups; g += THREADS / lanes)
+    {
+        const float sum = reduce(g);
+        if (lane == 0) sStat[g].y = 1.0f / sqrtf(fmaf(sum, inv, a.epsilon));
+    }
+    __syncthreads();
+    if (row >= rows) return;
+    f.prepare(a, sStat, g0, c);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+        if (row + i * rows < pixels) f.template store<MX4>(a, x[i], m, c, int64_t(n) * pixels + row + i * rows);
 }
 
 // Statistics of one part of one image for a range of whole groups.  A thread keeps eight channels and walks the
@@ -62,7 +252,7 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
     const int64_t p0 = int64_t(chunk) * a.chunkPixels;
     const int count = int(min(int64_t(a.chunkPixels), a.pixels - p0));
     const T* in = static_cast<const T*>(a.in) + (n * a.pixels + p0) * a.C + c0;
-    float2* out = a.partial + (int64_t(n) * a.chunks + chunk) * a.G + g0;
+    float2* out = a.partial + (int64_t(n) * a.G + g0) * a.chunks + chunk;
     const int tid = threadIdx.x, vecs = (tileC + kVec - 1) / kVec;
 
     if (vecs > kThreads)
@@ -83,7 +273,7 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
                     if (i < m) { const float d = v[i] - k; s += d; q = fmaf(d, d, q); }
             }
         const float cnt = float(have), total = float(count) * float(tileC);
-        const float mean = have ? k + s / cnt : 0.0f, m2 = have ? fmaxf(q - s * s / cnt, 0.0f) : 0.0f;
+        const float mean = have ? k + s / cnt : 0.0f, m2 = have ? spread(q, s, 1.0f / cnt) : 0.0f;
         sMean[tid] = cnt * mean;
         __syncthreads();
         float all = 0.0f;
@@ -110,20 +300,39 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
 #pragma unroll
         for (int i = 0; i < kVec; ++i) k[i] = s[i] = q[i] = 0.0f;
         if (row < count) loadUpTo8(src + int64_t(row) * a.C, m, k);
-#pragma unroll 4
-        for (int p = row + rows; p < count; p += rows)
+        int p = row + rows;
+        // four loads in flight
+        for (; p + 3 * rows < count; p += 4 * rows)
         {
-            float v[kVec];
-            loadUpTo8(src + int64_t(p) * a.C, m, v);
+            Held<T> v[4];
+            if (m == kVec)
+            {
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) { const float d = v[i] - k[i]; s[i] += d; q[i] = fmaf(d, d, q[i]); }
+                for (int u = 0; u < 4; ++u) v[u].load(src + int64_t(p + u * rows) * a.C);
+            }
+            else
+            {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) loadHeld(src + int64_t(p + u * rows) * a.C, m, v[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) { const float d = v[u].get(i) - k[i]; s[i] += d; q[i] = fmaf(d, d, q[i]); }
+        }
+        for (; p < count; p += rows)
+        {
+            Held<T> v;
+            loadHeld(src + int64_t(p) * a.C, m, v);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) { const float d = v.get(i) - k[i]; s[i] += d; q[i] = fmaf(d, d, q[i]); }
         }
         const float inv = 1.0f / float(max(1, (count - row + rows - 1) / rows));
 #pragma unroll
         for (int i = 0; i < kVec; ++i)
         {
             sMean[(row * vecs + col) * kVec + i] = fmaf(s[i], inv, k[i]);
-            sM2[(row * vecs + col) * kVec + i] = fmaxf(q[i] - s[i] * s[i] * inv, 0.0f);
+            sM2[(row * vecs + col) * kVec + i] = spread(q[i], s[i], inv);
         }
     }
     __syncthreads();
@@ -144,7 +353,7 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
     }
     __syncthreads();
     // join the channels of each group: equal counts
-    const int lanes = lanesPerGroup(groups), lane = tid & (lanes - 1);
+    const int lanes = lanesPerGroup(groups, kThreads), lane = tid & (lanes - 1);
     for (int g = tid / lanes; g < groups; g += kThreads / lanes)
     {
         float mean = 0.0f, m2 = 0.0f;
@@ -156,17 +365,43 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
             m2 += sM2[g * a.groupC + c] + float(count) * d * d;
         }
         m2 = sumLanes(m2, lanes);
-        if (lane == 0) out[g] = float2{mean, m2};
+        if (lane == 0) out[int64_t(g) * a.chunks] = float2{mean, m2};
     }
 }
 
-// Normalises, scales, activates and stores (MX4: as 4-bit blocks) a part of an image; the parts' statistics are
-// joined by every workgroup for the groups it needs.
+// The parts of one group of one image joined by `lanes` lanes: (mean, 1 / deviation).
+__device__ __forceinline__ float2 joinParts(const NormArgs& a, const float2* partial, int lane, int lanes)
+{
+    const float lastPixels = float(a.pixels - int64_t(a.chunks - 1) * a.chunkPixels);
+    float mean = 0.0f, m2 = 0.0f;
+    for (int k = lane; k < a.chunks; k += lanes) mean += (k == a.chunks - 1 ? lastPixels : float(a.chunkPixels)) * partial[k].x;
+    mean = sumLanes(mean, lanes) / float(a.pixels);
+    for (int k = lane; k < a.chunks; k += lanes)
+    {
+        const float2 v = partial[k];
+        const float d = v.x - mean;
+        m2 += v.y + (k == a.chunks - 1 ? lastPixels : float(a.chunkPixels)) * float(a.groupC) * d * d;
+    }
+    m2 = sumLanes(m2, lanes);
+    return float2{mean, 1.0f / sqrtf(m2 / (float(a.pixels) * float(a.groupC)) + a.epsilon)};
+}
+
+// One wave joins the parts of one group.
+__global__ __launch_bounds__(kThreads) void NormJoinKernel(const NormArgs a)
+{
+    const int group = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+    if (group >= a.groupsInAll) return;
+    const float2 v = joinParts(a, a.partial + int64_t(group) * a.chunks, threadIdx.x & 63, 64);
+    if ((threadIdx.x & 63) == 0) a.joined[group] = v;
+}
+
+// Normalises, scales, activates and stores (MX4: as 4-bit blocks) a part of an image.
 template <typename T, bool MX4>
 __global__ __launch_bounds__(kThreads) void NormApplyKernel(const NormArgs a)
 {
     __shared__ float2 sStat[kTileC];
-    int b = blockIdx.x;
+    // from the last part to the first: the statistics kernel read the last ones last, so they are still cached
+    int b = gridDim.x - 1 - blockIdx.x;
     const int tile = b % a.applyTiles; b /= a.applyTiles;
     const int chunk = b % a.applyChunks, n = b / a.applyChunks;
     const int c0 = tile * kTileC, tileC = min(kTileC, a.C - c0);
@@ -175,63 +410,42 @@ __global__ __launch_bounds__(kThreads) void NormApplyKernel(const NormArgs a)
     const int count = int(min(int64_t(a.applyPixels), a.pixels - p0));
     const int tid = threadIdx.x;
 
+    const int vecs = vecsFor<MX4>(tileC), rows = kThreads / vecs, row = tid / vecs, col = tid - row * vecs;
+    const int m = row < rows ? max(0, min(kVec, tileC - col * kVec)) : 0, c = c0 + col * kVec;
+    const T* in = static_cast<const T*>(a.in) + (n * a.pixels + p0) * a.C + c;
+    constexpr int kFlight = 4;
+    Held<T> x[kFlight];
+    // the first loads do not wait for the statistics
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u)
+        if (row + u * rows < count) loadHeld(in + int64_t(row + u * rows) * a.C, m, x[u]);
+
+    if (a.chunks > kJoin)
     {
-        const int lanes = lanesPerGroup(groups), lane = tid & (lanes - 1);
-        const float2* partial = a.partial + int64_t(n) * a.chunks * a.G + g0;
-        const float lastPixels = float(a.pixels - int64_t(a.chunks - 1) * a.chunkPixels);
-        for (int g = tid / lanes; g < groups; g += kThreads / lanes)
+        for (int g = tid; g < groups; g += kThreads) sStat[g] = a.joined[int64_t(n) * a.G + g0 + g];
+    }
+    else
+    {
+        const int lane = tid & (kJoin - 1);
+        for (int g = tid / kJoin; g < groups; g += kThreads / kJoin)
         {
-            float mean = 0.0f, m2 = 0.0f;
-            for (int k = lane; k < a.chunks; k += lanes)
-                mean += (k == a.chunks - 1 ? lastPixels : float(a.chunkPixels)) * partial[int64_t(k) * a.G + g].x;
-            mean = sumLanes(mean, lanes) / float(a.pixels);
-            for (int k = lane; k < a.chunks; k += lanes)
-            {
-                const float2 v = partial[int64_t(k) * a.G + g];
-                const float d = v.x - mean;
-                m2 += v.y + (k == a.chunks - 1 ? lastPixels : float(a.chunkPixels)) * float(a.groupC) * d * d;
-            }
-            m2 = sumLanes(m2, lanes);
-            if (lane == 0) sStat[g] = float2{mean, 1.0f / sqrtf(m2 / (float(a.pixels) * float(a.groupC)) + a.epsilon)};
+            const float2 v = joinParts(a, a.partial + (int64_t(n) * a.G + g0 + g) * a.chunks, lane, kJoin);
+            if (lane == 0) sStat[g] = v;
         }
     }
     __syncthreads();
-
-    int vecs = (tileC + kVec - 1) / kVec;
-    if (MX4) vecs = (vecs + 3) & ~3;                    // whole blocks: four threads each
-    const int rows = kThreads / vecs, row = tid / vecs, col = tid - row * vecs;
     if (row >= rows) return;
-    const int m = max(0, min(kVec, tileC - col * kVec)), c = c0 + col * kVec;
-    float mean[kVec], mul[kVec], add[kVec];
-#pragma unroll
-    for (int i = 0; i < kVec; ++i)
+    Finish<T> f;
+    f.prepare(a, sStat, g0, c);
+    const int64_t pixel0 = n * a.pixels + p0;
+    for (int p = row; p < count; p += kFlight * rows)
     {
-        const int ci = min(c + i, a.C - 1);
-        const float2 st = sStat[ci / a.groupC - g0];
-        mean[i] = st.x;
-        mul[i] = st.y * (a.scale ? (float)static_cast<const T*>(a.scale)[ci] : 1.0f);
-        add[i] = a.bias ? (float)static_cast<const T*>(a.bias)[ci] : 0.0f;
-    }
-    const T* in = static_cast<const T*>(a.in) + (n * a.pixels + p0) * a.C + c;
-    const int64_t blocks = mxBlocks(a.C);
-    for (int p = row; p < count; p += rows)
-    {
-        float v[kVec];
-        loadUpTo8(in + int64_t(p) * a.C, m, v);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) v[i] = activate(fmaf(v[i] - mean[i], mul[i], add[i]), a.activation);
-        const int64_t pixel = n * a.pixels + p0 + p;
-        if (MX4)
-        {
+        for (int u = 0; u < kFlight; ++u)
+            if (p + u * rows < count) f.template store<MX4>(a, x[u], m, c, pixel0 + p + u * rows);
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) v[i] = i < m ? v[i] : 0.0f;
-            unsigned scale;
-            const unsigned codes = mxQuantise(v, scale);
-            const int64_t block = pixel * blocks + (c >> 5);
-            *reinterpret_cast<unsigned*>(a.codes + block * kMxBytes + (col & 3) * 4) = codes;
-            if ((col & 3) == 0) a.scales[block] = uint8_t(scale);
-        }
-        else storeUpTo8(static_cast<T*>(a.out) + pixel * a.C + c, m, v);
+        for (int u = 0; u < kFlight; ++u)
+            if (p + (kFlight + u) * rows < count) loadHeld(in + int64_t(p + (kFlight + u) * rows) * a.C, m, x[u]);
     }
 }
 
@@ -295,16 +509,53 @@ __global__ __launch_bounds__(kThreads) void DequantizeKernel(const MxArgs a)
     }
 }
 
-// How a normalisation is cut into workgroups.
-void planNorm(const ML::Operator& op, NormArgs& a)
+// How a normalisation is cut into workgroups.  Slabs (NormSlabKernel) where all pixels of the fewest whole groups fit
+// one workgroup's registers; otherwise parts of images.
+struct NormPlan
 {
+    NormArgs a{};
+    int slabThreads = 0, slabHeld = 0;     // 0: no slabs
+    int64_t images = 0;
+};
+
+NormPlan planNorm(const ML::Operator& op, bool mx4)
+{
+    NormPlan p;
+    NormArgs& a = p.a;
     a.C = int(op.inputSizes[1]);
     a.G = int(op.groups);
     a.groupC = a.C / a.G;
     a.pixels = int64_t(op.inputSizes[2]) * op.inputSizes[3];
+    a.epsilon = op.epsilon;
+    a.activation = int(op.activation);
+    p.images = op.inputSizes[0];
+    const int64_t n = p.images;
+    a.groupsInAll = int(n * a.G < INT32_MAX ? n * a.G : INT32_MAX);
+
+    // slabs: the fewest groups that are a whole number of 64-byte lines (of blocks of 32 channels)
+    const int unit = mx4 || op.dataType == ML::TensorDataType::FLOAT16 ? 32 : 16;
+    int groups = 1;
+    while (groups < a.G && (groups * a.groupC) % unit != 0) ++groups;
+    if (a.pixels <= 1 << 20 && (!mx4 || groups == a.G || (groups * a.groupC) % 32 == 0))
+    {
+        const int64_t vecs = mx4 ? vecsFor<true>(groups * a.groupC) : vecsFor<false>(groups * a.groupC);
+        const int most = op.dataType == ML::TensorDataType::FLOAT16 ? 16 : 8;
+        for (const int threads : {256, 1024})
+        {
+            if (vecs > threads) continue;
+            const int64_t rows = threads / vecs, held = (a.pixels + rows - 1) / rows;
+            if (held > (threads == 256 ? 4 : most)) continue;
+            p.slabThreads = threads;
+            p.slabHeld = int(held);
+            a.tileGroups = groups;
+            a.tiles = (a.G + groups - 1) / groups;
+            if (n * a.tiles <= INT32_MAX) return p;
+        }
+    }
+    p.slabThreads = 0;
+
     a.tileGroups = a.groupC >= kTileC ? 1 : (kTileC / a.groupC < a.G ? kTileC / a.groupC : a.G);
     a.tiles = (a.G + a.tileGroups - 1) / a.tileGroups;
-    const int64_t n = op.inputSizes[0];
     // enough parts for the whole device, no part below 16 pixels
     int64_t chunks = (1024 + n * a.tiles - 1) / (n * a.tiles);
     const int64_t most = (a.pixels + 15) / 16;
@@ -318,24 +569,58 @@ void planNorm(const ML::Operator& op, NormArgs& a)
     if (parts < a.chunks) parts = a.chunks;
     a.applyPixels = int((a.pixels + parts - 1) / parts);
     a.applyChunks = int((a.pixels + a.applyPixels - 1) / a.applyPixels);
-    a.epsilon = op.epsilon;
-    a.activation = int(op.activation);
+    return p;
+}
+
+size_t normWorkspace(const NormPlan& p)
+{
+    if (p.slabThreads) return 0;
+    return size_t(p.images) * p.a.G * (p.a.chunks + (p.a.chunks > kJoin ? 1 : 0)) * sizeof(float2);
+}
+
+template <typename T, bool MX4>
+hipError_t launchNorm(const NormPlan& p, hipStream_t s)
+{
+    const NormArgs& a = p.a;
+    if (p.slabThreads)
+    {
+        const dim3 grid(static_cast<unsigned>(p.images * a.tiles));
+        constexpr bool kHalf = sizeof(T) == 2;
+        if (p.slabThreads == 256 && p.slabHeld == 1) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 256, 1>), grid, dim3(256), 0, s, a);
+        else if (p.slabThreads == 256) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 256, 4>), grid, dim3(256), 0, s, a);
+        else if (p.slabHeld <= 4) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 1024, 4>), grid, dim3(1024), 0, s, a);
+        else if (p.slabHeld <= 8) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 1024, 8>), grid, dim3(1024), 0, s, a);
+        else if constexpr (kHalf) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 1024, 16>), grid, dim3(1024), 0, s, a);
+        return hipGetLastError();
+    }
+    const int64_t statsGrid = p.images * a.chunks * a.tiles, applyGrid = p.images * a.applyChunks * a.applyTiles;
+    if (statsGrid > INT32_MAX || applyGrid > INT32_MAX || p.images * a.G > INT32_MAX) return hipErrorInvalidValue;
+    const dim3 block(kThreads);
+    hipLaunchKernelGGL(NormStatsKernel<T>, dim3(unsigned(statsGrid)), block, 0, s, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (a.chunks > kJoin)
+    {
+        hipLaunchKernelGGL(NormJoinKernel, dim3(unsigned((a.groupsInAll + 3) / 4)), block, 0, s, a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL((NormApplyKernel<T, MX4>), dim3(unsigned(applyGrid)), block, 0, s, a);
+    return hipGetLastError();
 }
 
 }  // namespace
 
 size_t GroupNormWorkspace(const ML::Operator& op)
 {
-    NormArgs a{};
-    planNorm(op, a);
-    return size_t(op.inputSizes[0]) * a.chunks * a.G * sizeof(float2);
+    const size_t plain = normWorkspace(planNorm(op, false)), mx4 = normWorkspace(planNorm(op, true));
+    return plain > mx4 ? plain : mx4;
 }
 
 hipError_t LaunchGroupNorm(const ML::Operator& op, const void* in, const void* scale, const void* bias, void* out,
                            uint8_t* codes, uint8_t* scales, void* workspace, hipStream_t s)
 {
-    NormArgs a{};
-    planNorm(op, a);
+    NormPlan p = planNorm(op, codes != nullptr);
+    NormArgs& a = p.a;
     a.in = in;
     a.scale = scale;
     a.bias = bias;
@@ -343,20 +628,10 @@ hipError_t LaunchGroupNorm(const ML::Operator& op, const void* in, const void* s
     a.codes = codes;
     a.scales = scales;
     a.partial = static_cast<float2*>(workspace);
-    const int64_t n = op.inputSizes[0];
-    const int64_t statsGrid = n * a.chunks * a.tiles, applyGrid = n * a.applyChunks * a.applyTiles;
-    if (statsGrid > INT32_MAX || applyGrid > INT32_MAX) return hipErrorInvalidValue;
-    const dim3 block(kThreads), g1(static_cast<unsigned>(statsGrid)), g2(static_cast<unsigned>(applyGrid));
+    a.joined = a.partial + size_t(p.images) * a.G * a.chunks;
     const bool half = op.dataType == ML::TensorDataType::FLOAT16;
-    if (half) hipLaunchKernelGGL(NormStatsKernel<f16>, g1, block, 0, s, a);
-    else hipLaunchKernelGGL(NormStatsKernel<float>, g1, block, 0, s, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    if (half && codes) hipLaunchKernelGGL((NormApplyKernel<f16, true>), g2, block, 0, s, a);
-    else if (half) hipLaunchKernelGGL((NormApplyKernel<f16, false>), g2, block, 0, s, a);
-    else if (codes) hipLaunchKernelGGL((NormApplyKernel<float, true>), g2, block, 0, s, a);
-    else hipLaunchKernelGGL((NormApplyKernel<float, false>), g2, block, 0, s, a);
-    return hipGetLastError();
+    if (half) return codes ? launchNorm<f16, true>(p, s) : launchNorm<f16, false>(p, s);
+    return codes ? launchNorm<float, true>(p, s) : launchNorm<float, false>(p, s);
 }
 
 namespace {

@@ -44,7 +44,7 @@ def test_block_form_arguments_refused():
     refused(S.layer_dequantize_mx4, 0, P, P, 1, 1, P + 1)
 
 
-def norm(dtype=0, x=P, sizes=(1, 8, 4, 4), groups=2, scale=P, bias=P, epsilon=1e-5, act=0, out=P, work=P, nbytes=1 << 20):
+def norm(dtype=0, x=P, sizes=(1, 8, 300, 200), groups=2, scale=P, bias=P, epsilon=1e-5, act=0, out=P, work=P, nbytes=1 << 20):
     return (dtype, x, sizes, groups, scale, bias, epsilon, act, out, work, nbytes)
 
 
@@ -96,5 +96,5 @@ def test_host_memory_is_refused():
     assert "not device memory" in refused(S.layer_quantize_mx4, 0, p, 1, 32, p + 1024, p + 2048)
     assert "not device memory" in refused(S.layer_dequantize_mx4, 0, p, p + 1024, 1, 32, p + 2048)
     need = S.layer_group_norm_workspace(0, (1, 8, 4, 4), 2)
-    assert "not device memory" in refused(S.layer_group_norm, *norm(x=p, out=p, scale=None, bias=None, work=p + 2048, nbytes=need))
+    assert "not device memory" in refused(S.layer_group_norm, *norm(x=p, sizes=(1, 8, 4, 4), out=p, scale=None, bias=None, work=p + 2048, nbytes=need))
     assert "not device memory" in refused(S.layer_conv2d_mx4, *conv(codes=p, scales=p, fc=p, fs=p, bias=None, out=p))
