@@ -318,12 +318,15 @@ srx_status srx_layer_add(int32_t dtype, const void* a, const void* b, void* out,
  *
  *   - The first pointer of a call must be device memory; the call runs on the GPU that holds it, whichever is
  *     current, and `stream` must belong to that GPU (NULL = its default stream).  All other pointers must be memory
- *     that GPU can reach.  Tensors need the alignment of their element type only; sizes may be odd.
+ *     that GPU can reach.  Codes must lie at a multiple of 16 bytes; scales may lie anywhere (those of tensors whose
+ *     blocks come in fours are read faster from a multiple of 4), other tensors at a multiple of their element.
+ *     Sizes may be odd.
  *   - Nothing is allocated and nothing is kept between calls: every call may be captured into a HIP graph, and calls
  *     may overlap on different streams as long as their outputs and workspaces are different memory.
  *   - Results do not depend on what runs beside a call: no atomics, fixed orders of summation.
  *   - A call that is refused (SRX_ERR_INVALID) has launched nothing.  Sizes of zero are refused.
- *   - At most 2^20 channels and filters; N*H*W at most 2^31 - 1 in srx_layer_conv2d_mx4.
+ *   - At most 2^20 channels and filters; in srx_layer_conv2d_mx4 N*H*W is at most 2^31 - 1 and kh * kw * ceil(C / 32)
+ *     below 2^19.
  *
  * Activations: 0 = none, 1 = ReLU, 2 = SiLU, y / (1 + exp(-y)).
  *

@@ -1146,7 +1146,7 @@ srx_status groupNorm(const char* who, int32_t dtype, const void* in, const uint3
         return fail(SRX_ERR_INVALID, std::string(who) + ": bad pointer, data type, sizes, groups (a divisor of the channels), epsilon (positive) or activation");
     if (!aligned(in, dtype) || !aligned(scale, dtype) || !aligned(bias, dtype) || !aligned(out, dtype))
         return fail(SRX_ERR_INVALID, std::string(who) + ": a tensor is not aligned to its element type");
-    if (reinterpret_cast<uintptr_t>(codes) & 3) return fail(SRX_ERR_INVALID, std::string(who) + ": codes must be a multiple of 4");
+    if (reinterpret_cast<uintptr_t>(codes) & 15) return fail(SRX_ERR_INVALID, std::string(who) + ": codes must be a multiple of 16");
     const size_t need = srx::GroupNormWorkspace(op);
     if (need && (!workspace || workspaceBytes < need || (reinterpret_cast<uintptr_t>(workspace) & 7)))
         return fail(SRX_ERR_INVALID, std::string(who) + ": the workspace must hold " + std::to_string(need) + " bytes (a multiple of 8)");
@@ -1173,8 +1173,8 @@ srx_status srx_layer_quantize_mx4(int32_t dtype, const void* in, uint64_t rows, 
 {
     srx::ML::Util util;
     if (!in || !codes || !scales || !utilFor(dtype, 1, util) || !validMx4(rows, columns) || !aligned(in, dtype) ||
-        (reinterpret_cast<uintptr_t>(codes) & 3))
-        return fail(SRX_ERR_INVALID, "srx_layer_quantize_mx4: bad pointer (codes: a multiple of 4), data type or sizes");
+        (reinterpret_cast<uintptr_t>(codes) & 15))
+        return fail(SRX_ERR_INVALID, "srx_layer_quantize_mx4: bad pointer (codes: a multiple of 16), data type or sizes");
     const OnDeviceOf scope(in);
     if (!scope.valid) return fail(SRX_ERR_INVALID, std::string("srx_layer_quantize_mx4") + kNotOnDevice);
     SRX_HIP(srx::LaunchQuantizeMx4(util.GetDataType(), in, int64_t(rows), int64_t(columns), static_cast<uint8_t*>(codes),
@@ -1188,8 +1188,8 @@ srx_status srx_layer_dequantize_mx4(int32_t dtype, const void* codes, const void
 {
     srx::ML::Util util;
     if (!codes || !scales || !out || !utilFor(dtype, 1, util) || !validMx4(rows, columns) || !aligned(out, dtype) ||
-        (reinterpret_cast<uintptr_t>(codes) & 3))
-        return fail(SRX_ERR_INVALID, "srx_layer_dequantize_mx4: bad pointer (codes: a multiple of 4), data type or sizes");
+        (reinterpret_cast<uintptr_t>(codes) & 15))
+        return fail(SRX_ERR_INVALID, "srx_layer_dequantize_mx4: bad pointer (codes: a multiple of 16), data type or sizes");
     const OnDeviceOf scope(codes);
     if (!scope.valid) return fail(SRX_ERR_INVALID, std::string("srx_layer_dequantize_mx4") + kNotOnDevice);
     SRX_HIP(srx::LaunchDequantizeMx4(util.GetDataType(), static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales),
@@ -1238,8 +1238,8 @@ srx_status srx_layer_conv2d_mx4(int32_t dtype, const void* codes, const void* sc
     if (!codes || !scales || !sizes || !filterCodes || !filterScales || !filterSizes || !out || !utilFor(dtype, 1, util) ||
         !util.CreateConvolutionMx4Layer(sizes, filterSizes, uint32_t(activation), op))
         return fail(SRX_ERR_INVALID, "srx_layer_conv2d_mx4: bad pointer, data type, activation or sizes (filter depth must equal the input channels, sides <= 7)");
-    if (!aligned(out, dtype) || !aligned(bias, dtype) || (reinterpret_cast<uintptr_t>(codes) & 3) || (reinterpret_cast<uintptr_t>(filterCodes) & 3))
-        return fail(SRX_ERR_INVALID, "srx_layer_conv2d_mx4: a tensor is not aligned to its element type (codes: a multiple of 4)");
+    if (!aligned(out, dtype) || !aligned(bias, dtype) || (reinterpret_cast<uintptr_t>(codes) & 15) || (reinterpret_cast<uintptr_t>(filterCodes) & 15))
+        return fail(SRX_ERR_INVALID, "srx_layer_conv2d_mx4: a tensor is not aligned to its element type (codes: a multiple of 16)");
     const OnDeviceOf scope(codes);
     if (!scope.valid) return fail(SRX_ERR_INVALID, std::string("srx_layer_conv2d_mx4") + kNotOnDevice);
     SRX_HIP(srx::LaunchConvMx4(op, static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales),

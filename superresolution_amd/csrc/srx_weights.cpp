@@ -186,6 +186,8 @@ bool Util::CreateConvolutionMx4Layer(const uint32_t inputSizes[4], const uint32_
     if (filterSizes[2] > 7 || filterSizes[3] > 7 || inputSizes[1] > kMaxChannels || filterSizes[0] > kMaxChannels) return false;
     if (uint64_t(inputSizes[0]) * inputSizes[2] * inputSizes[3] > uint64_t(INT32_MAX)) return false;
     if (!validSizes(os)) return false;
+    // the filters of a tile lie within 2^31 bytes of each other
+    if (uint64_t(filterSizes[2]) * filterSizes[3] * ((inputSizes[1] + 31) / 32) >= (1u << 19)) return false;
     opOut.kind = Operator::Kind::CONVOLUTION_MX4;
     opOut.activation = Activation(activation);
     return true;

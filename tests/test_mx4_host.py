@@ -36,7 +36,7 @@ def test_block_form_arguments_refused():
     refused(S.layer_quantize_mx4, 0, P, 1, 1, P, None)
     refused(S.layer_quantize_mx4, 0, P + 1, 1, 1, P, P)          # fp16 at an odd address
     refused(S.layer_quantize_mx4, 1, P + 2, 1, 1, P, P)          # fp32 at half its size
-    refused(S.layer_quantize_mx4, 0, P, 1, 1, P + 2, P)          # codes are written as words
+    refused(S.layer_quantize_mx4, 0, P, 1, 1, P + 8, P)          # codes at a multiple of 16
     refused(S.layer_dequantize_mx4, -1, P, P, 1, 1, P)
     refused(S.layer_dequantize_mx4, 0, None, P, 1, 1, P)
     refused(S.layer_dequantize_mx4, 0, P, None, 1, 1, P)
@@ -58,7 +58,7 @@ def test_group_norm_arguments_refused(change):
     args = norm(**change)
     refused(S.layer_group_norm, *args)
     dtype, x, sizes, groups, scale, bias, epsilon, act, out, work, nbytes = args
-    codes = out if out != P + 1 else P + 2
+    codes = out if out != P + 1 else P + 8
     refused(S.layer_group_norm_mx4, dtype, x, sizes, groups, scale, bias, epsilon, act, codes, P, work, nbytes)
 
 
@@ -82,9 +82,10 @@ def conv(dtype=0, codes=P, scales=P, sizes=(1, 8, 4, 4), fc=P, fs=P, fsizes=(5, 
 @pytest.mark.parametrize("change", [
     dict(dtype=2), dict(codes=None), dict(scales=None), dict(fc=None), dict(fs=None), dict(out=None), dict(act=3), dict(act=-1),
     dict(fsizes=(5, 9, 3, 3)), dict(fsizes=(5, 8, 8, 3)), dict(fsizes=(5, 8, 3, 8)), dict(fsizes=(0, 8, 3, 3)),
-    dict(fsizes=(5, 8, 0, 3)), dict(sizes=(0, 8, 4, 4)), dict(sizes=(1, 8, 4, 0)), dict(codes=P + 2), dict(fc=P + 1),
+    dict(fsizes=(5, 8, 0, 3)), dict(sizes=(0, 8, 4, 4)), dict(sizes=(1, 8, 4, 0)), dict(codes=P + 8), dict(fc=P + 4),
     dict(out=P + 1), dict(bias=P + 1), dict(dtype=1, out=P + 2), dict(sizes=(2, 8, 1 << 15, 1 << 15)),
-    dict(sizes=(1, (1 << 20) + 32, 1, 1), fsizes=(1, (1 << 20) + 32, 1, 1)), dict(fsizes=((1 << 20) + 1, 8, 1, 1))])
+    dict(sizes=(1, (1 << 20) + 32, 1, 1), fsizes=(1, (1 << 20) + 32, 1, 1)), dict(fsizes=((1 << 20) + 1, 8, 1, 1)),
+    dict(sizes=(1, 1 << 20, 4, 4), fsizes=(1, 1 << 20, 4, 4))])
 def test_conv_arguments_refused(change):
     refused(S.layer_conv2d_mx4, *conv(**change))
 
