@@ -39,7 +39,7 @@ struct ConvMxArgs
     int pixels, H, W, O, kw, taps, padTop, padLeft;
     int blocks, total;                // blocks of a pixel, blocks of the whole reduction
     Divider byW, byH, byBlocks, byKw, byTilesO;
-    int tilesO;
+    int tilesO, tilesP;
     int activation;
 };
 
@@ -69,9 +69,10 @@ __device__ __forceinline__ void loadToLds(i32x4 from, unsigned offset, unsigned 
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(from) : "memory");
 }
-__device__ __forceinline__ unsigned loadWord(i32x4 from, unsigned offset)
+// The same with 4 bytes a lane.
+__device__ __forceinline__ void loadWordToLds(i32x4 from, unsigned offset, unsigned lds)
 {
-    return __builtin_amdgcn_raw_buffer_load_b32(__builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(uint64_t(unsigned(from[0])) | uint64_t(unsigned(from[1])) << 32), 0, from[2], from[3]), offset, 0, 0);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(from) : "memory");
 }
 __device__ __forceinline__ unsigned loadByte(i32x4 from, unsigned offset)
 {
@@ -128,157 +129,165 @@ __device__ __forceinline__ void finish(const ConvMxArgs& a, const f32x16 (&acc)[
     }
 }
 
-// A workgroup (four waves) makes BO output channels of BP pixels; wave w makes 32 * FO channels of 32 * FP pixels.
+// A workgroup makes BO output channels of BP pixels; a wave makes 32 * FO channels of 32 * FP pixels.
 // The reduction goes in chunks of eight blocks through two buffers in LDS: while one is multiplied, the next is on its
 // way from memory to the other (one barrier a chunk).
-//   WITHIN: no chunk crosses from one tap to the next (each tap's blocks are padded to whole chunks), so that a tap's
-//           offsets are found once; otherwise blocks are numbered through and every thread finds its own tap.
-//   WORDS:  the blocks of a pixel come in fours, so that a lane's four scales of a chunk are one word, read right into
-//           the lane that needs it; otherwise scales are staged in LDS byte by byte.
-template <typename T, int BO, int BP, int FO, int FP, bool WITHIN, bool WORDS>
-__global__ __launch_bounds__(kThreads) void ConvMxKernel(const ConvMxArgs a)
+//   WITHIN: no chunk crosses from one tap to the next (each tap's blocks are padded to whole chunks), so that a chunk's
+//           tap is found once for all; otherwise blocks are numbered through and every thread finds its own tap.
+//   WORDS:  the blocks of a pixel come in fours, so that scales are staged in words of four; otherwise byte by byte.
+template <typename T, int THREADS, int BO, int BP, int FO, int FP, bool WITHIN, bool WORDS>
+__global__ __launch_bounds__(THREADS) void ConvMxKernel(const ConvMxArgs a)
 {
-    static_assert(BO * BP == 4 * 32 * FO * 32 * FP, "four waves");
-    constexpr int kCodes = (BO + BP) * kRow, kStage = kCodes + (WORDS ? 0 : (BO + BP) * kChunk);
+    static_assert(BO * BP == THREADS / 64 * 32 * FO * 32 * FP, "the waves' tiles make the workgroup's");
+    constexpr int kPass = THREADS / 8;                                // rows of codes that a pass of all threads stages
+    constexpr int kXRows = BP / kPass, kWRows = BO / kPass;
+    constexpr int kXWords = (BP * 2 + THREADS - 1) / THREADS, kWWords = (BO * 2 + THREADS - 1) / THREADS;
+    constexpr int kCodes = (BO + BP) * kRow, kStage = kCodes + (kXWords + kWWords) * THREADS * 4, kXScales = kCodes + kWWords * THREADS * 4;
     constexpr int kOutRow = 32 * FO * int(sizeof(T)) + 16;            // bytes of a pixel in the epilogue, padded
-    constexpr int kLds = 2 * kStage > 4 * 32 * kOutRow ? 2 * kStage : 4 * 32 * kOutRow;
+    constexpr int kOut = THREADS / 64 * 32 * kOutRow, kLds = 2 * kStage > kOut ? 2 * kStage : kOut;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
     __shared__ __attribute__((aligned(16))) float sBias[BO];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
-    const unsigned tileP = a.byTilesO(blockIdx.x);
-    const int o0 = int(blockIdx.x - tileP * a.tilesO) * BO;
+    // Workgroups are dealt round-robin over the 8 XCDs.  Where there are enough pixel tiles, all channel tiles of the same
+    // pixels go to one XCD and share its L2 (256 -> 256 channels, 1x1, 65536 pixels, 64x64 tiles: 13.4 instead of 16.5 us);
+    // pixels are dealt out singly (one long run of them for each XCD: 163 instead of 134 us for 64 -> 64 channels, 3x3,
+    // 1920x1080).
+    unsigned tileO, tileP;
+    if (a.tilesP >= 64)
+    {
+        const unsigned turn = blockIdx.x >> 3, round = a.byTilesO(turn);
+        tileO = turn - round * a.tilesO;
+        tileP = round * 8 + (blockIdx.x & 7);
+    }
+    else
+    {
+        tileP = a.byTilesO(blockIdx.x);
+        tileO = blockIdx.x - tileP * a.tilesO;
+    }
+    if (tileP >= unsigned(a.tilesP)) return;
+    const int o0 = int(tileO) * BO;
     const int64_t m0 = int64_t(tileP) * BP;
     constexpr int kWavesO = BO / (32 * FO);
     const int wo = (wave % kWavesO) * 32 * FO, wp = (wave / kWavesO) * 32 * FP;
     const unsigned ldsAt = unsigned(uintptr_t((__attribute__((address_space(3))) uint8_t*)lds));
 
-    // Staging: eight threads a row of codes, rows 32 apart; a thread's place in LDS is fixed, so the swizzle picks its block.
-    constexpr int kXRows = BP / 32, kWRows = BO / 32;
-    const int sr = tid >> 3, sb = (tid & 7) ^ ((sr >> 1) & 7);
+    // Staging.  Codes: eight threads a row; a thread's place in LDS is fixed, so the swizzle picks its block.
+    // Scales: two threads a row, four blocks each (WORDS); else with the codes.
+    const int sr = tid >> 3, sb = (tid & 7) ^ ((sr >> 1) & 7), zr = tid >> 1, zb = (tid & 1) * 4;
     const int pixelBytes = a.blocks * kMxBytes;
     const unsigned rowBytes = unsigned(a.W) * unsigned(pixelBytes);     // below 2^31 where it is used (!WITHIN)
-    const auto place = [&](int64_t m, int& y, int& x) {
+    const auto place = [&](int64_t m, bool exists, int& y, int& x) {
         const unsigned row = a.byW(unsigned(m));
-        x = int(unsigned(m) - row * unsigned(a.W));
-        y = m < a.pixels ? int(row - a.byH(row) * unsigned(a.H)) : INT32_MIN / 2;   // never inside
+        x = int(unsigned(m) - row * unsigned(a.W)) - a.padLeft;
+        y = exists && m < a.pixels ? int(row - a.byH(row) * unsigned(a.H)) - a.padTop : INT32_MIN / 2;   // never inside
     };
-    int y[kXRows], x[kXRows], fy[FP], fx[FP];
+    int y[kXRows], x[kXRows], zy[kXWords], zx[kXWords];                 // of the window's first tap
+    unsigned xOff[kXRows], wOff[kWRows], zOff[kXWords], vOff[kWWords];
 #pragma unroll
-    for (int i = 0; i < kXRows; ++i) place(m0 + sr + 32 * i, y[i], x[i]);
+    for (int i = 0; i < kXRows; ++i)
+    {
+        place(m0 + sr + kPass * i, true, y[i], x[i]);
+        xOff[i] = unsigned((sr + kPass * i) * a.blocks + (WITHIN ? sb : 0)) * kMxBytes;
+    }
+#pragma unroll
+    for (int i = 0; i < kWRows; ++i) wOff[i] = o0 + sr + kPass * i < a.O ? unsigned((sr + kPass * i) * a.total + sb) * kMxBytes : kRange;
     if (WORDS)
     {
 #pragma unroll
-        for (int j = 0; j < FP; ++j) place(m0 + wp + 32 * j + l, fy[j], fx[j]);
+        for (int i = 0; i < kXWords; ++i)
+        {
+            const int r = zr + THREADS / 2 * i;
+            place(m0 + r, r < BP, zy[i], zx[i]);
+            zOff[i] = unsigned(r * a.blocks + (WITHIN ? zb : 0));
+        }
+#pragma unroll
+        for (int i = 0; i < kWWords; ++i)
+        {
+            const int r = zr + THREADS / 2 * i;
+            vOff[i] = r < BO && o0 + r < a.O ? unsigned(r * a.total + zb) : kRange;
+        }
     }
     const auto inside = [&](int yy, int xx) { return unsigned(yy) < unsigned(a.H) && unsigned(xx) < unsigned(a.W); };
 
-    // where the next chunk is
-    int tap = 0, c0 = 0, k0 = 0;                                        // WITHIN: tap and block of the pixel; else block of all
-    const uint8_t *xBase = nullptr, *zBase = nullptr;
-    unsigned xOff[kXRows], wOff[kWRows], zOff[FP], vOff[FO];
+    // The next chunk: tap and block of the pixel (WITHIN), or block of all.  Beyond the last, nothing is read.
+    int tap = 0, c0 = 0;
+    constexpr int kLoads = kWRows + kXRows + (WORDS ? kWWords + kXWords : 0);
+    i32x4 xd, zd, wd, vd;
+    unsigned off[kLoads];
+    uint8_t xz[kXRows], wz[kWRows];
+    // where the next chunk's data are
+    const auto prepare = [&]() {
+        // the pixels' descriptors start at the window's first tap (of the tile's first pixel) or at the chunk's tap
+        int ky = 0, kx = 0;
+        if (WITHIN) { ky = int(a.byKw(unsigned(tap))); kx = tap - ky * a.kw; }
+        const int64_t first = m0 + int64_t(ky - a.padTop) * a.W + kx - a.padLeft;
+        const int kb = WITHIN ? tap * a.blocks + c0 : c0;
+        xd = descriptor(a.codes + (first * a.blocks + (WITHIN ? c0 : 0)) * kMxBytes, kRange);
+        zd = descriptor(a.scales + first * a.blocks + (WITHIN ? c0 : 0), WORDS ? kRange : kRange >> 4);
+        wd = descriptor(a.wCodes + (int64_t(o0) * a.total + kb) * kMxBytes, kRange);
+        vd = descriptor(a.wScales + int64_t(o0) * a.total + kb, WORDS ? kRange : kRange >> 4);
+        const int limit = WITHIN ? (tap < a.taps ? a.blocks : 0) : a.total;
+        const unsigned out = c0 + sb < limit ? 0u : kRange;
+        unsigned from = 0;
+        if (!WITHIN)
+        {
+            const int t = int(a.byBlocks(unsigned(c0 + sb)));
+            ky = int(a.byKw(unsigned(t)));
+            kx = t - ky * a.kw;
+            from = unsigned(ky) * rowBytes + unsigned(kx * pixelBytes + (c0 + sb - t * a.blocks) * kMxBytes);
+        }
 #pragma unroll
-    for (int i = 0; i < kWRows; ++i) wOff[i] = o0 + sr + 32 * i < a.O ? unsigned((sr + 32 * i) * a.total + sb) * kMxBytes : kRange;
-    if (WORDS)
-    {
+        for (int i = 0; i < kWRows; ++i) off[i] = wOff[i] | out;
 #pragma unroll
-        for (int i = 0; i < FO; ++i) vOff[i] = o0 + wo + 32 * i + l < a.O ? unsigned((wo + 32 * i + l) * a.total + 4 * h) : kRange;
-    }
-    const auto enterTap = [&]() {
-        const int ky = int(a.byKw(unsigned(tap))), dy = ky - a.padTop, dx = tap - ky * a.kw - a.padLeft;
-        xBase = a.codes + (m0 + int64_t(dy) * a.W + dx) * pixelBytes;
-        zBase = a.scales + (m0 + int64_t(dy) * a.W + dx) * a.blocks;
-#pragma unroll
-        for (int i = 0; i < kXRows; ++i) xOff[i] = inside(y[i] + dy, x[i] + dx) ? unsigned((sr + 32 * i) * a.blocks + sb) * kMxBytes : kRange;
+        for (int i = 0; i < kXRows; ++i) off[kWRows + i] = (inside(y[i] + ky, x[i] + kx) ? xOff[i] + from : kRange) | out;
         if (WORDS)
         {
+            const unsigned zOut = c0 + zb < limit ? 0u : kRange;
+            if (!WITHIN)
+            {
+                const int t = int(a.byBlocks(unsigned(c0 + zb)));
+                ky = int(a.byKw(unsigned(t)));
+                kx = t - ky * a.kw;
+                from = (unsigned(ky) * rowBytes + unsigned(kx * pixelBytes)) / kMxBytes + unsigned(c0 + zb - t * a.blocks);
+            }
 #pragma unroll
-            for (int j = 0; j < FP; ++j) zOff[j] = inside(fy[j] + dy, fx[j] + dx) ? unsigned((wp + 32 * j + l) * a.blocks + 4 * h) : kRange;
+            for (int i = 0; i < kWWords; ++i) off[kWRows + kXRows + i] = vOff[i] | zOut;
+#pragma unroll
+            for (int i = 0; i < kXWords; ++i)
+                off[kWRows + kXRows + kWWords + i] = (inside(zy[i] + ky, zx[i] + kx) ? zOff[i] + from : kRange) | zOut;
         }
-    };
-    if (WITHIN) enterTap();
-    else
-    {
-        xBase = a.codes + (m0 - int64_t(a.padTop) * a.W - a.padLeft) * pixelBytes;
-        zBase = a.scales + (m0 - int64_t(a.padTop) * a.W - a.padLeft) * a.blocks;
-    }
-
-    unsigned xs[FP], ws[FO], nextX[FP], nextW[FO], xz[kXRows], wz[kWRows];
-    const auto fetch = [&](int stage) {
-        const int block = WITHIN ? c0 : 0;
-        const int kb = WITHIN ? tap * a.blocks + c0 : k0;
-        const bool in = WITHIN ? c0 + sb < a.blocks : k0 + sb < a.total;
-        const i32x4 xd = descriptor(xBase + int64_t(block) * kMxBytes, kRange), wd = descriptor(a.wCodes + (int64_t(o0) * a.total + kb) * kMxBytes, kRange);
-        const i32x4 zd = descriptor(zBase + block, WORDS ? kRange : kRange >> 4), vd = descriptor(a.wScales + int64_t(o0) * a.total + kb, WORDS ? kRange : kRange >> 4);
-        const unsigned at = ldsAt + stage + wave * 1024;
-        unsigned off[kXRows];
+        c0 += kChunk;
         if (WITHIN)
         {
-#pragma unroll
-            for (int i = 0; i < kXRows; ++i) off[i] = in ? xOff[i] : kRange;
+            tap = c0 >= a.blocks ? tap + 1 : tap;
+            c0 = c0 >= a.blocks ? 0 : c0;
         }
-        else
-        {
-            const int t = int(a.byBlocks(unsigned(k0 + sb))), ky = int(a.byKw(unsigned(t))), kx = t - ky * a.kw;
-            const unsigned from = unsigned(ky) * rowBytes + unsigned(kx * pixelBytes + (k0 + sb - t * a.blocks) * kMxBytes);
-#pragma unroll
-            for (int i = 0; i < kXRows; ++i)
-                off[i] = in && inside(y[i] + ky - a.padTop, x[i] + kx - a.padLeft) ? from + unsigned((sr + 32 * i) * pixelBytes) : kRange;
-        }
-#pragma unroll
-        for (int i = 0; i < kWRows; ++i) loadToLds(wd, in ? wOff[i] : kRange, at + i * 4096);
-#pragma unroll
-        for (int i = 0; i < kXRows; ++i) loadToLds(xd, off[i], at + BO * kRow + i * 4096);
-        if (WORDS && WITHIN)
-        {
-            const bool zin = c0 + 4 * h < a.blocks;
-#pragma unroll
-            for (int i = 0; i < FO; ++i) nextW[i] = loadWord(vd, zin ? vOff[i] : kRange);
-#pragma unroll
-            for (int j = 0; j < FP; ++j) nextX[j] = loadWord(zd, zin ? zOff[j] : kRange);
-        }
-        else if (WORDS)
-        {
-            const int kz = k0 + 4 * h;
-            const int t = int(a.byBlocks(unsigned(kz))), ky = int(a.byKw(unsigned(t))), kx = t - ky * a.kw;
-            const bool zin = kz < a.total;
-            const unsigned from = (unsigned(ky) * rowBytes + unsigned(kx * pixelBytes)) / kMxBytes + unsigned(kz - t * a.blocks);
-#pragma unroll
-            for (int i = 0; i < FO; ++i) nextW[i] = loadWord(vd, zin ? vOff[i] : kRange);
-#pragma unroll
-            for (int j = 0; j < FP; ++j)
-                nextX[j] = loadWord(zd, zin && inside(fy[j] + ky - a.padTop, fx[j] + kx - a.padLeft) ? from + unsigned((wp + 32 * j + l) * a.blocks) : kRange);
-        }
-        else
-        {
-#pragma unroll
-            for (int i = 0; i < kWRows; ++i) wz[i] = loadByte(vd, (in ? wOff[i] : kRange) / kMxBytes);
-#pragma unroll
-            for (int i = 0; i < kXRows; ++i) xz[i] = loadByte(zd, off[i] / kMxBytes);
-        }
-        if (WITHIN)
-        {
-            c0 += kChunk;
-            if (c0 >= a.blocks) { c0 = 0; ++tap; if (tap < a.taps) enterTap(); }
-        }
-        else k0 += kChunk;
     };
-    // after fetch(stage): what does not go to LDS by itself
+    // load number i of the prepared chunk
+    const auto load = [&](int i, int stage) {
+        const unsigned at = ldsAt + stage + wave * 1024, zAt = ldsAt + stage + kCodes + wave * 256;
+        if (i < kWRows) loadToLds(wd, off[i], at + i * THREADS * 16);
+        else if (i < kWRows + kXRows) loadToLds(xd, off[i], at + BO * kRow + (i - kWRows) * THREADS * 16);
+        else if (i < kWRows + kXRows + kWWords) loadWordToLds(vd, off[i], zAt + (i - kWRows - kXRows) * THREADS * 4);
+        else loadWordToLds(zd, off[i], zAt + kXScales - kCodes + (i - kWRows - kXRows - kWWords) * THREADS * 4);
+    };
+    const auto loadBytes = [&]() {
+#pragma unroll
+        for (int i = 0; i < kWRows; ++i) wz[i] = loadByte(vd, off[i] / kMxBytes);
+#pragma unroll
+        for (int i = 0; i < kXRows; ++i) xz[i] = loadByte(zd, off[kWRows + i] / kMxBytes);
+    };
+    const auto loadAll = [&](int stage) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) load(i, stage);
+        if (!WORDS) loadBytes();
+    };
+    // the bytes of loadBytes() to the chunk's place in LDS
     const auto settle = [&](int stage) {
-        if (WORDS)
-        {
 #pragma unroll
-            for (int i = 0; i < FO; ++i) ws[i] = nextW[i];
+        for (int i = 0; i < kWRows; ++i) lds[stage + kCodes + (sr + kPass * i) * kChunk + sb] = wz[i];
 #pragma unroll
-            for (int j = 0; j < FP; ++j) xs[j] = nextX[j];
-        }
-        else
-        {
-            uint8_t* z = lds + stage + kCodes;
-#pragma unroll
-            for (int i = 0; i < kWRows; ++i) z[(sr + 32 * i) * kChunk + sb] = uint8_t(wz[i]);
-#pragma unroll
-            for (int i = 0; i < kXRows; ++i) z[(BO + sr + 32 * i) * kChunk + sb] = uint8_t(xz[i]);
-        }
+        for (int i = 0; i < kXRows; ++i) lds[stage + kXScales + (sr + kPass * i) * kChunk + sb] = xz[i];
     };
 
     f32x16 acc[FO][FP];
@@ -289,79 +298,278 @@ __global__ __launch_bounds__(kThreads) void ConvMxKernel(const ConvMxArgs a)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
-    fetch(0);
-    for (int o = tid; o < BO; o += kThreads)
-        sBias[o] = a.bias && o0 + o < a.O ? (float)static_cast<const T*>(a.bias)[o0 + o] : 0.0f;
-    settle(0);
+    // Step s multiplies the blocks s (lanes 0-31) and 4 + s (lanes 32-63) of the chunk: a lane's four scales are one word.
+    uint4 wf[2][FO], xf[2][FP];
+    unsigned ws[FO], xs[FP], oldW[FO], oldX[FP];
+    const auto read = [&](int set, int stage, int s) {
+#pragma unroll
+        for (int i = 0; i < FO; ++i) wf[set][i] = *reinterpret_cast<const uint4*>(lds + stage + slot(wo + 32 * i + l, 4 * h + s));
+#pragma unroll
+        for (int j = 0; j < FP; ++j) xf[set][j] = *reinterpret_cast<const uint4*>(lds + stage + BO * kRow + slot(wp + 32 * j + l, 4 * h + s));
+    };
+    const auto readScales = [&](int stage) {
+#pragma unroll
+        for (int i = 0; i < FO; ++i) ws[i] = *reinterpret_cast<const unsigned*>(lds + stage + kCodes + (wo + 32 * i + l) * kChunk + 4 * h);
+#pragma unroll
+        for (int j = 0; j < FP; ++j) xs[j] = *reinterpret_cast<const unsigned*>(lds + stage + kXScales + (wp + 32 * j + l) * kChunk + 4 * h);
+    };
+#define SRX_MULTIPLY(S, SET, WS, XS)                                                                                   \
+    _Pragma("unroll") for (int i = 0; i < FO; ++i)                                                                     \
+        _Pragma("unroll") for (int j = 0; j < FP; ++j)                                                                 \
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(wf[SET][i]), widen(xf[SET][j]), acc[i][j], 4, 4, S, WS[i], S, XS[j]);
+
     const int chunks = WITHIN ? a.taps * ((a.blocks + kChunk - 1) / kChunk) : (a.total + kChunk - 1) / kChunk;
-    int stage = 0, left = WITHIN ? a.blocks : a.total;                  // blocks left in the tap / in all
-    for (int c = 0; c < chunks; ++c)
+    prepare();
+    loadAll(0);
+    for (int o = tid; o < BO; o += THREADS)
+        sBias[o] = a.bias && o0 + o < a.O ? (float)static_cast<const T*>(a.bias)[o0 + o] : 0.0f;
+    if (!WORDS) settle(0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    read(0, 0, 0);
+    readScales(0);
+    if (chunks > 1)
     {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const uint8_t* from = lds + stage;
-        stage = kStage - stage;
-        if (c + 1 < chunks) fetch(stage);
-        if (!WORDS)
-        {
-            const unsigned* z = reinterpret_cast<const unsigned*>(from + kCodes);
-#pragma unroll
-            for (int i = 0; i < FO; ++i) ws[i] = z[(wo + 32 * i + l) * 2 + h];
-#pragma unroll
-            for (int j = 0; j < FP; ++j) xs[j] = z[(BO + wp + 32 * j + l) * 2 + h];
-        }
-        // step s multiplies the blocks s (lanes 0-31) and 4 + s (lanes 32-63): a lane's four scales are one word
-#define SRX_STEP(S)                                                                                                    \
-        if (S < left)                                                                                                  \
-        {                                                                                                              \
-            i32x8 wf[FO], xf[FP];                                                                                      \
-            _Pragma("unroll") for (int i = 0; i < FO; ++i)                                                             \
-                wf[i] = widen(*reinterpret_cast<const uint4*>(from + slot(wo + 32 * i + l, 4 * h + S)));               \
-            _Pragma("unroll") for (int j = 0; j < FP; ++j)                                                             \
-                xf[j] = widen(*reinterpret_cast<const uint4*>(from + BO * kRow + slot(wp + 32 * j + l, 4 * h + S)));   \
-            _Pragma("unroll") for (int i = 0; i < FO; ++i)                                                             \
-                _Pragma("unroll") for (int j = 0; j < FP; ++j)                                                         \
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[i], xf[j], acc[i][j], 4, 4, S, ws[i], S, xs[j]); \
-        }
-        SRX_STEP(0)
-        SRX_STEP(1)
-        SRX_STEP(2)
-        SRX_STEP(3)
-#undef SRX_STEP
-        left -= kChunk;
-        if (WITHIN && left <= 0) left = a.blocks;
-        if (c + 1 < chunks) settle(stage);
+        prepare();
+        loadAll(kStage);
     }
-    __syncthreads();
+    int stage = 0;
+    for (int c = 1; c < chunks; ++c)
+    {
+        // The first step's operands are in set 0; a step's operands are read while the one before is multiplied.
+        read(1, stage, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        SRX_MULTIPLY(0, 0, ws, xs)
+        __builtin_amdgcn_sched_barrier(0);
+        read(0, stage, 2);
+        __builtin_amdgcn_sched_barrier(0);
+        // the addresses of the chunk after the next, between the products
+        prepare();
+        SRX_MULTIPLY(1, 1, ws, xs)
+#pragma unroll
+        for (int i = 0; i < FO * FP; ++i)
+        {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);            // one product,
+            __builtin_amdgcn_sched_group_barrier(0x6, 96 / (FO * FP), 0);   // then scalar and vector arithmetic
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        read(1, stage, 3);
+        __builtin_amdgcn_sched_barrier(0);
+        SRX_MULTIPLY(2, 0, ws, xs)
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < FO; ++i) oldW[i] = ws[i];
+#pragma unroll
+        for (int j = 0; j < FP; ++j) oldX[j] = xs[j];
+        stage = kStage - stage;
+        if (!WORDS) settle(stage);
+        // after this the next chunk is there, and this one is in registers in every wave: its place is free
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        read(0, stage, 0);
+        readScales(stage);
+        __builtin_amdgcn_sched_barrier(0);
+        // the loads go out between the products
+#pragma unroll
+        for (int i = 0; i < FO; ++i)
+#pragma unroll
+            for (int j = 0; j < FP; ++j)
+            {
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(wf[1][i]), widen(xf[1][j]), acc[i][j], 4, 4, 3, oldW[i], 3, oldX[j]);
+                __builtin_amdgcn_sched_barrier(0);
+                constexpr int kN = FO * FP;
+#pragma unroll
+                for (int k = kLoads * (i * FP + j) / kN; k < kLoads * (i * FP + j + 1) / kN; ++k) load(k, kStage - stage);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        if (!WORDS) loadBytes();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    // The last chunk: where three blocks or less are left, they lie in the first steps' lower lanes.
+    const int last = WITHIN ? a.blocks - (a.blocks - 1) / kChunk * kChunk : a.total - (a.total - 1) / kChunk * kChunk;
+    SRX_MULTIPLY(0, 0, ws, xs)
+    if (last > 1)
+    {
+        read(1, stage, 1);
+        SRX_MULTIPLY(1, 1, ws, xs)
+        if (last > 2)
+        {
+            read(0, stage, 2);
+            SRX_MULTIPLY(2, 0, ws, xs)
+            if (last > 3)
+            {
+                read(1, stage, 3);
+                SRX_MULTIPLY(3, 1, ws, xs)
+            }
+        }
+    }
+#undef SRX_MULTIPLY
+    // (also the loads of the chunk after the last, which write zeros)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     uint8_t* mine = lds + wave * 32 * kOutRow;
     if (a.activation == 0) finish<T, FO, FP, 0>(a, acc, sBias + wo, mine, m0 + wp, o0 + wo, lane);
     else if (a.activation == 1) finish<T, FO, FP, 1>(a, acc, sBias + wo, mine, m0 + wp, o0 + wo, lane);
     else finish<T, FO, FP, 2>(a, acc, sBias + wo, mine, m0 + wp, o0 + wo, lane);
 }
 
-template <typename T, int BO, int BP, int FO, int FP>
+// 16 bytes a lane, by the compiler's own count.
+__device__ __forceinline__ uint4 loadCodes(i32x4 from, unsigned offset)
+{
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(__builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(uint64_t(unsigned(from[0])) | uint64_t(unsigned(from[1])) << 32), 0, from[2], from[3]), offset, 0, 0);
+    return uint4{v[0], v[1], v[2], v[3]};
+}
+__device__ __forceinline__ unsigned loadWord(i32x4 from, unsigned offset)
+{
+    return __builtin_amdgcn_raw_buffer_load_b32(__builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(uint64_t(unsigned(from[0])) | uint64_t(unsigned(from[1])) << 32), 0, from[2], from[3]), offset, 0, 0);
+}
+
+// Few pixels: a workgroup makes 16 output channels of 16 * FP pixels on v_mfma_scale_f32_16x16x128_f8f6f4, and its waves
+// share the reduction: wave w takes the chunks w, w + 8, .. of sixteen blocks, straight from memory into registers, and the
+// partial sums are added up in LDS in the waves' order.  Lane l holds row (or column) l & 15; step s multiplies the
+// blocks 4 * (l >> 4) + s, so that a lane's four scales are one word and its codes 64 bytes in a row.
+constexpr int kRowWaves = 8;
+template <typename T, int FP, bool WORDS>
+__global__ __launch_bounds__(64 * kRowWaves) void ConvMxRowsKernel(const ConvMxArgs a)
+{
+    __shared__ __attribute__((aligned(16))) f32x4 part[kRowWaves][FP][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), q = lane >> 4, l = lane & 15;
+    const unsigned tileP = a.byTilesO(blockIdx.x);
+    const int o0 = int(blockIdx.x - tileP * a.tilesO) * 16;
+    const int64_t m0 = int64_t(tileP) * 16 * FP;
+    const int pixelBytes = a.blocks * kMxBytes;
+    const unsigned rowBytes = unsigned(a.W) * unsigned(pixelBytes);
+    int y[FP], x[FP];
+#pragma unroll
+    for (int j = 0; j < FP; ++j)
+    {
+        const int64_t m = m0 + 16 * j + l;
+        const unsigned row = a.byW(unsigned(m));
+        x[j] = int(unsigned(m) - row * unsigned(a.W)) - a.padLeft;
+        y[j] = m < a.pixels ? int(row - a.byH(row) * unsigned(a.H)) - a.padTop : INT32_MIN / 2;
+    }
+    const auto inside = [&](int yy, int xx) { return unsigned(yy) < unsigned(a.H) && unsigned(xx) < unsigned(a.W); };
+    const int64_t first = m0 - int64_t(a.padTop) * a.W - a.padLeft;
+    const i32x4 xd = descriptor(a.codes + first * pixelBytes, kRange), zd = descriptor(a.scales + first * a.blocks, kRange >> 4);
+    const i32x4 wd = descriptor(a.wCodes + int64_t(o0) * a.total * kMxBytes, kRange), vd = descriptor(a.wScales + int64_t(o0) * a.total, kRange >> 4);
+    const unsigned wRow = o0 + l < a.O ? unsigned(l * a.total) * kMxBytes : kRange;
+
+    f32x4 acc[FP];
+#pragma unroll
+    for (int j = 0; j < FP; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k0 = wave * 16; k0 < a.total; k0 += kRowWaves * 16)
+    {
+        uint4 wf[4], xf[FP][4];
+        unsigned ws = 0, xs[FP];
+#pragma unroll
+        for (int j = 0; j < FP; ++j) xs[j] = 0;
+        const int kb = k0 + 4 * q;
+        unsigned off[FP];
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+        {
+            const unsigned out = kb + s < a.total ? 0u : kRange;
+            const unsigned at = (wRow + unsigned(kb + s) * kMxBytes) | out;
+            wf[s] = loadCodes(wd, at);
+            if (!WORDS) ws |= unsigned(loadByte(vd, at / kMxBytes)) << (8 * s);
+            if (!WORDS || s == 0)
+            {
+                const int t = int(a.byBlocks(unsigned(kb + s))), ky = int(a.byKw(unsigned(t))), kx = t - ky * a.kw;
+                const unsigned from = unsigned(ky) * rowBytes + unsigned(kx * pixelBytes + (kb + s - t * a.blocks) * kMxBytes);
+#pragma unroll
+                for (int j = 0; j < FP; ++j) off[j] = (inside(y[j] + ky, x[j] + kx) ? from + unsigned((16 * j + l) * pixelBytes) : kRange) | out;
+            }
+#pragma unroll
+            for (int j = 0; j < FP; ++j)
+            {
+                xf[j][s] = loadCodes(xd, WORDS ? off[j] + s * kMxBytes : off[j]);
+                if (!WORDS) xs[j] |= unsigned(loadByte(zd, off[j] / kMxBytes)) << (8 * s);
+            }
+        }
+        if (WORDS)
+        {
+            ws = loadWord(vd, ((wRow + unsigned(kb) * kMxBytes) | (kb < a.total ? 0u : kRange)) / kMxBytes);
+#pragma unroll
+            for (int j = 0; j < FP; ++j) xs[j] = loadWord(zd, off[j] / kMxBytes);
+        }
+#define SRX_STEP(S)                                                                                                    \
+        _Pragma("unroll") for (int j = 0; j < FP; ++j)                                                                 \
+            acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(wf[S]), widen(xf[j][S]), acc[j], 4, 4, S, ws, S, xs[j]);
+        SRX_STEP(0)
+        SRX_STEP(1)
+        SRX_STEP(2)
+        SRX_STEP(3)
+#undef SRX_STEP
+    }
+#pragma unroll
+    for (int j = 0; j < FP; ++j) part[wave][j][lane] = acc[j];
+    __syncthreads();
+    if (wave >= FP) return;
+    // a lane holds, for its pixel, output channels 4 * (lane >> 4) ..
+    f32x4 sum = part[0][wave][lane];
+    const int waves = min(kRowWaves, (a.total + 15) / 16);
+    for (int w = 1; w < waves; ++w) sum += part[w][wave][lane];
+    const int64_t m = m0 + 16 * wave + l;
+    if (m >= a.pixels) return;
+    const int o = o0 + 4 * q;
+    T* out = static_cast<T*>(a.out) + m * a.O + o;
+    const T* bias = static_cast<const T*>(a.bias);
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = (T)activate(sum[k] + (bias && o + k < a.O ? (float)bias[o + k] : 0.0f), a.activation);
+    if (o + 4 <= a.O) __builtin_memcpy(out, &v, sizeof(v));
+    else
+    {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (o + k < a.O) out[k] = v[k];
+    }
+}
+
+template <typename T, int FP>
+hipError_t launchRows(const ConvMxArgs& args, bool words, hipStream_t s)
+{
+    ConvMxArgs a = args;
+    a.tilesO = (a.O + 15) / 16;
+    a.byTilesO = Divider(unsigned(a.tilesO));
+    const int64_t grid = int64_t(a.tilesO) * ((int64_t(a.pixels) + 16 * FP - 1) / (16 * FP));
+    if (grid > INT32_MAX) return hipErrorInvalidValue;
+    const dim3 g(static_cast<unsigned>(grid)), block(64 * kRowWaves);
+    if (words) hipLaunchKernelGGL((ConvMxRowsKernel<T, FP, true>), g, block, 0, s, a);
+    else hipLaunchKernelGGL((ConvMxRowsKernel<T, FP, false>), g, block, 0, s, a);
+    return hipGetLastError();
+}
+template <int FP>
+hipError_t launchRows(bool half, const ConvMxArgs& a, hipStream_t s)
+{
+    const bool words = a.blocks % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.scales) | reinterpret_cast<uintptr_t>(a.wScales)) & 3) == 0;
+    return half ? launchRows<f16, FP>(a, words, s) : launchRows<float, FP>(a, words, s);
+}
+
+template <typename T, int THREADS, int BO, int BP, int FO, int FP>
 hipError_t launch(const ConvMxArgs& args, hipStream_t s)
 {
     ConvMxArgs a = args;
     a.tilesO = (a.O + BO - 1) / BO;
     a.byTilesO = Divider(unsigned(a.tilesO));
-    const int64_t grid = int64_t(a.tilesO) * ((int64_t(a.pixels) + BP - 1) / BP);
+    a.tilesP = int((int64_t(a.pixels) + BP - 1) / BP);
+    const int64_t grid = int64_t(a.tilesO) * (a.tilesP >= 64 ? (a.tilesP + 7) / 8 * 8 : a.tilesP);
     if (grid > INT32_MAX) return hipErrorInvalidValue;
-    const dim3 g(static_cast<unsigned>(grid)), block(kThreads);
+    const dim3 g(static_cast<unsigned>(grid)), block(THREADS);
     // Numbered-through blocks need all taps of a tile within the range of one descriptor.
     const int64_t span = ((int64_t(a.taps / a.kw) * a.W + a.kw + BP) * a.blocks + a.total) * kMxBytes;
     const bool within = a.taps == 1 || a.blocks % kChunk == 0 || span >= int64_t(kRange);
     const bool words = a.blocks % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.scales) | reinterpret_cast<uintptr_t>(a.wScales)) & 3) == 0;
-    if (within && words) hipLaunchKernelGGL((ConvMxKernel<T, BO, BP, FO, FP, true, true>), g, block, 0, s, a);
-    else if (within) hipLaunchKernelGGL((ConvMxKernel<T, BO, BP, FO, FP, true, false>), g, block, 0, s, a);
-    else if (words) hipLaunchKernelGGL((ConvMxKernel<T, BO, BP, FO, FP, false, true>), g, block, 0, s, a);
-    else hipLaunchKernelGGL((ConvMxKernel<T, BO, BP, FO, FP, false, false>), g, block, 0, s, a);
+    if (within && words) hipLaunchKernelGGL((ConvMxKernel<T, THREADS, BO, BP, FO, FP, true, true>), g, block, 0, s, a);
+    else if (within) hipLaunchKernelGGL((ConvMxKernel<T, THREADS, BO, BP, FO, FP, true, false>), g, block, 0, s, a);
+    else if (words) hipLaunchKernelGGL((ConvMxKernel<T, THREADS, BO, BP, FO, FP, false, true>), g, block, 0, s, a);
+    else hipLaunchKernelGGL((ConvMxKernel<T, THREADS, BO, BP, FO, FP, false, false>), g, block, 0, s, a);
     return hipGetLastError();
 }
 
-template <int BO, int BP, int FO, int FP>
+template <int THREADS, int BO, int BP, int FO, int FP>
 hipError_t launch(bool half, const ConvMxArgs& a, hipStream_t s)
 {
-    return half ? launch<f16, BO, BP, FO, FP>(a, s) : launch<float, BO, BP, FO, FP>(a, s);
+    return half ? launch<f16, THREADS, BO, BP, FO, FP>(a, s) : launch<float, THREADS, BO, BP, FO, FP>(a, s);
 }
 
 }  // namespace
@@ -391,7 +599,23 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
     a.byBlocks = Divider(unsigned(a.blocks));
     a.byKw = Divider(unsigned(a.kw));
     a.activation = int(op.activation);
-    return launch<64, 256, 2, 2>(op.dataType == ML::TensorDataType::FLOAT16, a, s);
+    const bool half = op.dataType == ML::TensorDataType::FLOAT16;
+    const auto tiles = [&](int64_t o, int64_t p) { return (a.O + o - 1) / o * ((a.pixels + p - 1) / p); };
+
+    // Few pixels: the shared reduction (ConvMxRowsKernel), as wide as 256 workgroups allow, while what its workgroups read
+    // (their number times 1 + FP rows of 16) takes less time than the chunks of a tile take one after the other.
+    // 4096 -> 4096 channels, 1x1: 4.1 (1 pixel), 9.2 (64) us instead of 9.9, 10.2 with tiles of 64x64; 26.8 instead of 13.5
+    // for 256 pixels.  256 -> 256 channels, 3x3, 16x16: 3.8 instead of 6.9.
+    const int rows = tiles(16, 64) >= 256 ? 4 : tiles(16, 32) >= 256 ? 2 : 1;
+    if (tiles(16, 16 * rows) * (1 + rows) < 1560)
+        return rows == 4 ? launchRows<4>(half, a, s) : rows == 2 ? launchRows<2>(half, a, s) : launchRows<1>(half, a, s);
+    // The largest tile that leaves no CU without one: 256x256 reads a quarter of what 64x64 does (512 -> 512 channels, 3x3,
+    // 256x256: 92 instead of 158 us), but 64 such tiles for 2048 -> 2048 channels, 1x1, 2048 pixels take 19 instead of 11.6.
+    if (a.O > 128 && tiles(256, 256) >= 256) return launch<512, 256, 256, 2, 4>(half, a, s);
+    if (a.O > 64 && tiles(128, 64) >= 512) return launch<256, 128, 64, 2, 1>(half, a, s);
+    if (a.O <= 32 && tiles(32, 128) >= 256) return launch<256, 32, 128, 1, 1>(half, a, s);
+    if (a.O <= 64 && tiles(64, 128) >= 1024) return launch<256, 64, 128, 1, 2>(half, a, s);
+    return launch<256, 64, 64, 1, 1>(half, a, s);
 }
 
 }  // namespace srx
