@@ -355,7 +355,7 @@ srx_status srx_layer_group_norm_workspace(int32_t dtype, const uint32_t sizes[4]
 /* Group normalisation with an activation.  The channels are taken in `groups` groups of C / groups neighbours; with the
  * mean and the (uncorrected) variance of an image's group over all its pixels,
  *     out = act((in - mean) / sqrt(variance + epsilon) * scale[c] + bias[c]).
- * scale and bias are C values of the tensor's type; NULL stands for 1 and 0.  `out` may be `in`.  The workspace may be
+ * epsilon is a positive normal number; scale and bias are C values of the tensor's type, NULL stands for 1 and 0.  `out` may be `in`.  The workspace may be
  * reused by the next call on the same stream. */
 srx_status srx_layer_group_norm(int32_t dtype, const void* in, const uint32_t sizes[4], uint32_t groups,
                                 const void* scale, const void* bias, float epsilon, int32_t activation, void* out,

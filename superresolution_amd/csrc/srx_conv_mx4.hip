@@ -17,19 +17,6 @@ namespace {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-// Division of numbers below 2^31 by a constant d: (mulhi(n, mul) + n) >> shift.
-struct Divider
-{
-    unsigned mul = 0, shift = 0, d = 1;
-    Divider() = default;
-    explicit Divider(unsigned by) : d(by)
-    {
-        while ((uint64_t(1) << shift) < by) ++shift;
-        mul = unsigned((uint64_t(1) << 32) * ((uint64_t(1) << shift) - by) / by + 1);
-    }
-    __device__ __forceinline__ unsigned operator()(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
-};
-
 struct ConvMxArgs
 {
     const uint8_t *codes, *scales;    // [pixels][blocks][16], [pixels][blocks]

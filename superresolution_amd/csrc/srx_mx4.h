@@ -10,6 +10,19 @@
 namespace srx {
 namespace dev {
 
+// Division of numbers below 2^31 by a constant d: (mulhi(n, mul) + n) >> shift.
+struct Divider
+{
+    unsigned mul = 0, shift = 0, d = 1;
+    Divider() = default;
+    explicit Divider(unsigned by) : d(by)
+    {
+        while ((uint64_t(1) << shift) < by) ++shift;
+        mul = unsigned((uint64_t(1) << 32) * ((uint64_t(1) << shift) - by) / by + 1);
+    }
+    __device__ __forceinline__ unsigned operator()(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+
 constexpr int kMxBlock = 32;                          // values that share a scale
 constexpr int kMxBytes = kMxBlock / 2;                // bytes of a block's codes
 

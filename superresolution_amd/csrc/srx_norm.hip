@@ -32,6 +32,8 @@ struct NormArgs
     int tileGroups, tiles;            // whole groups per workgroup (statistics, slabs)
     int applyChunks, applyPixels, applyTiles;
     int groupsInAll;                  // N * G
+    int slabRows;                     // pixels that the threads of a slab hold at a time
+    Divider byTiles, byChunks, byGroupC, byVecs;
     float epsilon;
     int activation;
 };
@@ -74,6 +76,13 @@ __device__ __forceinline__ float spread(float squares, float sum, float inverseC
     return m2 < 0.0f ? 0.0f : m2;
 }
 
+// 1 / sqrt(v): the special function unit's estimate (one part in 2^22) and one Newton step.
+__device__ __forceinline__ float inverseRoot(float v)
+{
+    const float r = __builtin_amdgcn_rsqf(v);
+    return v < 3.0e38f ? fmaf(0.5f * r, fmaf(-v * r, r, 1.0f), r) : r;
+}
+
 // Threads that share one group's reduction when `threads` of them reduce `groups` groups.
 __device__ __forceinline__ int lanesPerGroup(int groups, int threads)
 {
@@ -87,19 +96,25 @@ template <typename T>
 struct Finish
 {
     float mean[kVec], mul[kVec], add[kVec];
-    // channels c ..; stat: (mean, 1 / deviation) of group g0 and the following ones
-    __device__ __forceinline__ void prepare(const NormArgs& a, const float2* stat, int g0, int c)
+    Held<T> scale, bias;
+    // the parameters of m channels from c on: asked for early, used in prepare()
+    __device__ __forceinline__ void load(const NormArgs& a, int m, int c)
     {
-        int g = min(c, a.C - 1) / a.groupC, left = (g + 1) * a.groupC - c;
+        if (a.scale) loadHeld(static_cast<const T*>(a.scale) + c, m, scale);
+        if (a.bias) loadHeld(static_cast<const T*>(a.bias) + c, m, bias);
+    }
+    // stat: (mean, 1 / deviation) of group g0 and the following ones
+    __device__ __forceinline__ void prepare(const NormArgs& a, const float2* stat, int g0, int m, int c)
+    {
+        int g = int(a.byGroupC(unsigned(min(c, a.C - 1)))), left = (g + 1) * a.groupC - c;
 #pragma unroll
         for (int i = 0; i < kVec; ++i)
         {
-            const int ci = min(c + i, a.C - 1);
-            if (i == left && c + i < a.C) { ++g; left += a.groupC; }
+            if (i == left && i < m) { ++g; left += a.groupC; }
             const float2 st = stat[g - g0];
             mean[i] = st.x;
-            mul[i] = st.y * (a.scale ? (float)static_cast<const T*>(a.scale)[ci] : 1.0f);
-            add[i] = a.bias ? (float)static_cast<const T*>(a.bias)[ci] : 0.0f;
+            mul[i] = a.scale ? st.y * scale.get(i) : st.y;
+            add[i] = a.bias ? bias.get(i) : 0.0f;
         }
     }
     // m channels exist; `pixel` counts over all images, `column` is the thread's place among the pixel's eighths of blocks
@@ -140,10 +155,11 @@ __global__ __launch_bounds__(THREADS) void NormSlabKernel(const NormArgs a)
 {
     __shared__ float sPart[THREADS * kVec];
     __shared__ float2 sStat[THREADS * kVec];
-    const int tid = threadIdx.x, tile = blockIdx.x % a.tiles, n = blockIdx.x / a.tiles;
+    const int tid = threadIdx.x, n = int(a.byTiles(blockIdx.x)), tile = int(blockIdx.x) - n * a.tiles;
     const int g0 = tile * a.tileGroups, groups = min(a.tileGroups, a.G - g0);
     const int c0 = g0 * a.groupC, tileC = groups * a.groupC;
-    const int vecs = vecsFor<MX4>(tileC), rows = THREADS / vecs, row = tid / vecs, col = tid - row * vecs;
+    // (the last tile may be narrower: its threads keep the others' places)
+    const int vecs = int(a.byVecs.d), row = int(a.byVecs(unsigned(tid))), rows = a.slabRows, col = tid - row * vecs;
     const int m = row < rows ? max(0, min(kVec, tileC - col * kVec)) : 0;
     const int c = c0 + col * kVec, pixels = int(a.pixels);
     const T* in = static_cast<const T*>(a.in) + int64_t(n) * pixels * a.C + c;
@@ -151,8 +167,10 @@ __global__ __launch_bounds__(THREADS) void NormSlabKernel(const NormArgs a)
 #pragma unroll
     for (int i = 0; i < R; ++i)
         if (row + i * rows < pixels) loadHeld(in + int64_t(row + i * rows) * a.C, m, x[i]);
+    Finish<T> f;
+    f.load(a, m, c);
 
-    const int lanes = lanesPerGroup(groups, THREADS), lane = tid & (lanes - 1);
+    const int lanes = lanesPerGroup(a.tileGroups, THREADS), lane = tid & (lanes - 1);
     const float inv = 1.0f / (float(pixels) * float(a.groupC));
     // Where a group is whole eighths, a thread adds up its eight channels first.
     const int per = a.groupC % kVec == 0 ? 1 : kVec;
@@ -199,10 +217,9 @@ __global__ __launch_bounds__(THREADS) void NormSlabKernel(const NormArgs a)
         if (lane == 0) sStat[g].x = sum * inv;
     }
     __syncthreads();
-    Finish<T> f;
     if (m > 0)
     {
-        int g = (col * kVec) / a.groupC, left = (g + 1) * a.groupC - col * kVec;
+        int g = int(a.byGroupC(unsigned(col * kVec))), left = (g + 1) * a.groupC - col * kVec;
 #pragma unroll
         for (int k = 0; k < kVec; ++k)
         {
@@ -228,11 +245,11 @@ __global__ __launch_bounds__(THREADS) void NormSlabKernel(const NormArgs a)
     for (int g = tid / lanes; g < groups; g += THREADS / lanes)
     {
         const float sum = reduce(g);
-        if (lane == 0) sStat[g].y = 1.0f / sqrtf(fmaf(sum, inv, a.epsilon));
+        if (lane == 0) sStat[g].y = inverseRoot(fmaf(sum, inv, a.epsilon));
     }
     __syncthreads();
     if (row >= rows) return;
-    f.prepare(a, sStat, g0, c);
+    f.prepare(a, sStat, g0, m, c);
 #pragma unroll
     for (int i = 0; i < R; ++i)
         if (row + i * rows < pixels) f.template store<MX4>(a, x[i], m, c, int64_t(n) * pixels + row + i * rows);
@@ -244,9 +261,8 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
 {
     __shared__ float sMean[kTileC], sM2[kTileC];
-    int b = blockIdx.x;
-    const int tile = b % a.tiles; b /= a.tiles;
-    const int chunk = b % a.chunks, n = b / a.chunks;
+    const int b = int(a.byTiles(blockIdx.x)), tile = int(blockIdx.x) - b * a.tiles;
+    const int n = int(a.byChunks(unsigned(b))), chunk = b - n * a.chunks;
     const int g0 = tile * a.tileGroups, groups = min(a.tileGroups, a.G - g0);
     const int c0 = g0 * a.groupC, tileC = groups * a.groupC;
     const int64_t p0 = int64_t(chunk) * a.chunkPixels;
@@ -300,30 +316,26 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
 #pragma unroll
         for (int i = 0; i < kVec; ++i) k[i] = s[i] = q[i] = 0.0f;
         if (row < count) loadUpTo8(src + int64_t(row) * a.C, m, k);
+        // a batch of loads in flight
+        constexpr int kFlight = sizeof(T) == 2 ? 8 : 4;
+        const int64_t step = int64_t(rows) * a.C;
+        const T* at = src + int64_t(row + rows) * a.C;
         int p = row + rows;
-        // four loads in flight
-        for (; p + 3 * rows < count; p += 4 * rows)
-        {
-            Held<T> v[4];
-            if (m == kVec)
+        if (m == kVec)
+            for (; p + (kFlight - 1) * rows < count; p += kFlight * rows, at += kFlight * step)
             {
+                Held<T> v[kFlight];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) v[u].load(src + int64_t(p + u * rows) * a.C);
+                for (int u = 0; u < kFlight; ++u) v[u].load(at + u * step);
+#pragma unroll
+                for (int u = 0; u < kFlight; ++u)
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) { const float d = v[u].get(i) - k[i]; s[i] += d; q[i] = fmaf(d, d, q[i]); }
             }
-            else
-            {
-#pragma unroll
-                for (int u = 0; u < 4; ++u) loadHeld(src + int64_t(p + u * rows) * a.C, m, v[u]);
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) { const float d = v[u].get(i) - k[i]; s[i] += d; q[i] = fmaf(d, d, q[i]); }
-        }
-        for (; p < count; p += rows)
+        for (; p < count; p += rows, at += step)
         {
             Held<T> v;
-            loadHeld(src + int64_t(p) * a.C, m, v);
+            loadHeld(at, m, v);
 #pragma unroll
             for (int i = 0; i < kVec; ++i) { const float d = v.get(i) - k[i]; s[i] += d; q[i] = fmaf(d, d, q[i]); }
         }
@@ -369,30 +381,39 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
     }
 }
 
-// The parts of one group of one image joined by `lanes` lanes: (mean, 1 / deviation).
+// The parts of one group of one image joined by `lanes` lanes: (mean, 1 / deviation).  PER parts of each lane are asked for
+// at once and kept; more than that only images of over 2^32 pixels have.
+template <int PER>
 __device__ __forceinline__ float2 joinParts(const NormArgs& a, const float2* partial, int lane, int lanes)
 {
-    const float lastPixels = float(a.pixels - int64_t(a.chunks - 1) * a.chunkPixels);
+    const float last = float(a.pixels - int64_t(a.chunks - 1) * a.chunkPixels), each = float(a.chunkPixels), all = 1.0f / float(a.pixels);
+    const auto pixels = [&](int k) { return k < a.chunks - 1 ? each : (k == a.chunks - 1 ? last : 0.0f); };
+    float2 v[PER];
     float mean = 0.0f, m2 = 0.0f;
-    for (int k = lane; k < a.chunks; k += lanes) mean += (k == a.chunks - 1 ? lastPixels : float(a.chunkPixels)) * partial[k].x;
-    mean = sumLanes(mean, lanes) / float(a.pixels);
-    for (int k = lane; k < a.chunks; k += lanes)
-    {
-        const float2 v = partial[k];
-        const float d = v.x - mean;
-        m2 += v.y + (k == a.chunks - 1 ? lastPixels : float(a.chunkPixels)) * float(a.groupC) * d * d;
-    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = lane + i * lanes < a.chunks ? partial[lane + i * lanes] : float2{0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mean = fmaf(pixels(lane + i * lanes), v[i].x, mean);
+    for (int k = lane + PER * lanes; k < a.chunks; k += lanes) mean = fmaf(pixels(k), partial[k].x, mean);
+    mean = sumLanes(mean, lanes) * all;
+    const auto join = [&](int k, float2 p) {
+        const float d = p.x - mean;
+        m2 += k < a.chunks ? fmaf(pixels(k) * float(a.groupC), d * d, p.y) : 0.0f;
+    };
+#pragma unroll
+    for (int i = 0; i < PER; ++i) join(lane + i * lanes, v[i]);
+    for (int k = lane + PER * lanes; k < a.chunks; k += lanes) join(k, partial[k]);
     m2 = sumLanes(m2, lanes);
-    return float2{mean, 1.0f / sqrtf(m2 / (float(a.pixels) * float(a.groupC)) + a.epsilon)};
+    return float2{mean, inverseRoot(fmaf(m2, all / float(a.groupC), a.epsilon))};
 }
 
 // One wave joins the parts of one group.
-__global__ __launch_bounds__(kThreads) void NormJoinKernel(const NormArgs a)
+constexpr int kJoinPer = 16;
+__global__ __launch_bounds__(64) void NormJoinKernel(const NormArgs a)
 {
-    const int group = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-    if (group >= a.groupsInAll) return;
-    const float2 v = joinParts(a, a.partial + int64_t(group) * a.chunks, threadIdx.x & 63, 64);
-    if ((threadIdx.x & 63) == 0) a.joined[group] = v;
+    const int group = blockIdx.x;
+    const float2 v = joinParts<kJoinPer>(a, a.partial + int64_t(group) * a.chunks, threadIdx.x, 64);
+    if (threadIdx.x == 0) a.joined[group] = v;
 }
 
 // Normalises, scales, activates and stores (MX4: as 4-bit blocks) a part of an image.
@@ -401,11 +422,10 @@ __global__ __launch_bounds__(kThreads) void NormApplyKernel(const NormArgs a)
 {
     __shared__ float2 sStat[kTileC];
     // from the last part to the first: the statistics kernel read the last ones last, so they are still cached
-    int b = gridDim.x - 1 - blockIdx.x;
-    const int tile = b % a.applyTiles; b /= a.applyTiles;
-    const int chunk = b % a.applyChunks, n = b / a.applyChunks;
+    const int b0 = int(gridDim.x - 1 - blockIdx.x), b = int(a.byTiles(unsigned(b0))), tile = b0 - b * a.tiles;
+    const int n = int(a.byChunks(unsigned(b))), chunk = b - n * a.applyChunks;
     const int c0 = tile * kTileC, tileC = min(kTileC, a.C - c0);
-    const int g0 = c0 / a.groupC, groups = (c0 + tileC - 1) / a.groupC + 1 - g0;
+    const int g0 = int(a.byGroupC(unsigned(c0))), groups = int(a.byGroupC(unsigned(c0 + tileC - 1))) + 1 - g0;
     const int64_t p0 = int64_t(chunk) * a.applyPixels;
     const int count = int(min(int64_t(a.applyPixels), a.pixels - p0));
     const int tid = threadIdx.x;
@@ -415,10 +435,12 @@ __global__ __launch_bounds__(kThreads) void NormApplyKernel(const NormArgs a)
     const T* in = static_cast<const T*>(a.in) + (n * a.pixels + p0) * a.C + c;
     constexpr int kFlight = 4;
     Held<T> x[kFlight];
-    // the first loads do not wait for the statistics
+    // neither the first loads nor those of the parameters wait for the statistics
 #pragma unroll
     for (int u = 0; u < kFlight; ++u)
         if (row + u * rows < count) loadHeld(in + int64_t(row + u * rows) * a.C, m, x[u]);
+    Finish<T> f;
+    f.load(a, m, c);
 
     if (a.chunks > kJoin)
     {
@@ -429,23 +451,25 @@ __global__ __launch_bounds__(kThreads) void NormApplyKernel(const NormArgs a)
         const int lane = tid & (kJoin - 1);
         for (int g = tid / kJoin; g < groups; g += kThreads / kJoin)
         {
-            const float2 v = joinParts(a, a.partial + (int64_t(n) * a.G + g0 + g) * a.chunks, lane, kJoin);
+            const float2 v = joinParts<1>(a, a.partial + (int64_t(n) * a.G + g0 + g) * a.chunks, lane, kJoin);
             if (lane == 0) sStat[g] = v;
         }
     }
     __syncthreads();
     if (row >= rows) return;
-    Finish<T> f;
-    f.prepare(a, sStat, g0, c);
+    f.prepare(a, sStat, g0, m, c);
     const int64_t pixel0 = n * a.pixels + p0;
     for (int p = row; p < count; p += kFlight * rows)
     {
+        Held<T> next[kFlight];
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u)
+            if (p + (kFlight + u) * rows < count) loadHeld(in + int64_t(p + (kFlight + u) * rows) * a.C, m, next[u]);
 #pragma unroll
         for (int u = 0; u < kFlight; ++u)
             if (p + u * rows < count) f.template store<MX4>(a, x[u], m, c, pixel0 + p + u * rows);
 #pragma unroll
-        for (int u = 0; u < kFlight; ++u)
-            if (p + (kFlight + u) * rows < count) loadHeld(in + int64_t(p + (kFlight + u) * rows) * a.C, m, x[u]);
+        for (int u = 0; u < kFlight; ++u) x[u] = next[u];
     }
 }
 
@@ -530,6 +554,7 @@ NormPlan planNorm(const ML::Operator& op, bool mx4)
     a.activation = int(op.activation);
     p.images = op.inputSizes[0];
     const int64_t n = p.images;
+    a.byGroupC = Divider(unsigned(a.groupC));
     a.groupsInAll = int(n * a.G < INT32_MAX ? n * a.G : INT32_MAX);
 
     // slabs: the fewest groups that are a whole number of 64-byte lines (of blocks of 32 channels)
@@ -549,6 +574,9 @@ NormPlan planNorm(const ML::Operator& op, bool mx4)
             p.slabHeld = int(held);
             a.tileGroups = groups;
             a.tiles = (a.G + groups - 1) / groups;
+            a.slabRows = int(rows);
+            a.byTiles = Divider(unsigned(a.tiles));
+            a.byVecs = Divider(unsigned(vecs));
             if (n * a.tiles <= INT32_MAX) return p;
         }
     }
@@ -556,17 +584,24 @@ NormPlan planNorm(const ML::Operator& op, bool mx4)
 
     a.tileGroups = a.groupC >= kTileC ? 1 : (kTileC / a.groupC < a.G ? kTileC / a.groupC : a.G);
     a.tiles = (a.G + a.tileGroups - 1) / a.tileGroups;
-    // enough parts for the whole device, no part below 16 pixels
-    int64_t chunks = (1024 + n * a.tiles - 1) / (n * a.tiles);
-    const int64_t most = (a.pixels + 15) / 16;
+    // Statistics: parts of 64 KB at least, about 1024 workgroups at most; up to kJoin parts of an image spare the kernel
+    // that joins them, so no more are made while they stay below 128 KB.
+    const int64_t imageBytes = a.pixels * a.C * (op.dataType == ML::TensorDataType::FLOAT16 ? 2 : 4);
+    int64_t chunks = (imageBytes + (64 << 10) - 1) / (64 << 10);
+    if (chunks > kJoin && imageBytes <= int64_t(kJoin) * (128 << 10)) chunks = kJoin;
+    const int64_t most = (1024 + n * a.tiles - 1) / (n * a.tiles);
     if (chunks > most) chunks = most;
-    if (chunks < (a.pixels + (1 << 20) - 1) >> 20) chunks = (a.pixels + (1 << 20) - 1) >> 20;
+    // (no part is longer than 2^22 pixels: a thread's sums stay short)
+    if (chunks < (a.pixels + (1 << 22) - 1) >> 22) chunks = (a.pixels + (1 << 22) - 1) >> 22;
     a.chunkPixels = int((a.pixels + chunks - 1) / chunks);
     a.chunks = int((a.pixels + a.chunkPixels - 1) / a.chunkPixels);
+    // Output: about 2048 workgroups, four batches of pixels for each thread at most.
     a.applyTiles = (a.C + kTileC - 1) / kTileC;
-    int64_t parts = (4096 + n * a.applyTiles - 1) / (n * a.applyTiles);
-    if (parts > most) parts = most;
-    if (parts < a.chunks) parts = a.chunks;
+    const int rows = kTileC / (a.C < kTileC ? (a.C + 31) / 32 * 32 : kTileC);
+    int64_t parts = (2048 + n * a.applyTiles - 1) / (n * a.applyTiles);
+    const int64_t mostParts = (a.pixels + 4 * rows - 1) / (4 * rows);
+    if (parts > mostParts) parts = mostParts;
+    if (parts < (a.pixels + (1 << 22) - 1) >> 22) parts = (a.pixels + (1 << 22) - 1) >> 22;
     a.applyPixels = int((a.pixels + parts - 1) / parts);
     a.applyChunks = int((a.pixels + a.applyPixels - 1) / a.applyPixels);
     return p;
@@ -596,15 +631,21 @@ hipError_t launchNorm(const NormPlan& p, hipStream_t s)
     const int64_t statsGrid = p.images * a.chunks * a.tiles, applyGrid = p.images * a.applyChunks * a.applyTiles;
     if (statsGrid > INT32_MAX || applyGrid > INT32_MAX || p.images * a.G > INT32_MAX) return hipErrorInvalidValue;
     const dim3 block(kThreads);
-    hipLaunchKernelGGL(NormStatsKernel<T>, dim3(unsigned(statsGrid)), block, 0, s, a);
+    NormArgs st = a, ap = a;
+    st.byTiles = Divider(unsigned(a.tiles));
+    st.byChunks = Divider(unsigned(a.chunks));
+    ap.tiles = a.applyTiles;
+    ap.byTiles = Divider(unsigned(a.applyTiles));
+    ap.byChunks = Divider(unsigned(a.applyChunks));
+    hipLaunchKernelGGL(NormStatsKernel<T>, dim3(unsigned(statsGrid)), block, 0, s, st);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (a.chunks > kJoin)
     {
-        hipLaunchKernelGGL(NormJoinKernel, dim3(unsigned((a.groupsInAll + 3) / 4)), block, 0, s, a);
+        hipLaunchKernelGGL(NormJoinKernel, dim3(unsigned(a.groupsInAll)), dim3(64), 0, s, a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((NormApplyKernel<T, MX4>), dim3(unsigned(applyGrid)), block, 0, s, a);
+    hipLaunchKernelGGL((NormApplyKernel<T, MX4>), dim3(unsigned(applyGrid)), block, 0, s, ap);
     return hipGetLastError();
 }
 

@@ -51,7 +51,7 @@ def norm(dtype=0, x=P, sizes=(1, 8, 300, 200), groups=2, scale=P, bias=P, epsilo
 @pytest.mark.parametrize("change", [
     dict(dtype=2), dict(dtype=-1), dict(x=None), dict(out=None), dict(sizes=(0, 8, 4, 4)), dict(sizes=(1, 0, 4, 4)),
     dict(sizes=(1, 8, 0, 4)), dict(sizes=(1, 8, 4, 0)), dict(groups=0), dict(groups=3), dict(groups=16), dict(epsilon=0.0),
-    dict(epsilon=-1.0), dict(epsilon=float("nan")), dict(epsilon=float("inf")), dict(act=3), dict(act=-1), dict(work=None),
+    dict(epsilon=-1.0), dict(epsilon=1e-40), dict(epsilon=float("nan")), dict(epsilon=float("inf")), dict(act=3), dict(act=-1), dict(work=None),
     dict(nbytes=8), dict(work=P + 4), dict(x=P + 1), dict(scale=P + 1), dict(bias=P + 1), dict(out=P + 1),
     dict(dtype=1, x=P + 2), dict(sizes=(1, (1 << 20) + 2, 1, 1)), dict(sizes=(1 << 20, 1 << 10, 1 << 10, 1 << 5))])
 def test_group_norm_arguments_refused(change):
