@@ -124,21 +124,44 @@ __device__ __forceinline__ void store8(float* p, const float (&v)[8])
     __builtin_memcpy(p, &a, 16);
     __builtin_memcpy(p + 4, &b, 16);
 }
-// The first `count` (0 .. 8) of eight values; the others are zeros / stay untouched.
-template <typename T>
-__device__ __forceinline__ void loadUpTo8(const T* p, int count, float (&v)[8])
+// The same past the caches.
+__device__ __forceinline__ void streamOut8(f16* p, const float (&v)[8])
 {
-    if (count >= 8) { load8(p, v); return; }
+    typedef f16 f16x8u __attribute__((ext_vector_type(8), aligned(2)));
+    f16x8u h;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = (f16)v[i];
+    __builtin_nontemporal_store(h, reinterpret_cast<f16x8u*>(p));
+}
+__device__ __forceinline__ void streamOut8(float* p, const float (&v)[8])
+{
+    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+    __builtin_nontemporal_store(f32x4u{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4u*>(p));
+    __builtin_nontemporal_store(f32x4u{v[4], v[5], v[6], v[7]}, reinterpret_cast<f32x4u*>(p + 4));
+}
+// The first `count` (0 .. 8) of eight values.  Where eight are in the tensor (which ends at `end`) all are read, and the
+// others are somebody else's; only at the tensor's end are they read one by one, and the others are zeros.
+template <typename T>
+__device__ __forceinline__ void loadUpTo8(const T* p, int count, const T* end, float (&v)[8])
+{
+    if (count >= 8 || p + 8 <= end) { load8(p, v); return; }
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = i < count ? (float)p[i] : 0.0f;
 }
+// Stores the first `count` of eight values: eight, or four, two and one.
 template <typename T>
 __device__ __forceinline__ void storeUpTo8(T* p, int count, const float (&v)[8])
 {
     if (count >= 8) { store8(p, v); return; }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i < count) p[i] = (T)v[i];
+    typedef T T4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    typedef T T2 __attribute__((ext_vector_type(2), aligned(sizeof(T))));
+    const T v0 = (T)v[0], v1 = (T)v[1], v2 = (T)v[2], v3 = (T)v[3], v4 = (T)v[4], v5 = (T)v[5], v6 = (T)v[6];
+    const bool four = count & 4, two = count & 2;
+    if (four) *reinterpret_cast<T4*>(p) = T4{v0, v1, v2, v3};
+    const T a = four ? v4 : v0, b = four ? v5 : v1, c = four ? v6 : v2;
+    T* q = four ? p + 4 : p;
+    if (two) *reinterpret_cast<T2*>(q) = T2{a, b};
+    if (count & 1) q[two ? 2 : 0] = two ? c : a;
 }
 
 // 0 none, 1 ReLU, 2 SiLU: y / (1 + exp(-y)), with the exponential and the reciprocal of the special function unit

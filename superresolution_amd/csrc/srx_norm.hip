@@ -26,7 +26,7 @@ struct NormArgs
     uint8_t *codes, *scales;
     float2* partial;                  // [N][G][chunks] (mean, M2)
     float2* joined;                   // [N][G] (mean, 1 / deviation), where chunks > kJoin
-    int64_t pixels;                   // H * W
+    int64_t pixels, values;           // H * W; N * H * W * C
     int C, G, groupC;                 // channels, groups, channels of a group
     int chunks, chunkPixels;          // statistics: parts of an image
     int tileGroups, tiles;            // whole groups per workgroup (statistics, slabs)
@@ -36,6 +36,7 @@ struct NormArgs
     Divider byTiles, byChunks, byGroupC, byVecs;
     float epsilon;
     int activation;
+    int stream;                       // the output passes by the caches
 };
 
 // Eight values as they are held in memory: registers that wait for the statistics take half the room in fp16.
@@ -54,18 +55,38 @@ template <> struct Held<float>
     __device__ void set(int i, float x) { if (i < 4) a[i & 3] = x; else b[i & 3] = x; }
     __device__ float get(int i) const { return i < 4 ? a[i & 3] : b[i & 3]; }
 };
+// As loadUpTo8.
 template <typename T>
-__device__ __forceinline__ void loadHeld(const T* p, int count, Held<T>& v)
+__device__ __forceinline__ void loadHeld(const T* p, int count, const T* end, Held<T>& v)
 {
-    if (count >= kVec) { v.load(p); return; }
+    if (count >= kVec || (count > 0 && p + kVec <= end)) { v.load(p); return; }
 #pragma unroll
     for (int i = 0; i < kVec; ++i) v.set(i, i < count ? (float)p[i] : 0.0f);
 }
 
-// Sum over the `lanes` (a power of two up to 64) lanes of an aligned part of a wave.
+template <int CONTROL>
+__device__ __forceinline__ float moved(float v)
+{
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CONTROL, 0xf, 0xf, true));
+}
+// Sum over the `lanes` (a power of two up to 64, the same in the whole wave) lanes of an aligned part of a wave, in each
+// of them: neighbours, pairs, then mirrored halves of 8 and 16, and the exchanges of 16 and 32 lanes.
 __device__ __forceinline__ float sumLanes(float v, int lanes)
 {
-    for (int m = 1; m < lanes; m <<= 1) v += __shfl_xor(v, m);
+    if (lanes > 1) v += moved<0xB1>(v);
+    if (lanes > 2) v += moved<0x4E>(v);
+    if (lanes > 4) v += moved<0x141>(v);
+    if (lanes > 8) v += moved<0x140>(v);
+    if (lanes > 16)
+    {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if (lanes > 32)
+    {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
     return v;
 }
 
@@ -100,8 +121,8 @@ struct Finish
     // the parameters of m channels from c on: asked for early, used in prepare()
     __device__ __forceinline__ void load(const NormArgs& a, int m, int c)
     {
-        if (a.scale) loadHeld(static_cast<const T*>(a.scale) + c, m, scale);
-        if (a.bias) loadHeld(static_cast<const T*>(a.bias) + c, m, bias);
+        if (a.scale) loadHeld(static_cast<const T*>(a.scale) + c, m, static_cast<const T*>(a.scale) + a.C, scale);
+        if (a.bias) loadHeld(static_cast<const T*>(a.bias) + c, m, static_cast<const T*>(a.bias) + a.C, bias);
     }
     // stat: (mean, 1 / deviation) of group g0 and the following ones
     __device__ __forceinline__ void prepare(const NormArgs& a, const float2* stat, int g0, int m, int c)
@@ -137,6 +158,7 @@ struct Finish
             *reinterpret_cast<unsigned*>(a.codes + block * kMxBytes + ((c >> 1) & 12)) = codes;
             if ((c & 24) == 0) a.scales[block] = uint8_t(scale);
         }
+        else if (a.stream && m == kVec) streamOut8(static_cast<T*>(a.out) + pixel * a.C + c, v);
         else storeUpTo8(static_cast<T*>(a.out) + pixel * a.C + c, m, v);
     }
 };
@@ -163,10 +185,11 @@ __global__ __launch_bounds__(THREADS) void NormSlabKernel(const NormArgs a)
     const int m = row < rows ? max(0, min(kVec, tileC - col * kVec)) : 0;
     const int c = c0 + col * kVec, pixels = int(a.pixels);
     const T* in = static_cast<const T*>(a.in) + int64_t(n) * pixels * a.C + c;
+    const T* end = static_cast<const T*>(a.in) + a.values;
     Held<T> x[R];
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (row + i * rows < pixels) loadHeld(in + int64_t(row + i * rows) * a.C, m, x[i]);
+        if (row + i * rows < pixels) loadHeld(in + int64_t(row + i * rows) * a.C, m, end, x[i]);
     Finish<T> f;
     f.load(a, m, c);
 
@@ -257,10 +280,11 @@ __global__ __launch_bounds__(THREADS) void NormSlabKernel(const NormArgs a)
 
 // Statistics of one part of one image for a range of whole groups.  A thread keeps eight channels and walks the
 // part's pixels; sums are of x - (its first value of the channel), whose magnitude the part's own spread bounds.
-template <typename T>
+// WHOLE: no group range and no pixel ends inside eight channels.
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
 {
-    __shared__ float sMean[kTileC], sM2[kTileC];
+    __shared__ __attribute__((aligned(16))) float sMean[kTileC], sM2[kTileC];
     const int b = int(a.byTiles(blockIdx.x)), tile = int(blockIdx.x) - b * a.tiles;
     const int n = int(a.byChunks(unsigned(b))), chunk = b - n * a.chunks;
     const int g0 = tile * a.tileGroups, groups = min(a.tileGroups, a.G - g0);
@@ -268,6 +292,7 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
     const int64_t p0 = int64_t(chunk) * a.chunkPixels;
     const int count = int(min(int64_t(a.chunkPixels), a.pixels - p0));
     const T* in = static_cast<const T*>(a.in) + (n * a.pixels + p0) * a.C + c0;
+    const T* end = static_cast<const T*>(a.in) + a.values;
     float2* out = a.partial + (int64_t(n) * a.G + g0) * a.chunks + chunk;
     const int tid = threadIdx.x, vecs = (tileC + kVec - 1) / kVec;
 
@@ -281,7 +306,7 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
             {
                 float v[kVec];
                 const int m = min(kVec, tileC - col * kVec);
-                loadUpTo8(in + int64_t(p) * a.C + col * kVec, m, v);
+                loadUpTo8(in + int64_t(p) * a.C + col * kVec, m, end, v);
                 if (have == 0) k = v[0];
                 have += m;
 #pragma unroll
@@ -313,33 +338,52 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
         const int m = min(kVec, tileC - col * kVec);
         const T* src = in + col * kVec;
         float k[kVec], s[kVec], q[kVec];
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) k[i] = s[i] = q[i] = 0.0f;
-        if (row < count) loadUpTo8(src + int64_t(row) * a.C, m, k);
-        // a batch of loads in flight
-        constexpr int kFlight = sizeof(T) == 2 ? 8 : 4;
+        // The odd pixels first, then whole batches, the next of which is asked for before the current one is summed up.
+        constexpr int kFlight = 4;
+        const int mine = row < count ? (count - row + rows - 1) / rows : 0, odd = mine % kFlight;
         const int64_t step = int64_t(rows) * a.C;
-        const T* at = src + int64_t(row + rows) * a.C;
-        int p = row + rows;
-        if (m == kVec)
-            for (; p + (kFlight - 1) * rows < count; p += kFlight * rows, at += kFlight * step)
-            {
-                Held<T> v[kFlight];
+        const T* at = src + int64_t(row) * a.C;
+        Held<T> first[kFlight - 1], v[kFlight];
+        const auto load = [&](Held<T>& to, const T* from) {
+            if (WHOLE) to.load(from);
+            else loadHeld(from, m, end, to);
+        };
+        const auto sum = [&](const Held<T>& x) {
 #pragma unroll
-                for (int u = 0; u < kFlight; ++u) v[u].load(at + u * step);
+            for (int i = 0; i < kVec; ++i) { const float d = x.get(i) - k[i]; s[i] += d; q[i] = fmaf(d, d, q[i]); }
+        };
 #pragma unroll
-                for (int u = 0; u < kFlight; ++u)
-#pragma unroll
-                    for (int i = 0; i < kVec; ++i) { const float d = v[u].get(i) - k[i]; s[i] += d; q[i] = fmaf(d, d, q[i]); }
-            }
-        for (; p < count; p += rows, at += step)
+        for (int u = 0; u < kFlight - 1; ++u)
+            if (u < odd) load(first[u], at + u * step);
+        at += odd * step;
+        if (mine >= kFlight)
         {
-            Held<T> v;
-            loadHeld(at, m, v);
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) { const float d = v.get(i) - k[i]; s[i] += d; q[i] = fmaf(d, d, q[i]); }
+            for (int u = 0; u < kFlight; ++u) load(v[u], at + u * step);
         }
-        const float inv = 1.0f / float(max(1, (count - row + rows - 1) / rows));
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) { k[i] = odd ? first[0].get(i) : (mine ? v[0].get(i) : 0.0f); s[i] = q[i] = 0.0f; }
+#pragma unroll
+        for (int u = 0; u < kFlight - 1; ++u)
+            if (u < odd) sum(first[u]);
+        int batches = mine / kFlight;
+        for (; batches > 1; --batches)
+        {
+            Held<T> next[kFlight];
+            at += kFlight * step;
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) load(next[u], at + u * step);
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) sum(v[u]);
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) v[u] = next[u];
+        }
+        if (batches > 0)
+        {
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) sum(v[u]);
+        }
+        const float inv = 1.0f / float(max(1, mine));
 #pragma unroll
         for (int i = 0; i < kVec; ++i)
         {
@@ -348,34 +392,26 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
         }
     }
     __syncthreads();
-    // join the rows of each channel
-    const int stride = vecs * kVec;
-    for (int c = tid; c < tileC; c += kThreads)
-    {
-        float mean = 0.0f, m2 = 0.0f;
-        for (int r = 0; r < rows && r < count; ++r) mean += float((count - r + rows - 1) / rows) * sMean[r * stride + c];
-        mean /= float(count);
-        for (int r = 0; r < rows && r < count; ++r)
-        {
-            const float d = sMean[r * stride + c] - mean;
-            m2 += sM2[r * stride + c] + float((count - r + rows - 1) / rows) * d * d;
-        }
-        sMean[c] = mean;
-        sM2[c] = m2;
-    }
-    __syncthreads();
-    // join the channels of each group: equal counts
+    // Join the rows and channels of each group: row r has `whole` pixels, and one more below `rest`.
+    const int stride = vecs * kVec, whole = count / rows, rest = count - whole * rows, used = min(rows, count);
     const int lanes = lanesPerGroup(groups, kThreads), lane = tid & (lanes - 1);
+    const int dr = int(a.byGroupC(unsigned(lanes))), dc = lanes - dr * a.groupC;
+    const int firstR = int(a.byGroupC(unsigned(lane))), firstC = lane - firstR * a.groupC;
     for (int g = tid / lanes; g < groups; g += kThreads / lanes)
     {
         float mean = 0.0f, m2 = 0.0f;
-        for (int c = lane; c < a.groupC; c += lanes) mean += sMean[g * a.groupC + c];
-        mean = sumLanes(mean, lanes) / float(a.groupC);
-        for (int c = lane; c < a.groupC; c += lanes)
-        {
-            const float d = sMean[g * a.groupC + c] - mean;
-            m2 += sM2[g * a.groupC + c] + float(count) * d * d;
-        }
+        const auto each = [&](auto&& f) {
+            for (int r = firstR, c = firstC; r < used;)
+            {
+                f(float(whole + (r < rest ? 1 : 0)), r * stride + g * a.groupC + c);
+                r += dr;
+                c += dc;
+                if (c >= a.groupC) { c -= a.groupC; ++r; }
+            }
+        };
+        each([&](float n, int at) { mean = fmaf(n, sMean[at], mean); });
+        mean = sumLanes(mean, lanes) / (float(count) * float(a.groupC));
+        each([&](float n, int at) { const float d = sMean[at] - mean; m2 += fmaf(n * d, d, sM2[at]); });
         m2 = sumLanes(m2, lanes);
         if (lane == 0) out[int64_t(g) * a.chunks] = float2{mean, m2};
     }
@@ -417,7 +453,7 @@ __global__ __launch_bounds__(64) void NormJoinKernel(const NormArgs a)
 }
 
 // Normalises, scales, activates and stores (MX4: as 4-bit blocks) a part of an image.
-template <typename T, bool MX4>
+template <typename T, bool MX4, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void NormApplyKernel(const NormArgs a)
 {
     __shared__ float2 sStat[kTileC];
@@ -433,12 +469,22 @@ __global__ __launch_bounds__(kThreads) void NormApplyKernel(const NormArgs a)
     const int vecs = vecsFor<MX4>(tileC), rows = kThreads / vecs, row = tid / vecs, col = tid - row * vecs;
     const int m = row < rows ? max(0, min(kVec, tileC - col * kVec)) : 0, c = c0 + col * kVec;
     const T* in = static_cast<const T*>(a.in) + (n * a.pixels + p0) * a.C + c;
+    const T* end = static_cast<const T*>(a.in) + a.values;
     constexpr int kFlight = 4;
     Held<T> x[kFlight];
+    const auto load = [&](Held<T>& to, const T* from) {
+        if (WHOLE) to.load(from);
+        else loadHeld(from, m, end, to);
+    };
+    const int64_t step = int64_t(rows) * a.C;
+    const T* at = in + int64_t(row) * a.C;
     // neither the first loads nor those of the parameters wait for the statistics
+    if (m > 0)
+    {
 #pragma unroll
-    for (int u = 0; u < kFlight; ++u)
-        if (row + u * rows < count) loadHeld(in + int64_t(row + u * rows) * a.C, m, x[u]);
+        for (int u = 0; u < kFlight; ++u)
+            if (row + u * rows < count) load(x[u], at + u * step);
+    }
     Finish<T> f;
     f.load(a, m, c);
 
@@ -459,12 +505,28 @@ __global__ __launch_bounds__(kThreads) void NormApplyKernel(const NormArgs a)
     if (row >= rows) return;
     f.prepare(a, sStat, g0, m, c);
     const int64_t pixel0 = n * a.pixels + p0;
-    for (int p = row; p < count; p += kFlight * rows)
+    int p = row;
+    for (; p + (2 * kFlight - 1) * rows < count; p += kFlight * rows)
     {
         Held<T> next[kFlight];
+        at += kFlight * step;
+        if (m > 0)
+        {
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) load(next[u], at + u * step);
+        }
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u) f.template store<MX4>(a, x[u], m, c, pixel0 + p + u * rows);
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u) x[u] = next[u];
+    }
+    for (; p < count; p += kFlight * rows)
+    {
+        Held<T> next[kFlight];
+        at += kFlight * step;
 #pragma unroll
         for (int u = 0; u < kFlight; ++u)
-            if (p + (kFlight + u) * rows < count) loadHeld(in + int64_t(p + (kFlight + u) * rows) * a.C, m, next[u]);
+            if (m > 0 && p + (kFlight + u) * rows < count) load(next[u], at + u * step);
 #pragma unroll
         for (int u = 0; u < kFlight; ++u)
             if (p + u * rows < count) f.template store<MX4>(a, x[u], m, c, pixel0 + p + u * rows);
@@ -480,7 +542,7 @@ struct MxArgs
     const uint8_t *codesIn, *scalesIn;
     uint8_t *codes, *scales;
     int64_t units;                    // rows x eighths of a row's blocks
-    int64_t columns;
+    int64_t columns, values;          // values: rows * columns
     unsigned rowUnits;                // 4 * blocks of a row
 };
 
@@ -501,8 +563,14 @@ __global__ __launch_bounds__(kThreads) void QuantizeKernel(const MxArgs a)
         if (unit >= a.units) break;                     // units come in fours: a block's threads leave together
         const unsigned r = at / a.rowUnits, col = at - r * a.rowUnits;
         const int64_t c = int64_t(col) * kVec;
+        const int m = int(max(int64_t(0), min(int64_t(kVec), a.columns - c)));
         float v[kVec];
-        loadUpTo8(static_cast<const T*>(a.in) + (row0 + r) * a.columns + c, int(max(int64_t(0), min(int64_t(kVec), a.columns - c))), v);
+        loadUpTo8(static_cast<const T*>(a.in) + (row0 + r) * a.columns + c, m, static_cast<const T*>(a.in) + a.values, v);
+        if (m < kVec)
+        {
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) v[i] = i < m ? v[i] : 0.0f;
+        }
         unsigned scale;
         const unsigned codes = mxQuantise(v, scale);
         *reinterpret_cast<unsigned*>(a.codes + unit * 4) = codes;
@@ -528,7 +596,11 @@ __global__ __launch_bounds__(kThreads) void DequantizeKernel(const MxArgs a)
         mxValues8(*reinterpret_cast<const unsigned*>(a.codesIn + unit * 4), v);
         const float f = mxFactor(a.scalesIn[unit >> 2]);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) v[i] *= f;
+        for (int i = 0; i < kVec; ++i)
+        {
+            v[i] *= f;
+            asm("" : "+v"(v[i]));                       // else the rounding to fp16 becomes part of a fused product + 0: -0 would lose its sign
+        }
         storeUpTo8(static_cast<T*>(a.out) + (row0 + r) * a.columns + c, int(max(int64_t(0), min(int64_t(kVec), a.columns - c))), v);
     }
 }
@@ -550,6 +622,7 @@ NormPlan planNorm(const ML::Operator& op, bool mx4)
     a.G = int(op.groups);
     a.groupC = a.C / a.G;
     a.pixels = int64_t(op.inputSizes[2]) * op.inputSizes[3];
+    a.values = a.pixels * a.C * op.inputSizes[0];
     a.epsilon = op.epsilon;
     a.activation = int(op.activation);
     p.images = op.inputSizes[0];
@@ -604,6 +677,7 @@ NormPlan planNorm(const ML::Operator& op, bool mx4)
     if (parts < (a.pixels + (1 << 22) - 1) >> 22) parts = (a.pixels + (1 << 22) - 1) >> 22;
     a.applyPixels = int((a.pixels + parts - 1) / parts);
     a.applyChunks = int((a.pixels + a.applyPixels - 1) / a.applyPixels);
+    a.stream = n * imageBytes > (int64_t(96) << 20);
     return p;
 }
 
@@ -637,7 +711,9 @@ hipError_t launchNorm(const NormPlan& p, hipStream_t s)
     ap.tiles = a.applyTiles;
     ap.byTiles = Divider(unsigned(a.applyTiles));
     ap.byChunks = Divider(unsigned(a.applyChunks));
-    hipLaunchKernelGGL(NormStatsKernel<T>, dim3(unsigned(statsGrid)), block, 0, s, st);
+    const bool whole = a.C % kVec == 0 && (a.tileGroups == a.G || (a.tileGroups * a.groupC) % kVec == 0);
+    if (whole) hipLaunchKernelGGL((NormStatsKernel<T, true>), dim3(unsigned(statsGrid)), block, 0, s, st);
+    else hipLaunchKernelGGL((NormStatsKernel<T, false>), dim3(unsigned(statsGrid)), block, 0, s, st);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (a.chunks > kJoin)
@@ -645,7 +721,8 @@ hipError_t launchNorm(const NormPlan& p, hipStream_t s)
         hipLaunchKernelGGL(NormJoinKernel, dim3(unsigned(a.groupsInAll)), dim3(64), 0, s, a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((NormApplyKernel<T, MX4>), dim3(unsigned(applyGrid)), block, 0, s, ap);
+    if (a.C % kVec == 0) hipLaunchKernelGGL((NormApplyKernel<T, MX4, true>), dim3(unsigned(applyGrid)), block, 0, s, ap);
+    else hipLaunchKernelGGL((NormApplyKernel<T, MX4, false>), dim3(unsigned(applyGrid)), block, 0, s, ap);
     return hipGetLastError();
 }
 
@@ -679,6 +756,7 @@ namespace {
 bool planMx(int64_t rows, int64_t columns, MxArgs& a, dim3& grid)
 {
     a.columns = columns;
+    a.values = rows * columns;
     a.rowUnits = unsigned(4 * mxBlocks(columns));
     a.units = rows * a.rowUnits;
     const int64_t blocks = (a.units + kThreads * kUnits - 1) / (kThreads * kUnits);
