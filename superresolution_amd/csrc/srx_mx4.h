@@ -125,6 +125,20 @@ __device__ __forceinline__ void store8(float* p, const float (&v)[8])
     __builtin_memcpy(p + 4, &b, 16);
 }
 // The same past the caches.
+__device__ __forceinline__ void streamIn8(const f16* p, float (&v)[8])
+{
+    typedef f16 f16x8u __attribute__((ext_vector_type(8), aligned(2)));
+    const f16x8u h = __builtin_nontemporal_load(reinterpret_cast<const f16x8u*>(p));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)h[i];
+}
+__device__ __forceinline__ void streamIn8(const float* p, float (&v)[8])
+{
+    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+    const f32x4u a = __builtin_nontemporal_load(reinterpret_cast<const f32x4u*>(p)), b = __builtin_nontemporal_load(reinterpret_cast<const f32x4u*>(p + 4));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+}
 __device__ __forceinline__ void streamOut8(f16* p, const float (&v)[8])
 {
     typedef f16 f16x8u __attribute__((ext_vector_type(8), aligned(2)));

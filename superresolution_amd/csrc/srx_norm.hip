@@ -17,6 +17,7 @@ namespace {
 
 constexpr int kVec = 8;               // channels of one thread
 constexpr int kTileC = kThreads * kVec;
+constexpr int64_t kStreamBytes = int64_t(96) << 20;   // a tensor that would fill the last-level cache (256 MB) passes by it
 constexpr int kJoin = 16;             // parts of an image that every workgroup of NormApplyKernel joins by itself
 
 struct NormArgs
@@ -112,6 +113,16 @@ __device__ __forceinline__ int lanesPerGroup(int groups, int threads)
     return lanes;
 }
 
+// f(activation as a constant): the branch is taken once, not for every value.
+template <int ACT> struct Constant { static constexpr int value = ACT; };
+template <typename F>
+__device__ __forceinline__ void forActivation(int activation, F&& f)
+{
+    if (activation == 0) f(Constant<0>{});
+    else if (activation == 1) f(Constant<1>{});
+    else f(Constant<2>{});
+}
+
 // What a thread needs to finish its eight channels, and the finish.
 template <typename T>
 struct Finish
@@ -139,12 +150,12 @@ struct Finish
         }
     }
     // m channels exist; `pixel` counts over all images, `column` is the thread's place among the pixel's eighths of blocks
-    template <bool MX4>
+    template <bool MX4, int ACT>
     __device__ __forceinline__ void store(const NormArgs& a, const Held<T>& x, int m, int c, int64_t pixel) const
     {
         float v[kVec];
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) v[i] = activate(fmaf(x.get(i) - mean[i], mul[i], add[i]), a.activation);
+        for (int i = 0; i < kVec; ++i) v[i] = activate(fmaf(x.get(i) - mean[i], mul[i], add[i]), ACT);
         if (MX4)
         {
             if (m < kVec)
@@ -273,9 +284,11 @@ __global__ __launch_bounds__(THREADS) void NormSlabKernel(const NormArgs a)
     __syncthreads();
     if (row >= rows) return;
     f.prepare(a, sStat, g0, m, c);
+    forActivation(a.activation, [&](auto act) {
 #pragma unroll
-    for (int i = 0; i < R; ++i)
-        if (row + i * rows < pixels) f.template store<MX4>(a, x[i], m, c, int64_t(n) * pixels + row + i * rows);
+        for (int i = 0; i < R; ++i)
+            if (row + i * rows < pixels) f.template store<MX4, act.value>(a, x[i], m, c, int64_t(n) * pixels + row + i * rows);
+    });
 }
 
 // Statistics of one part of one image for a range of whole groups.  A thread keeps eight channels and walks the
@@ -505,34 +518,36 @@ __global__ __launch_bounds__(kThreads) void NormApplyKernel(const NormArgs a)
     if (row >= rows) return;
     f.prepare(a, sStat, g0, m, c);
     const int64_t pixel0 = n * a.pixels + p0;
-    int p = row;
-    for (; p + (2 * kFlight - 1) * rows < count; p += kFlight * rows)
-    {
-        Held<T> next[kFlight];
-        at += kFlight * step;
-        if (m > 0)
+    forActivation(a.activation, [&](auto act) {
+        int p = row;
+        for (; p + (2 * kFlight - 1) * rows < count; p += kFlight * rows)
         {
+            Held<T> next[kFlight];
+            at += kFlight * step;
+            if (m > 0)
+            {
 #pragma unroll
-            for (int u = 0; u < kFlight; ++u) load(next[u], at + u * step);
+                for (int u = 0; u < kFlight; ++u) load(next[u], at + u * step);
+            }
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) f.template store<MX4, act.value>(a, x[u], m, c, pixel0 + p + u * rows);
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) x[u] = next[u];
         }
+        for (; p < count; p += kFlight * rows)
+        {
+            Held<T> next[kFlight];
+            at += kFlight * step;
 #pragma unroll
-        for (int u = 0; u < kFlight; ++u) f.template store<MX4>(a, x[u], m, c, pixel0 + p + u * rows);
+            for (int u = 0; u < kFlight; ++u)
+                if (m > 0 && p + (kFlight + u) * rows < count) load(next[u], at + u * step);
 #pragma unroll
-        for (int u = 0; u < kFlight; ++u) x[u] = next[u];
-    }
-    for (; p < count; p += kFlight * rows)
-    {
-        Held<T> next[kFlight];
-        at += kFlight * step;
+            for (int u = 0; u < kFlight; ++u)
+                if (p + u * rows < count) f.template store<MX4, act.value>(a, x[u], m, c, pixel0 + p + u * rows);
 #pragma unroll
-        for (int u = 0; u < kFlight; ++u)
-            if (m > 0 && p + (kFlight + u) * rows < count) load(next[u], at + u * step);
-#pragma unroll
-        for (int u = 0; u < kFlight; ++u)
-            if (p + u * rows < count) f.template store<MX4>(a, x[u], m, c, pixel0 + p + u * rows);
-#pragma unroll
-        for (int u = 0; u < kFlight; ++u) x[u] = next[u];
-    }
+            for (int u = 0; u < kFlight; ++u) x[u] = next[u];
+        }
+    });
 }
 
 struct MxArgs
@@ -544,35 +559,59 @@ struct MxArgs
     int64_t units;                    // rows x eighths of a row's blocks
     int64_t columns, values;          // values: rows * columns
     unsigned rowUnits;                // 4 * blocks of a row
+    Divider byRow;
+    int stream;                       // the unquantised side passes by the caches
 };
 
 constexpr int kUnits = 4;             // units per thread
 
 // A thread makes the codes of eight values; four neighbours share a block.
+// `row` and place of unit number `base + local` among the rows' units; local < 2^31, rem = base's place in its row.
+struct Unit
+{
+    int64_t row;
+    unsigned col;
+    __device__ __forceinline__ Unit(const MxArgs& a, int64_t row0, unsigned rem, unsigned local)
+    {
+        const unsigned at = rem + local, r = a.byRow(at);
+        row = row0 + r;
+        col = at - r * a.rowUnits;
+    }
+};
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void QuantizeKernel(const MxArgs a)
 {
     const int64_t base = int64_t(blockIdx.x) * (kThreads * kUnits);
     const int64_t row0 = base / a.rowUnits;
     const unsigned rem = unsigned(base - row0 * a.rowUnits);
+    const T* in = static_cast<const T*>(a.in);
+    float v[kUnits][kVec];
+    // all loads first; units come in fours: a block's threads are there or not together
 #pragma unroll
     for (int u = 0; u < kUnits; ++u)
     {
-        const unsigned at = rem + u * kThreads + threadIdx.x;
-        const int64_t unit = base + u * kThreads + threadIdx.x;
-        if (unit >= a.units) break;                     // units come in fours: a block's threads leave together
-        const unsigned r = at / a.rowUnits, col = at - r * a.rowUnits;
-        const int64_t c = int64_t(col) * kVec;
+        const unsigned local = u * kThreads + threadIdx.x;
+        if (base + local >= a.units) break;
+        const Unit unit(a, row0, rem, local);
+        const int64_t c = int64_t(unit.col) * kVec;
         const int m = int(max(int64_t(0), min(int64_t(kVec), a.columns - c)));
-        float v[kVec];
-        loadUpTo8(static_cast<const T*>(a.in) + (row0 + r) * a.columns + c, m, static_cast<const T*>(a.in) + a.values, v);
+        const T* p = in + unit.row * a.columns + c;
+        if (m == kVec && a.stream) streamIn8(p, v[u]);
+        else loadUpTo8(p, m, in + a.values, v[u]);
         if (m < kVec)
         {
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) v[i] = i < m ? v[i] : 0.0f;
+            for (int i = 0; i < kVec; ++i) v[u][i] = i < m ? v[u][i] : 0.0f;
         }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u)
+    {
+        const int64_t unit = base + u * kThreads + threadIdx.x;
+        if (unit >= a.units) break;
         unsigned scale;
-        const unsigned codes = mxQuantise(v, scale);
+        const unsigned codes = mxQuantise(v[u], scale);
         *reinterpret_cast<unsigned*>(a.codes + unit * 4) = codes;
         if ((threadIdx.x & 3) == 0) a.scales[unit >> 2] = uint8_t(scale);
     }
@@ -584,24 +623,35 @@ __global__ __launch_bounds__(kThreads) void DequantizeKernel(const MxArgs a)
     const int64_t base = int64_t(blockIdx.x) * (kThreads * kUnits);
     const int64_t row0 = base / a.rowUnits;
     const unsigned rem = unsigned(base - row0 * a.rowUnits);
+    unsigned codes[kUnits], scale[kUnits];
 #pragma unroll
     for (int u = 0; u < kUnits; ++u)
     {
-        const unsigned at = rem + u * kThreads + threadIdx.x;
         const int64_t unit = base + u * kThreads + threadIdx.x;
         if (unit >= a.units) break;
-        const unsigned r = at / a.rowUnits, col = at - r * a.rowUnits;
-        const int64_t c = int64_t(col) * kVec;
+        codes[u] = *reinterpret_cast<const unsigned*>(a.codesIn + unit * 4);
+        scale[u] = a.scalesIn[unit >> 2];
+    }
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u)
+    {
+        const unsigned local = u * kThreads + threadIdx.x;
+        if (base + local >= a.units) break;
+        const Unit unit(a, row0, rem, local);
+        const int64_t c = int64_t(unit.col) * kVec;
+        const int m = int(max(int64_t(0), min(int64_t(kVec), a.columns - c)));
         float v[kVec];
-        mxValues8(*reinterpret_cast<const unsigned*>(a.codesIn + unit * 4), v);
-        const float f = mxFactor(a.scalesIn[unit >> 2]);
+        mxValues8(codes[u], v);
+        const float f = mxFactor(scale[u]);
 #pragma unroll
         for (int i = 0; i < kVec; ++i)
         {
             v[i] *= f;
             asm("" : "+v"(v[i]));                       // else the rounding to fp16 becomes part of a fused product + 0: -0 would lose its sign
         }
-        storeUpTo8(static_cast<T*>(a.out) + (row0 + r) * a.columns + c, int(max(int64_t(0), min(int64_t(kVec), a.columns - c))), v);
+        T* p = static_cast<T*>(a.out) + unit.row * a.columns + c;
+        if (m == kVec && a.stream) streamOut8(p, v);
+        else storeUpTo8(p, m, v);
     }
 }
 
@@ -677,7 +727,7 @@ NormPlan planNorm(const ML::Operator& op, bool mx4)
     if (parts < (a.pixels + (1 << 22) - 1) >> 22) parts = (a.pixels + (1 << 22) - 1) >> 22;
     a.applyPixels = int((a.pixels + parts - 1) / parts);
     a.applyChunks = int((a.pixels + a.applyPixels - 1) / a.applyPixels);
-    a.stream = n * imageBytes > (int64_t(96) << 20);
+    a.stream = n * imageBytes > kStreamBytes;
     return p;
 }
 
@@ -753,12 +803,14 @@ hipError_t LaunchGroupNorm(const ML::Operator& op, const void* in, const void* s
 }
 
 namespace {
-bool planMx(int64_t rows, int64_t columns, MxArgs& a, dim3& grid)
+bool planMx(int64_t rows, int64_t columns, int bytes, MxArgs& a, dim3& grid)
 {
     a.columns = columns;
     a.values = rows * columns;
     a.rowUnits = unsigned(4 * mxBlocks(columns));
     a.units = rows * a.rowUnits;
+    a.byRow = Divider(a.rowUnits);
+    a.stream = a.values * bytes > kStreamBytes;
     const int64_t blocks = (a.units + kThreads * kUnits - 1) / (kThreads * kUnits);
     grid = dim3(unsigned(blocks));
     return blocks <= INT32_MAX;
@@ -770,7 +822,7 @@ hipError_t LaunchQuantizeMx4(ML::TensorDataType t, const void* in, int64_t rows,
 {
     MxArgs a{};
     dim3 grid;
-    if (!planMx(rows, columns, a, grid)) return hipErrorInvalidValue;
+    if (!planMx(rows, columns, t == ML::TensorDataType::FLOAT16 ? 2 : 4, a, grid)) return hipErrorInvalidValue;
     a.in = in;
     a.codes = codes;
     a.scales = scales;
@@ -784,7 +836,7 @@ hipError_t LaunchDequantizeMx4(ML::TensorDataType t, const uint8_t* codes, const
 {
     MxArgs a{};
     dim3 grid;
-    if (!planMx(rows, columns, a, grid)) return hipErrorInvalidValue;
+    if (!planMx(rows, columns, t == ML::TensorDataType::FLOAT16 ? 2 : 4, a, grid)) return hipErrorInvalidValue;
     a.codesIn = codes;
     a.scalesIn = scales;
     a.out = out;
