@@ -69,8 +69,9 @@ __device__ __forceinline__ unsigned loadByte(i32x4 from, unsigned offset)
 // Bias, activation and stores of a wave's 32 * FO channels of 32 * FP pixels.  A lane holds, for its pixel, output channels
 // 8 * (r >> 2) + 4 * h + (r & 3) of every 32; the wave turns 32 pixels at a time in its own part of LDS, so that whole
 // rows of channels are stored.
-template <typename T, int FO, int FP, int ACT>
-__device__ __forceinline__ void finish(const ConvMxArgs& a, const f32x16 (&acc)[FO][FP], const float* bias, uint8_t* mine, int64_t m0, int o0, int lane)
+// pixel(j, i): which pixel is number i of the j-th 32, or a negative number.
+template <typename T, int FO, int FP, int ACT, typename Pixel>
+__device__ __forceinline__ void finishAs(const ConvMxArgs& a, const f32x16 (&acc)[FO][FP], const float* bias, uint8_t* mine, int o0, int lane, Pixel&& pixel)
 {
     constexpr int kOutRow = 32 * FO * int(sizeof(T)) + 16;
     constexpr int kN = 16 / int(sizeof(T)), kPerRow = 32 * FO / kN;   // elements of a store, stores of a pixel
@@ -97,10 +98,10 @@ __device__ __forceinline__ void finish(const ConvMxArgs& a, const f32x16 (&acc)[
         for (int u = 0; u < 32 * kPerRow / 64; ++u)
         {
             const int px = (u * 64 + lane) / kPerRow, part = (u * 64 + lane) % kPerRow;
-            const int64_t m = m0 + 32 * j + px;
+            const int64_t m = pixel(j, px);
             const int o = o0 + part * kN;
             const uint4 v = *reinterpret_cast<const uint4*>(mine + px * kOutRow + part * 16);
-            if (m >= a.pixels) continue;
+            if (m < 0) continue;
             T* dst = out + m * a.O + o;
             if (o + kN <= a.O) __builtin_memcpy(dst, &v, 16);
             else
@@ -114,6 +115,14 @@ __device__ __forceinline__ void finish(const ConvMxArgs& a, const f32x16 (&acc)[
         }
         __builtin_amdgcn_wave_barrier();
     }
+}
+
+template <typename T, int FO, int FP, typename Pixel>
+__device__ __forceinline__ void finish(const ConvMxArgs& a, const f32x16 (&acc)[FO][FP], const float* bias, uint8_t* mine, int o0, int lane, Pixel&& pixel)
+{
+    if (a.activation == 0) finishAs<T, FO, FP, 0>(a, acc, bias, mine, o0, lane, pixel);
+    else if (a.activation == 1) finishAs<T, FO, FP, 1>(a, acc, bias, mine, o0, lane, pixel);
+    else finishAs<T, FO, FP, 2>(a, acc, bias, mine, o0, lane, pixel);
 }
 
 // A workgroup makes BO output channels of BP pixels; a wave makes 32 * FO channels of 32 * FP pixels.
@@ -392,9 +401,10 @@ __global__ __launch_bounds__(THREADS) void ConvMxKernel(const ConvMxArgs a)
     // (also the loads of the chunk after the last, which write zeros)
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     uint8_t* mine = lds + wave * 32 * kOutRow;
-    if (a.activation == 0) finish<T, FO, FP, 0>(a, acc, sBias + wo, mine, m0 + wp, o0 + wo, lane);
-    else if (a.activation == 1) finish<T, FO, FP, 1>(a, acc, sBias + wo, mine, m0 + wp, o0 + wo, lane);
-    else finish<T, FO, FP, 2>(a, acc, sBias + wo, mine, m0 + wp, o0 + wo, lane);
+    finish<T, FO, FP>(a, acc, sBias + wo, mine, o0 + wo, lane, [&](int j, int i) -> int64_t {
+        const int64_t m = m0 + wp + 32 * j + i;
+        return m < a.pixels ? m : -1;
+    });
 }
 
 // 16 bytes a lane, by the compiler's own count.
@@ -532,6 +542,218 @@ hipError_t launchRows(bool half, const ConvMxArgs& a, hipStream_t s)
     return half ? launchRows<f16, FP>(a, words, s) : launchRows<float, FP>(a, words, s);
 }
 
+// Filters of several taps over few channels: the tiles above would read every pixel once for each tap.  Here a workgroup
+// keeps the filters of 32 * FO output channels in LDS, and walks over tiles of 8 rows of 32 pixels: the window that a tile's
+// taps see is read once (NL loads of 16 bytes a thread), while the tile before it is multiplied.  A wave makes two rows.
+// Block kb of the reduction (tap kb / blocks) of the filters lies at kb * 32 * FO + channel; of the window at pixel * blocks +
+// (block, exclusive-or'ed with bits of the pixel's column so that neighbouring lanes spread over the banks).
+struct WindowArgs
+{
+    int winW, units;                  // window columns; window rows * columns * blocks
+    int steps;                        // pairs of blocks of the reduction
+    int swizzleShift, swizzleMask;
+    int tilesX, tilesY, tiles, slots; // tiles of all images; workgroups for each channel tile
+    Divider byTilesX, byTilesY, byWinRow;
+};
+constexpr int kWinH = 8, kWinW = 32;  // pixels of a tile
+
+template <typename T, int FO, int NL>
+struct WindowLds
+{
+    static constexpr int kBO = 32 * FO, kUnits = NL * kThreads, kOutRow = 32 * FO * int(sizeof(T)) + 16;
+    // places: two windows (codes, scales), the turn of the results, bias, table of the window's units, nothing, filters
+    static constexpr int kWindow = kUnits * 17, kTurn = 2 * kWindow, kBias = kTurn + 4 * 32 * kOutRow, kTable = kBias + kBO * 4,
+                         kNothing = kTable + kUnits * 4, kFilter = kNothing + 32;
+    static int bytes(int steps) { return kFilter + 2 * steps * kBO * 17; }
+};
+
+template <typename T, int FO, int NL>
+__global__ __launch_bounds__(kThreads) void ConvMxWindowKernel(const ConvMxArgs a, const WindowArgs w)
+{
+    using L = WindowLds<T, FO, NL>;
+    constexpr int kBO = L::kBO, FP = 2;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
+    const unsigned ldsAt = unsigned(uintptr_t((__attribute__((address_space(3))) uint8_t*)dyn));
+    // all channel tiles of a slot on one XCD, neighbouring slots on different ones
+    const unsigned turn = blockIdx.x >> 3, round = a.byTilesO(turn);
+    const int o0 = int(turn - round * a.tilesO) * kBO, slotNumber = int(round * 8 + (blockIdx.x & 7));
+    const int pixelBytes = a.blocks * kMxBytes;
+    const unsigned rowBytes = unsigned(a.W) * unsigned(pixelBytes);
+    const int filterScales = L::kFilter + 2 * w.steps * kBO * 16;
+
+    // the filters, once
+    {
+        const i32x4 wd = descriptor(a.wCodes + int64_t(o0) * a.total * kMxBytes, kRange), vd = descriptor(a.wScales + int64_t(o0) * a.total, kRange >> 4);
+        for (int u = wave * 64; u < 2 * w.steps * kBO; u += kThreads)
+        {
+            const int kb = (u + lane) / kBO, o = (u + lane) % kBO;
+            const unsigned off = kb < a.total && o0 + o < a.O ? unsigned(o * a.total + kb) * kMxBytes : kRange;
+            loadToLds(wd, off, ldsAt + L::kFilter + u * 16);
+            dyn[filterScales + u + lane] = uint8_t(loadByte(vd, off / kMxBytes));
+        }
+        float* bias = reinterpret_cast<float*>(dyn + L::kBias);
+        if (tid < kBO) bias[tid] = a.bias && o0 + tid < a.O ? (float)static_cast<const T*>(a.bias)[o0 + tid] : 0.0f;
+        if (tid < 8) reinterpret_cast<unsigned*>(dyn + L::kNothing)[tid] = 0;
+        // unit of the window: row, column, block (swizzled), or a row that no image has
+        unsigned* table = reinterpret_cast<unsigned*>(dyn + L::kTable);
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+        {
+            const unsigned u = i * kThreads + tid, row = w.byWinRow(u), rest = u - row * unsigned(w.winW * a.blocks);
+            const unsigned col = a.byBlocks(rest), block = (rest - col * unsigned(a.blocks)) ^ ((col >> w.swizzleShift) & unsigned(w.swizzleMask));
+            table[u] = int(u) < w.units ? row | col << 8 | block << 16 : 0xffffffffu;
+        }
+    }
+    __syncthreads();
+
+    uint8_t scale[NL];
+    const auto fetch = [&](int tile, int window) {
+        const unsigned q = w.byTilesX(unsigned(tile)), n = w.byTilesY(q);
+        const int x0 = int(unsigned(tile) - q * unsigned(w.tilesX)) * kWinW - a.padLeft, y0 = int(q - n * unsigned(w.tilesY)) * kWinH - a.padTop;
+        const int64_t first = (int64_t(n) * a.H + y0) * a.W + x0;
+        const i32x4 xd = descriptor(a.codes + first * pixelBytes, kRange), zd = descriptor(a.scales + first * a.blocks, kRange >> 4);
+        const unsigned* table = reinterpret_cast<const unsigned*>(dyn + L::kTable);
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+        {
+            const unsigned t = table[i * kThreads + tid], row = t & 255u, col = (t >> 8) & 255u, block = (t >> 16) & 255u;
+            const bool in = int(t) >= 0 && unsigned(y0 + int(row)) < unsigned(a.H) && unsigned(x0 + int(col)) < unsigned(a.W);
+            const unsigned off = in ? row * rowBytes + col * unsigned(pixelBytes) + block * kMxBytes : kRange;
+            loadToLds(xd, off, ldsAt + window + (i * kThreads + wave * 64) * 16);
+            scale[i] = uint8_t(loadByte(zd, off / kMxBytes));
+        }
+    };
+
+    int window = 0;
+    if (slotNumber < w.tiles) fetch(slotNumber, 0);
+    for (int tile = slotNumber; tile < w.tiles; tile += w.slots)
+    {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) dyn[window + L::kUnits * 16 + i * kThreads + tid] = scale[i];
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (tile + w.slots < w.tiles) fetch(tile + w.slots, L::kWindow - window);
+
+        f32x16 acc[FO][FP];
+#pragma unroll
+        for (int i = 0; i < FO; ++i)
+#pragma unroll
+            for (int j = 0; j < FP; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+
+        // Step s multiplies the blocks 2 s (lanes 0-31) and 2 s + 1 (lanes 32-63); the next step's operands are read meanwhile.
+        int kx = 0, ky = 0, cb = 0, kb = 0;                             // of the next block
+        uint4 wf[2][FO], xf[2][FP];
+        unsigned ws[2][FO], xs[2][FP];
+        const auto read = [&](int set) {
+            const int kx0 = kx, ky0 = ky, cb0 = cb, at = kb;
+            const auto next = [&]() {
+                ++kb;
+                const bool col = ++cb == a.blocks;
+                cb = col ? 0 : cb;
+                kx += col;
+                const bool row = kx == a.kw;
+                kx = row ? 0 : kx;
+                ky += row;
+            };
+            next();
+            const int px = l + (h ? kx : kx0), wrow = 2 * wave + (h ? ky : ky0), block = h ? cb : cb0;
+            const bool pad = h && kb >= a.total;                        // an odd reduction's last half step
+            const int unit = (wrow * w.winW + px) * a.blocks + (block ^ ((px >> w.swizzleShift) & w.swizzleMask));
+            next();
+#pragma unroll
+            for (int i = 0; i < FO; ++i)
+            {
+                const int f = (at + h) * kBO + 32 * i + l;
+                wf[set][i] = *reinterpret_cast<const uint4*>(dyn + L::kFilter + f * 16);
+                ws[set][i] = dyn[filterScales + f];
+            }
+#pragma unroll
+            for (int j = 0; j < FP; ++j)
+            {
+                const int u = unit + j * w.winW * a.blocks;
+                xf[set][j] = *reinterpret_cast<const uint4*>(dyn + (pad ? L::kNothing : window + u * 16));
+                xs[set][j] = dyn[pad ? L::kNothing : window + L::kUnits * 16 + u];
+            }
+        };
+#define SRX_MULTIPLY(SET)                                                                                              \
+    _Pragma("unroll") for (int i = 0; i < FO; ++i)                                                                     \
+        _Pragma("unroll") for (int j = 0; j < FP; ++j)                                                                 \
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(wf[SET][i]), widen(xf[SET][j]), acc[i][j], 4, 4, 0, ws[SET][i], 0, xs[SET][j]);
+        read(0);
+        int left = w.steps;
+        for (; left > 2; left -= 2)
+        {
+            read(1);
+            SRX_MULTIPLY(0)
+            read(0);
+            SRX_MULTIPLY(1)
+        }
+        if (left > 1)
+        {
+            read(1);
+            SRX_MULTIPLY(0)
+            SRX_MULTIPLY(1)
+        }
+        else { SRX_MULTIPLY(0) }
+#undef SRX_MULTIPLY
+
+        const unsigned q = w.byTilesX(unsigned(tile)), n = w.byTilesY(q);
+        const int x0 = int(unsigned(tile) - q * unsigned(w.tilesX)) * kWinW, y0 = int(q - n * unsigned(w.tilesY)) * kWinH + 2 * wave;
+        finish<T, FO, FP>(a, acc, reinterpret_cast<const float*>(dyn + L::kBias), dyn + L::kTurn + wave * 32 * L::kOutRow, o0, lane, [&](int j, int i) -> int64_t {
+            return y0 + j < a.H && x0 + i < a.W ? (int64_t(n) * a.H + y0 + j) * a.W + x0 + i : -1;
+        });
+        window = L::kWindow - window;
+    }
+    // nothing is in flight: the last tile fetched no other
+}
+
+template <typename T, int FO, int NL>
+hipError_t launchWindow(const ConvMxArgs& args, WindowArgs w, hipStream_t s)
+{
+    using L = WindowLds<T, FO, NL>;
+    ConvMxArgs a = args;
+    a.tilesO = (a.O + L::kBO - 1) / L::kBO;
+    a.byTilesO = Divider(unsigned(a.tilesO));
+    const void* kernel = reinterpret_cast<const void*>(ConvMxWindowKernel<T, FO, NL>);
+    const int lds = L::bytes(w.steps), most = 160 << 10;
+    if (lds > most) return hipErrorInvalidConfiguration;
+    const hipError_t e = dev::ensureDynamicLds(kernel, most);
+    if (e != hipSuccess) return e;
+    // as many workgroups as the device holds at a time, in eights
+    const int perCu = FO == 2 ? 2 : 3;                                  // by registers
+    const int resident = 256 * (most / lds < perCu ? most / lds : perCu);
+    int slots = (resident / a.tilesO + 7) / 8 * 8;
+    if (slots > (w.tiles + 7) / 8 * 8) slots = (w.tiles + 7) / 8 * 8;
+    w.slots = slots;
+    hipLaunchKernelGGL((ConvMxWindowKernel<T, FO, NL>), dim3(unsigned(slots * a.tilesO)), dim3(kThreads), lds, s, a, w);
+    return hipGetLastError();
+}
+// hipErrorInvalidConfiguration, and no launch, where the filters or the window do not fit.
+template <int FO>
+hipError_t launchWindow(bool half, const ConvMxArgs& a, hipStream_t s)
+{
+    if (a.blocks > 4 || (int64_t(a.taps / a.kw + kWinH) * a.W + a.kw + kWinW) * a.blocks * kMxBytes >= int64_t(kRange)) return hipErrorInvalidConfiguration;
+    WindowArgs w{};
+    const int winH = kWinH + a.taps / a.kw - 1;
+    w.winW = kWinW + a.kw - 1;
+    w.units = winH * w.winW * a.blocks;
+    w.steps = (a.total + 1) / 2;
+    w.swizzleShift = a.blocks == 4 ? 2 : 3;
+    w.swizzleMask = a.blocks == 4 ? 3 : a.blocks == 2 ? 1 : 0;
+    w.tilesX = (a.W + kWinW - 1) / kWinW;
+    w.tilesY = (a.H + kWinH - 1) / kWinH;
+    w.tiles = a.pixels / (a.H * a.W) * w.tilesX * w.tilesY;
+    w.byTilesX = Divider(unsigned(w.tilesX));
+    w.byTilesY = Divider(unsigned(w.tilesY));
+    w.byWinRow = Divider(unsigned(w.winW * a.blocks));
+    if (w.units <= 2 * kThreads) return half ? launchWindow<f16, FO, 2>(a, w, s) : launchWindow<float, FO, 2>(a, w, s);
+    if (w.units <= 4 * kThreads) return half ? launchWindow<f16, FO, 4>(a, w, s) : launchWindow<float, FO, 4>(a, w, s);
+    if (w.units > 7 * kThreads) return hipErrorInvalidConfiguration;
+    return half ? launchWindow<f16, FO, 7>(a, w, s) : launchWindow<float, FO, 7>(a, w, s);
+}
+
 template <typename T, int THREADS, int BO, int BP, int FO, int FP>
 hipError_t launch(const ConvMxArgs& args, hipStream_t s)
 {
@@ -598,6 +820,11 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
         return rows == 4 ? launchRows<4>(half, a, s) : rows == 2 ? launchRows<2>(half, a, s) : launchRows<1>(half, a, s);
     // The largest tile that leaves no CU without one: 256x256 reads a quarter of what 64x64 does (512 -> 512 channels, 3x3,
     // 256x256: 92 instead of 158 us), but 64 such tiles for 2048 -> 2048 channels, 1x1, 2048 pixels take 19 instead of 11.6.
+    if (a.taps > 1 && a.blocks <= 4 && a.W >= 16 && tiles(64, 256) >= 256)
+    {
+        const hipError_t e = a.O <= 32 ? launchWindow<1>(half, a, s) : launchWindow<2>(half, a, s);
+        if (e != hipErrorInvalidConfiguration) return e;
+    }
     if (a.O > 128 && tiles(256, 256) >= 256) return launch<512, 256, 256, 2, 4>(half, a, s);
     if (a.O > 64 && tiles(128, 64) >= 512) return launch<256, 128, 64, 2, 1>(half, a, s);
     if (a.O <= 32 && tiles(32, 128) >= 256) return launch<256, 32, 128, 1, 1>(half, a, s);

@@ -387,7 +387,10 @@ CONVS = [(1, 1, 1, 1, 1, 1, 1), (1, 32, 1, 1, 16, 1, 1), (1, 33, 1, 1, 5, 1, 1),
          (1, 2049, 1, 17, 33, 1, 1), (1, 64, 9, 11, 64, 3, 3), (2, 75, 13, 9, 33, 5, 2), (1, 96, 20, 30, 130, 3, 3), (3, 16, 7, 7, 8, 7, 7),
          (1, 256, 24, 24, 256, 3, 3), (1, 128, 40, 33, 70, 1, 1), (1, 300, 16, 16, 200, 2, 3), (2, 64, 50, 70, 3, 3, 3), (1, 3, 21, 33, 32, 5, 5),
          (1, 8, 1, 40, 12, 1, 7), (1, 8, 40, 1, 12, 7, 1), (1, 8, 2, 2, 12, 7, 7), (1, 288, 30, 31, 512, 1, 1), (4, 160, 33, 17, 96, 3, 1),
-         (1, 1024, 6, 6, 128, 3, 3), (1, 32, 130, 140, 40, 1, 1), (1, 512, 9, 15, 513, 1, 1), (1, 700, 1, 300, 260, 1, 1)]
+         (1, 1024, 6, 6, 128, 3, 3), (1, 32, 130, 140, 40, 1, 1), (1, 512, 9, 15, 513, 1, 1), (1, 700, 1, 300, 260, 1, 1),
+         (1, 64, 150, 170, 64, 3, 3), (1, 32, 140, 150, 70, 3, 3), (2, 96, 90, 110, 40, 3, 3), (1, 128, 130, 140, 32, 3, 3), (1, 20, 200, 160, 24, 5, 5),
+         (1, 50, 150, 150, 64, 5, 5), (1, 8, 150, 170, 33, 1, 7), (1, 100, 160, 150, 20, 2, 2), (1, 30, 150, 170, 10, 7, 7), (1, 64, 16, 5000, 24, 3, 3),
+         (1, 40, 3000, 17, 130, 3, 2), (1, 256, 256, 258, 256, 1, 1), (1, 130, 260, 256, 300, 1, 1), (1, 65, 150, 130, 160, 2, 2)]
 
 
 @pytest.mark.parametrize("dtype", [0, 1])
