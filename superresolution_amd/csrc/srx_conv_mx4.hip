@@ -68,16 +68,18 @@ __device__ __forceinline__ unsigned loadByte(i32x4 from, unsigned offset)
 
 // Bias, activation and stores of a wave's 32 * FO channels of 32 * FP pixels.  A lane holds, for its pixel, output channels
 // 8 * (r >> 2) + 4 * h + (r & 3) of every 32; the wave turns 32 pixels at a time in its own part of LDS, so that whole
-// rows of channels are stored.
-// pixel(j, i): which pixel is number i of the j-th 32, or a negative number.
-template <typename T, int FO, int FP, int ACT, typename Pixel>
-__device__ __forceinline__ void finishAs(const ConvMxArgs& a, const f32x16 (&acc)[FO][FP], const float* bias, uint8_t* mine, int o0, int lane, Pixel&& pixel)
+// rows of channels are stored.  place(j, to, count): where channel o0 of the first of the j-th 32 pixels goes, and how many
+// of them exist (both the same for all lanes).
+template <typename T, int FO, int FP, int ACT, typename Place>
+__device__ __forceinline__ void finishAs(const ConvMxArgs& a, const f32x16 (&acc)[FO][FP], const float* bias, uint8_t* mine, int o0, int lane, Place&& place)
 {
     constexpr int kOutRow = 32 * FO * int(sizeof(T)) + 16;
     constexpr int kN = 16 / int(sizeof(T)), kPerRow = 32 * FO / kN;   // elements of a store, stores of a pixel
+    constexpr int kPass = 64 / kPerRow;                               // pixels stored at a time
     typedef T T4 __attribute__((ext_vector_type(4)));
-    const int h = lane >> 5, l = lane & 31;
-    T* out = static_cast<T*>(a.out);
+    const int h = lane >> 5, l = lane & 31, px = lane / kPerRow, part = lane % kPerRow;
+    const int channels = a.O - o0 - part * kN;                        // that exist from this lane's first on
+    const unsigned lanes = unsigned(px) * unsigned(a.O) * unsigned(sizeof(T)) + part * 16, pass = unsigned(kPass) * unsigned(a.O) * unsigned(sizeof(T));
 #pragma unroll
     for (int j = 0; j < FP; ++j)
     {
@@ -94,35 +96,38 @@ __device__ __forceinline__ void finishAs(const ConvMxArgs& a, const f32x16 (&acc
                 *reinterpret_cast<T4*>(mine + l * kOutRow + o * int(sizeof(T))) = v4;
             }
         __builtin_amdgcn_wave_barrier();
+        uint8_t* to;
+        int count;
+        place(j, to, count);
 #pragma unroll
-        for (int u = 0; u < 32 * kPerRow / 64; ++u)
+        for (int u = 0; u < 32 / kPass; ++u)
         {
-            const int px = (u * 64 + lane) / kPerRow, part = (u * 64 + lane) % kPerRow;
-            const int64_t m = pixel(j, px);
-            const int o = o0 + part * kN;
-            const uint4 v = *reinterpret_cast<const uint4*>(mine + px * kOutRow + part * 16);
-            if (m < 0) continue;
-            T* dst = out + m * a.O + o;
-            if (o + kN <= a.O) __builtin_memcpy(dst, &v, 16);
+            const uint4 v = *reinterpret_cast<const uint4*>(mine + (u * kPass + px) * kOutRow + part * 16);
+            if (u * kPass + px >= count) continue;
+            uint8_t* dst = to + (lanes + u * pass);
+            if (channels >= kN)
+            {
+                typedef unsigned u32x4_at __attribute__((ext_vector_type(4), aligned(2)));
+                *reinterpret_cast<u32x4_at*>(dst) = u32x4_at{v.x, v.y, v.z, v.w};
+            }
             else
             {
                 T e[kN];
                 __builtin_memcpy(e, &v, 16);
 #pragma unroll
                 for (int k = 0; k < kN; ++k)
-                    if (o + k < a.O) dst[k] = e[k];
+                    if (k < channels) reinterpret_cast<T*>(dst)[k] = e[k];
             }
         }
         __builtin_amdgcn_wave_barrier();
     }
 }
-
-template <typename T, int FO, int FP, typename Pixel>
-__device__ __forceinline__ void finish(const ConvMxArgs& a, const f32x16 (&acc)[FO][FP], const float* bias, uint8_t* mine, int o0, int lane, Pixel&& pixel)
+template <typename T, int FO, int FP, typename Place>
+__device__ __forceinline__ void finish(const ConvMxArgs& a, const f32x16 (&acc)[FO][FP], const float* bias, uint8_t* mine, int o0, int lane, Place&& place)
 {
-    if (a.activation == 0) finishAs<T, FO, FP, 0>(a, acc, bias, mine, o0, lane, pixel);
-    else if (a.activation == 1) finishAs<T, FO, FP, 1>(a, acc, bias, mine, o0, lane, pixel);
-    else finishAs<T, FO, FP, 2>(a, acc, bias, mine, o0, lane, pixel);
+    if (a.activation == 0) finishAs<T, FO, FP, 0>(a, acc, bias, mine, o0, lane, place);
+    else if (a.activation == 1) finishAs<T, FO, FP, 1>(a, acc, bias, mine, o0, lane, place);
+    else finishAs<T, FO, FP, 2>(a, acc, bias, mine, o0, lane, place);
 }
 
 // A workgroup makes BO output channels of BP pixels; a wave makes 32 * FO channels of 32 * FP pixels.
@@ -401,9 +406,10 @@ __global__ __launch_bounds__(THREADS) void ConvMxKernel(const ConvMxArgs a)
     // (also the loads of the chunk after the last, which write zeros)
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     uint8_t* mine = lds + wave * 32 * kOutRow;
-    finish<T, FO, FP>(a, acc, sBias + wo, mine, o0 + wo, lane, [&](int j, int i) -> int64_t {
-        const int64_t m = m0 + wp + 32 * j + i;
-        return m < a.pixels ? m : -1;
+    finish<T, FO, FP>(a, acc, sBias + wo, mine, o0 + wo, lane, [&](int j, uint8_t*& to, int& count) {
+        const int64_t m = m0 + wp + 32 * j;
+        to = static_cast<uint8_t*>(a.out) + (m * a.O + o0 + wo) * int64_t(sizeof(T));
+        count = int(min(int64_t(32), a.pixels - m));
     });
 }
 
@@ -542,16 +548,16 @@ hipError_t launchRows(bool half, const ConvMxArgs& a, hipStream_t s)
     return half ? launchRows<f16, FP>(a, words, s) : launchRows<float, FP>(a, words, s);
 }
 
-// Filters of several taps over few channels: the tiles above would read every pixel once for each tap.  Here a workgroup
+// Up to two blocks a pixel: the tiles above would read every pixel once for each tap.  Here a workgroup
 // keeps the filters of 32 * FO output channels in LDS, and walks over tiles of 8 rows of 32 pixels: the window that a tile's
 // taps see is read once (NL loads of 16 bytes a thread), while the tile before it is multiplied.  A wave makes two rows.
 // Block kb of the reduction (tap kb / blocks) of the filters lies at kb * 32 * FO + channel; of the window at pixel * blocks +
-// (block, exclusive-or'ed with bits of the pixel's column so that neighbouring lanes spread over the banks).
+// block, with the two blocks of a pixel exchanged in every other eight columns: 16 neighbouring lanes then read all banks.
 struct WindowArgs
 {
     int winW, units;                  // window columns; window rows * columns * blocks
     int steps;                        // pairs of blocks of the reduction
-    int swizzleShift, swizzleMask;
+    int swizzle;                      // two blocks a pixel: eight columns in sixteen have theirs exchanged
     int tilesX, tilesY, tiles, slots; // tiles of all images; workgroups for each channel tile
     Divider byTilesX, byTilesY, byWinRow;
 };
@@ -563,8 +569,10 @@ struct WindowLds
     static constexpr int kBO = 32 * FO, kUnits = NL * kThreads, kOutRow = 32 * FO * int(sizeof(T)) + 16;
     // places: two windows (codes, scales), the turn of the results, bias, table of the window's units, nothing, filters
     static constexpr int kWindow = kUnits * 17, kTurn = 2 * kWindow, kBias = kTurn + 4 * 32 * kOutRow, kTable = kBias + kBO * 4,
-                         kNothing = kTable + kUnits * 4, kFilter = kNothing + 32;
-    static int bytes(int steps) { return kFilter + 2 * steps * kBO * 17; }
+                         kNothing = kTable + kUnits * 4, kSteps = kNothing + 32;
+    // then, for each step, the lanes' units (for the first wave) and the filters
+    __host__ __device__ static constexpr int filters(int steps) { return kSteps + steps * 256; }
+    static constexpr int bytes(int steps) { return filters(steps) + 2 * steps * kBO * 17; }
 };
 
 template <typename T, int FO, int NL>
@@ -580,7 +588,7 @@ __global__ __launch_bounds__(kThreads) void ConvMxWindowKernel(const ConvMxArgs 
     const int o0 = int(turn - round * a.tilesO) * kBO, slotNumber = int(round * 8 + (blockIdx.x & 7));
     const int pixelBytes = a.blocks * kMxBytes;
     const unsigned rowBytes = unsigned(a.W) * unsigned(pixelBytes);
-    const int filterScales = L::kFilter + 2 * w.steps * kBO * 16;
+    const int filters = L::filters(w.steps), filterScales = filters + 2 * w.steps * kBO * 16;
 
     // the filters, once
     {
@@ -589,7 +597,7 @@ __global__ __launch_bounds__(kThreads) void ConvMxWindowKernel(const ConvMxArgs 
         {
             const int kb = (u + lane) / kBO, o = (u + lane) % kBO;
             const unsigned off = kb < a.total && o0 + o < a.O ? unsigned(o * a.total + kb) * kMxBytes : kRange;
-            loadToLds(wd, off, ldsAt + L::kFilter + u * 16);
+            loadToLds(wd, off, ldsAt + filters + u * 16);
             dyn[filterScales + u + lane] = uint8_t(loadByte(vd, off / kMxBytes));
         }
         float* bias = reinterpret_cast<float*>(dyn + L::kBias);
@@ -601,8 +609,15 @@ __global__ __launch_bounds__(kThreads) void ConvMxWindowKernel(const ConvMxArgs 
         for (int i = 0; i < NL; ++i)
         {
             const unsigned u = i * kThreads + tid, row = w.byWinRow(u), rest = u - row * unsigned(w.winW * a.blocks);
-            const unsigned col = a.byBlocks(rest), block = (rest - col * unsigned(a.blocks)) ^ ((col >> w.swizzleShift) & unsigned(w.swizzleMask));
+            const unsigned col = a.byBlocks(rest), block = (rest - col * unsigned(a.blocks)) ^ ((col >> 3) & unsigned(w.swizzle));
             table[u] = int(u) < w.units ? row | col << 8 | block << 16 : 0xffffffffu;
+        }
+        // Step s multiplies the blocks 2 s (lanes 0-31) and 2 s + 1 (lanes 32-63); an odd reduction's last half step has none.
+        for (int u = tid; u < w.steps * 64; u += kThreads)
+        {
+            const int kb = (u >> 6) * 2 + ((u >> 5) & 1), tap = int(a.byBlocks(unsigned(kb))), ky = int(a.byKw(unsigned(tap)));
+            const int px = (u & 31) + tap - ky * a.kw, block = (kb - tap * a.blocks) ^ ((px >> 3) & w.swizzle);
+            reinterpret_cast<int*>(dyn + L::kSteps)[u] = kb < a.total ? (ky * w.winW + px) * a.blocks + block : -1;
         }
     }
     __syncthreads();
@@ -642,40 +657,34 @@ __global__ __launch_bounds__(kThreads) void ConvMxWindowKernel(const ConvMxArgs 
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
-        // Step s multiplies the blocks 2 s (lanes 0-31) and 2 s + 1 (lanes 32-63); the next step's operands are read meanwhile.
-        int kx = 0, ky = 0, cb = 0, kb = 0;                             // of the next block
+        // the next step's operands are read while one is multiplied
         uint4 wf[2][FO], xf[2][FP];
         unsigned ws[2][FO], xs[2][FP];
+        const int rowUnits = w.winW * a.blocks;
+        const uint8_t* stepAt = dyn + L::kSteps + lane * 4;
+        const uint8_t* filterAt = dyn + filters + (h * kBO + l) * 16;
+        const uint8_t* filterScaleAt = dyn + filterScales + h * kBO + l;
+        const uint8_t* windowAt = dyn + window + 2 * wave * rowUnits * 16;
+        const uint8_t* windowScaleAt = dyn + window + L::kUnits * 16 + 2 * wave * rowUnits;
+        int unit = *reinterpret_cast<const int*>(stepAt);
         const auto read = [&](int set) {
-            const int kx0 = kx, ky0 = ky, cb0 = cb, at = kb;
-            const auto next = [&]() {
-                ++kb;
-                const bool col = ++cb == a.blocks;
-                cb = col ? 0 : cb;
-                kx += col;
-                const bool row = kx == a.kw;
-                kx = row ? 0 : kx;
-                ky += row;
-            };
-            next();
-            const int px = l + (h ? kx : kx0), wrow = 2 * wave + (h ? ky : ky0), block = h ? cb : cb0;
-            const bool pad = h && kb >= a.total;                        // an odd reduction's last half step
-            const int unit = (wrow * w.winW + px) * a.blocks + (block ^ ((px >> w.swizzleShift) & w.swizzleMask));
-            next();
 #pragma unroll
             for (int i = 0; i < FO; ++i)
             {
-                const int f = (at + h) * kBO + 32 * i + l;
-                wf[set][i] = *reinterpret_cast<const uint4*>(dyn + L::kFilter + f * 16);
-                ws[set][i] = dyn[filterScales + f];
+                wf[set][i] = *reinterpret_cast<const uint4*>(filterAt + 512 * i);
+                ws[set][i] = filterScaleAt[32 * i];
             }
+            filterAt += 2 * kBO * 16;
+            filterScaleAt += 2 * kBO;
 #pragma unroll
             for (int j = 0; j < FP; ++j)
             {
-                const int u = unit + j * w.winW * a.blocks;
-                xf[set][j] = *reinterpret_cast<const uint4*>(dyn + (pad ? L::kNothing : window + u * 16));
-                xs[set][j] = dyn[pad ? L::kNothing : window + L::kUnits * 16 + u];
+                const int u = unit + j * rowUnits;
+                xf[set][j] = *reinterpret_cast<const uint4*>(unit < 0 ? dyn + L::kNothing : windowAt + u * 16);
+                xs[set][j] = unit < 0 ? dyn[L::kNothing] : windowScaleAt[u];
             }
+            stepAt += 256;
+            unit = *reinterpret_cast<const int*>(stepAt);               // (after the last step: of the filters, and not used)
         };
 #define SRX_MULTIPLY(SET)                                                                                              \
     _Pragma("unroll") for (int i = 0; i < FO; ++i)                                                                     \
@@ -701,8 +710,9 @@ __global__ __launch_bounds__(kThreads) void ConvMxWindowKernel(const ConvMxArgs 
 
         const unsigned q = w.byTilesX(unsigned(tile)), n = w.byTilesY(q);
         const int x0 = int(unsigned(tile) - q * unsigned(w.tilesX)) * kWinW, y0 = int(q - n * unsigned(w.tilesY)) * kWinH + 2 * wave;
-        finish<T, FO, FP>(a, acc, reinterpret_cast<const float*>(dyn + L::kBias), dyn + L::kTurn + wave * 32 * L::kOutRow, o0, lane, [&](int j, int i) -> int64_t {
-            return y0 + j < a.H && x0 + i < a.W ? (int64_t(n) * a.H + y0 + j) * a.W + x0 + i : -1;
+        finish<T, FO, FP>(a, acc, reinterpret_cast<const float*>(dyn + L::kBias), dyn + L::kTurn + wave * 32 * L::kOutRow, o0, lane, [&](int j, uint8_t*& to, int& count) {
+            to = static_cast<uint8_t*>(a.out) + (((int64_t(n) * a.H + y0 + j) * a.W + x0) * a.O + o0) * int64_t(sizeof(T));
+            count = y0 + j < a.H ? min(32, a.W - x0) : 0;
         });
         window = L::kWindow - window;
     }
@@ -731,27 +741,26 @@ hipError_t launchWindow(const ConvMxArgs& args, WindowArgs w, hipStream_t s)
     return hipGetLastError();
 }
 // hipErrorInvalidConfiguration, and no launch, where the filters or the window do not fit.
-template <int FO>
-hipError_t launchWindow(bool half, const ConvMxArgs& a, hipStream_t s)
+template <typename T, int FO>
+hipError_t launchWindow(const ConvMxArgs& a, hipStream_t s)
 {
-    if (a.blocks > 4 || (int64_t(a.taps / a.kw + kWinH) * a.W + a.kw + kWinW) * a.blocks * kMxBytes >= int64_t(kRange)) return hipErrorInvalidConfiguration;
+    if (a.blocks > 2 || (int64_t(a.taps / a.kw + kWinH) * a.W + a.kw + kWinW) * a.blocks * kMxBytes >= int64_t(kRange)) return hipErrorInvalidConfiguration;
     WindowArgs w{};
     const int winH = kWinH + a.taps / a.kw - 1;
     w.winW = kWinW + a.kw - 1;
     w.units = winH * w.winW * a.blocks;
     w.steps = (a.total + 1) / 2;
-    w.swizzleShift = a.blocks == 4 ? 2 : 3;
-    w.swizzleMask = a.blocks == 4 ? 3 : a.blocks == 2 ? 1 : 0;
+    w.swizzle = a.blocks == 2 ? 1 : 0;
     w.tilesX = (a.W + kWinW - 1) / kWinW;
     w.tilesY = (a.H + kWinH - 1) / kWinH;
     w.tiles = a.pixels / (a.H * a.W) * w.tilesX * w.tilesY;
     w.byTilesX = Divider(unsigned(w.tilesX));
     w.byTilesY = Divider(unsigned(w.tilesY));
     w.byWinRow = Divider(unsigned(w.winW * a.blocks));
-    if (w.units <= 2 * kThreads) return half ? launchWindow<f16, FO, 2>(a, w, s) : launchWindow<float, FO, 2>(a, w, s);
-    if (w.units <= 4 * kThreads) return half ? launchWindow<f16, FO, 4>(a, w, s) : launchWindow<float, FO, 4>(a, w, s);
-    if (w.units > 7 * kThreads) return hipErrorInvalidConfiguration;
-    return half ? launchWindow<f16, FO, 7>(a, w, s) : launchWindow<float, FO, 7>(a, w, s);
+    if (w.units <= 2 * kThreads) return launchWindow<T, FO, 2>(a, w, s);
+    if (w.units <= 4 * kThreads) return launchWindow<T, FO, 4>(a, w, s);
+    if (w.units <= 7 * kThreads) return launchWindow<T, FO, 7>(a, w, s);
+    return hipErrorInvalidConfiguration;
 }
 
 template <typename T, int THREADS, int BO, int BP, int FO, int FP>
@@ -818,13 +827,16 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
     const int rows = tiles(16, 64) >= 256 ? 4 : tiles(16, 32) >= 256 ? 2 : 1;
     if (tiles(16, 16 * rows) * (1 + rows) < 1560)
         return rows == 4 ? launchRows<4>(half, a, s) : rows == 2 ? launchRows<2>(half, a, s) : launchRows<1>(half, a, s);
-    // The largest tile that leaves no CU without one: 256x256 reads a quarter of what 64x64 does (512 -> 512 channels, 3x3,
-    // 256x256: 92 instead of 158 us), but 64 such tiles for 2048 -> 2048 channels, 1x1, 2048 pixels take 19 instead of 11.6.
-    if (a.taps > 1 && a.blocks <= 4 && a.W >= 16 && tiles(64, 256) >= 256)
+    // Up to 64 channels on large images: the window kernel.  64 -> 64 channels, 3x3: 92 instead of 139 us for 1920x1080, 17.8
+    // instead of 20 for 640x360 (900 tiles), but 8.4 instead of 7.2 for 320x180 (240); 1x1, 1920x1080: 74 instead of 104.
+    // 96 -> 96, 3x3, 960x540: 83 instead of 78.  fp32 results leave room for 32 channels at a time only (34 instead of 43 us).
+    if (a.blocks <= 2 && a.W >= kWinW && a.H >= kWinH && tiles(64, 256) >= 768)
     {
-        const hipError_t e = a.O <= 32 ? launchWindow<1>(half, a, s) : launchWindow<2>(half, a, s);
+        const hipError_t e = !half ? launchWindow<float, 1>(a, s) : a.O <= 32 ? launchWindow<f16, 1>(a, s) : launchWindow<f16, 2>(a, s);
         if (e != hipErrorInvalidConfiguration) return e;
     }
+    // The largest tile that leaves no CU without one: 256x256 reads a quarter of what 64x64 does (512 -> 512 channels, 3x3,
+    // 256x256: 90 instead of 158 us), but 64 such tiles for 2048 -> 2048 channels, 1x1, 2048 pixels take 19 instead of 11.7.
     if (a.O > 128 && tiles(256, 256) >= 256) return launch<512, 256, 256, 2, 4>(half, a, s);
     if (a.O > 64 && tiles(128, 64) >= 512) return launch<256, 128, 64, 2, 1>(half, a, s);
     if (a.O <= 32 && tiles(32, 128) >= 256) return launch<256, 32, 128, 1, 1>(half, a, s);

@@ -18,7 +18,7 @@ namespace {
 constexpr int kVec = 8;               // channels of one thread
 constexpr int kTileC = kThreads * kVec;
 constexpr int64_t kStreamBytes = int64_t(96) << 20;   // a tensor that would fill the last-level cache (256 MB) passes by it
-constexpr int kJoin = 16;             // parts of an image that every workgroup of NormApplyKernel joins by itself
+constexpr int kJoin = 64;             // parts of an image that every workgroup of NormApplyKernel joins by itself
 
 struct NormArgs
 {
@@ -507,10 +507,10 @@ __global__ __launch_bounds__(kThreads) void NormApplyKernel(const NormArgs a)
     }
     else
     {
-        const int lane = tid & (kJoin - 1);
-        for (int g = tid / kJoin; g < groups; g += kThreads / kJoin)
+        const int lanes = lanesPerGroup(groups, kThreads), lane = tid & (lanes - 1);
+        for (int g = tid / lanes; g < groups; g += kThreads / lanes)
         {
-            const float2 v = joinParts<1>(a, a.partial + (int64_t(n) * a.G + g0 + g) * a.chunks, lane, kJoin);
+            const float2 v = joinParts<8>(a, a.partial + (int64_t(n) * a.G + g0 + g) * a.chunks, lane, lanes);
             if (lane == 0) sStat[g] = v;
         }
     }
@@ -707,11 +707,11 @@ NormPlan planNorm(const ML::Operator& op, bool mx4)
 
     a.tileGroups = a.groupC >= kTileC ? 1 : (kTileC / a.groupC < a.G ? kTileC / a.groupC : a.G);
     a.tiles = (a.G + a.tileGroups - 1) / a.tileGroups;
-    // Statistics: parts of 64 KB at least, about 1024 workgroups at most; up to kJoin parts of an image spare the kernel
-    // that joins them, so no more are made while they stay below 128 KB.
+    // Statistics: parts of 64 KB at least, about 1024 workgroups at most.  Up to kJoin parts of an image spare the kernel
+    // that joins them (4.6 us), which pays while they stay below 192 KB.
     const int64_t imageBytes = a.pixels * a.C * (op.dataType == ML::TensorDataType::FLOAT16 ? 2 : 4);
     int64_t chunks = (imageBytes + (64 << 10) - 1) / (64 << 10);
-    if (chunks > kJoin && imageBytes <= int64_t(kJoin) * (128 << 10)) chunks = kJoin;
+    if (chunks > kJoin && imageBytes <= int64_t(kJoin) * (192 << 10)) chunks = kJoin;
     const int64_t most = (1024 + n * a.tiles - 1) / (n * a.tiles);
     if (chunks > most) chunks = most;
     // (no part is longer than 2^22 pixels: a thread's sums stay short)
