@@ -105,27 +105,28 @@ def nearest(v):
 
 def values64(codes, scales, columns):
     code = torch.stack([codes & 15, codes >> 4], dim=-1).reshape(*scales.shape, 32).long()
-    v = GRID[code & 7] * torch.where(code >= 8, -1.0, 1.0).double()
+    v = GRID.to(codes.device)[code & 7] * torch.where(code >= 8, -1.0, 1.0).double()
     f = torch.exp2(scales.double() - 127)
     f = torch.where(scales == 255, torch.full_like(f, float("nan")), f)
     return (v * f[..., None]).reshape(*scales.shape[:-1], -1)[..., :columns]
 
 
 def conv64(x, w, bias, act):
-    """x [n, h, w, c], w [o, kh, kw, c]; also the sum of the magnitudes of the terms."""
+    """x [n, h, w, c], w [o, kh, kw, c], on either side; also the sum of the magnitudes of the terms."""
     n, H, W, c = x.shape
     o, kh, kw, _ = w.shape
-    p = torch.zeros(n, H + kh - 1, W + kw - 1, c, dtype=torch.float64)
+    p = torch.zeros(n, H + kh - 1, W + kw - 1, c, dtype=torch.float64, device=x.device)
     p[:, kh // 2:kh // 2 + H, kw // 2:kw // 2 + W] = x
-    y = torch.zeros(n, H, W, o, dtype=torch.float64)
+    y = torch.zeros(n, H, W, o, dtype=torch.float64, device=x.device)
     size = torch.zeros_like(y)
     for i in range(kh):
         for j in range(kw):
             part = p[:, i:i + H, j:j + W].reshape(-1, c)
-            y += (part @ w[:, i, j].T).reshape(y.shape)
-            size += (part.abs() @ w[:, i, j].abs().T).reshape(y.shape)
+            f = w[:, i, j].T.contiguous()
+            y += (part @ f).reshape(y.shape)
+            size += (part.abs() @ f.abs()).reshape(y.shape)
     if bias is not None:
-        y, size = y + bias.double(), size + bias.double().abs()
+        y, size = y + bias.double().to(y.device), size + bias.double().abs().to(y.device)
     return act64(y, act), size, y
 
 
@@ -252,10 +253,11 @@ def test_round_trip(dtype, rows, columns):
 
 def test_offsets_past_32_bits():
     """More than 2^32 values: the last rows are the same as alone, and so are rows on both sides of 2^32."""
-    rows, columns = (1 << 26) + 40, 64
+    h, w, columns = 8200, 8192, 64                               # 2^26 and 65536 rows
+    rows = h * w
     x = torch.zeros(rows, columns, dtype=torch.float16, device="cuda")
     tail = rnd((96, columns), 9)
-    for at in (rows - 96, (1 << 25) - 48, (1 << 26) - 300):
+    for at in (rows - 96, (1 << 25) - 48, (1 << 26) - 48):
         x[at:at + 96] = tail.cuda()
     codes = torch.empty(rows, 2, 16, dtype=torch.uint8, device="cuda")
     scales = torch.empty(rows, 2, dtype=torch.uint8, device="cuda")
@@ -267,9 +269,15 @@ def test_offsets_past_32_bits():
     y = torch.empty(rows, 64, dtype=torch.float16, device="cuda")
     S.layer_conv2d_mx4(0, codes.data_ptr(), scales.data_ptr(), (1, 64, 1, rows), wc.ptr(), ws.ptr(), (64, 64, 1, 1), None, 0, y.data_ptr(), stream())
     torch.cuda.synchronize()
+    # as an image: other kernels, the same sums (of one step)
+    z = torch.empty_like(y)
+    S.layer_conv2d_mx4(0, codes.data_ptr(), scales.data_ptr(), (1, 64, h, w), wc.ptr(), ws.ptr(), (64, 64, 1, 1), None, 0, z.data_ptr(), stream())
+    torch.cuda.synchronize()
+    assert torch.equal(z, y)
+    del z
     v = values64(want, want_s, columns)
     ref, size, raw = conv64(v.reshape(1, 1, 96, 64), values64(wc.whole(), ws.whole(), 64).reshape(64, 1, 1, 64), None, 0)
-    for at in (rows - 96, (1 << 25) - 48, (1 << 26) - 300):
+    for at in (rows - 96, (1 << 25) - 48, (1 << 26) - 48):
         assert torch.equal(codes[at:at + 96].cpu(), want) and torch.equal(scales[at:at + 96].cpu(), want_s)
         assert torch.equal(x[at:at + 96].cpu(), v.half())
         assert ((y[at:at + 96].cpu().double() - ref[0, 0]).abs() <= conv_tolerance(size, raw, 2)[0, 0] + step(0, ref)[0, 0]).all()
@@ -405,6 +413,68 @@ def test_conv(dtype, n, c, h, w, o, kh, kw):
         ref, size, y = conv64(x64, w64, bias, act)
         got = convolve(xc, xs, (n, c, h, w), wc, ws, (o, c, kh, kw), bias, act, dtype)
         assert ((got.double() - ref).abs() <= step(dtype, ref) + conv_tolerance(size, y, kh * kw * -(-c // 32))).all()
+
+
+LARGE = [(1, 64, 450, 450, 64, 3, 3), (1, 33, 453, 441, 40, 3, 3), (2, 32, 310, 330, 64, 3, 3), (1, 3, 451, 449, 24, 5, 5), (1, 64, 450, 443, 33, 7, 7),
+         (3, 20, 270, 260, 130, 5, 5), (1, 64, 450, 450, 64, 1, 1), (1, 17, 449, 450, 3, 1, 7), (1, 60, 450, 450, 32, 7, 1), (1, 32, 9, 33000, 64, 2, 2),
+         (1, 50, 6000, 33, 5, 3, 2), (1, 64, 330, 330, 200, 3, 3), (1, 30, 450, 450, 70, 7, 7)]
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("n,c,h,w,o,kh,kw", LARGE)
+def test_conv_of_large_images(dtype, n, c, h, w, o, kh, kw):
+    """At most 64 channels of many pixels (the 64-bit reference runs on the GPU here)."""
+    x, f = rnd((n * h * w, c), c + o), rnd((o * kh * kw, c), c * o + 1) / 8
+    x[(n * h * w) // 2, 1] = float("nan")                        # one pixel in the middle: its neighbours' outputs, and no others
+    xc, xs = quantise(x, 0)
+    wc, ws = quantise(f, 0)
+    x64 = values64(xc.t, xs.t, c).reshape(n, h, w, c)
+    w64 = values64(wc.t, ws.t, c).reshape(o, kh, kw, c)
+    act = c % 3
+    bias = rnd((o,), 7, dtype) if act else None
+    ref, size, y = conv64(x64, w64, bias, act)
+    got = convolve(xc, xs, (n, c, h, w), wc, ws, (o, c, kh, kw), bias, act, dtype).cuda().double()
+    assert int(ref.isnan().sum()) > 0 and torch.equal(got.isnan(), ref.isnan())
+    ok = (got - ref).abs() <= step(dtype, ref) + conv_tolerance(size, y, kh * kw * -(-c // 32))
+    assert (ok | ref.isnan()).all()
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_tensors_anywhere(dtype):
+    """Tensors at multiples of their element, scales at odd addresses: the same results as aligned ones, bit for bit."""
+    n, c, h, w, o, groups = 1, 128, 40, 33, 70, 8
+    t = TYPES[dtype]
+    size = t.itemsize
+
+    def moved(v, by):
+        raw = torch.zeros(v.numel() * v.element_size() + 512, dtype=torch.uint8, device="cuda")
+        part = raw[by:by + v.numel() * v.element_size()]
+        part.copy_(v.contiguous().view(-1).view(torch.uint8))
+        return raw, part, raw.data_ptr() + by
+
+    x, scale, bias, cb = (rnd(s, k, dtype).cuda() for k, s in enumerate([(n, h, w, c), (c,), (c,), (o,)]))
+    wc, ws = quantise((rnd((o * 9, c), 9) / 30).to(t), dtype)
+    need = S.layer_group_norm_workspace(dtype, (n, c, h, w), groups)
+    work = torch.empty(need + 8, dtype=torch.uint8, device="cuda")
+    results = []
+    for by, odd in ((0, 0), (size, 1), (3 * size, 3)):
+        keep = [moved(v, by) for v in (x, scale, bias, cb)]
+        px, ps, pb, pc = (k[2] for k in keep)
+        y, out, back = (torch.zeros(m * size + 512, dtype=torch.uint8, device="cuda") for m in (x.numel(), n * h * w * o, x.numel()))
+        codes, xs = torch.empty(n * h * w * 4, 16, dtype=torch.uint8, device="cuda"), torch.empty(n * h * w * 4 + 8, dtype=torch.uint8, device="cuda")
+        fs = torch.empty(o * 36 + 8, dtype=torch.uint8, device="cuda")
+        fs[odd:odd + o * 36] = ws.t.view(-1)
+        S.layer_group_norm(dtype, px, (n, c, h, w), groups, ps, pb, 1e-5, 2, y.data_ptr() + by, work.data_ptr(), need, stream())
+        S.layer_group_norm_mx4(dtype, px, (n, c, h, w), groups, ps, pb, 1e-5, 2, codes.data_ptr(), xs.data_ptr() + odd, work.data_ptr(), need, stream())
+        S.layer_conv2d_mx4(dtype, codes.data_ptr(), xs.data_ptr() + odd, (n, c, h, w), wc.ptr(), fs.data_ptr() + odd, (o, c, 3, 3), pc, 1, out.data_ptr() + by, stream())
+        S.layer_dequantize_mx4(dtype, codes.data_ptr(), xs.data_ptr() + odd, n * h * w, c, back.data_ptr() + by, stream())
+        torch.cuda.synchronize()
+        results.append([v[by:by + m * size].clone() for v, m in ((y, x.numel()), (out, n * h * w * o), (back, x.numel()))] + [codes, xs[odd:odd + n * h * w * 4].clone()])
+        S.layer_quantize_mx4(dtype, back.data_ptr() + by, n * h * w, c, codes.data_ptr(), xs.data_ptr() + odd, stream())
+        torch.cuda.synchronize()
+        results[-1][-2] = codes.clone()
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))
 
 
 @pytest.mark.parametrize("m,o", [(1, 40), (5, 64), (700, 150)])
