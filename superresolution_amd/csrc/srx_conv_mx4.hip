@@ -837,7 +837,7 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
     }
     // The largest tile that leaves no CU without one: 256x256 reads a quarter of what 64x64 does (512 -> 512 channels, 3x3,
     // 256x256: 90 instead of 158 us), but 64 such tiles for 2048 -> 2048 channels, 1x1, 2048 pixels take 19 instead of 11.7.
-    if (a.O > 128 && tiles(256, 256) >= 256) return launch<512, 256, 256, 2, 4>(half, a, s);
+    if (a.O > 128 && tiles(256, 256) >= 256) return launch<512, 256, 256, 4, 2>(half, a, s);
     if (a.O > 64 && tiles(128, 64) >= 512) return launch<256, 128, 64, 2, 1>(half, a, s);
     if (a.O <= 32 && tiles(32, 128) >= 256) return launch<256, 32, 128, 1, 1>(half, a, s);
     if (a.O <= 64 && tiles(64, 128) >= 1024) return launch<256, 64, 128, 1, 2>(half, a, s);

@@ -149,9 +149,9 @@ struct Finish
             add[i] = a.bias ? bias.get(i) : 0.0f;
         }
     }
-    // m channels exist; `pixel` counts over all images, `column` is the thread's place among the pixel's eighths of blocks
+    // m channels exist
     template <bool MX4, int ACT>
-    __device__ __forceinline__ void store(const NormArgs& a, const Held<T>& x, int m, int c, int64_t pixel) const
+    __device__ __forceinline__ void store(const NormArgs& a, const Held<T>& x, int m, T* out, uint8_t* codes, uint8_t* scaleOf) const
     {
         float v[kVec];
 #pragma unroll
@@ -163,14 +163,35 @@ struct Finish
 #pragma unroll
                 for (int i = 0; i < kVec; ++i) v[i] = i < m ? v[i] : 0.0f;
             }
-            unsigned scale;
-            const unsigned codes = mxQuantise(v, scale);
-            const int64_t block = pixel * mxBlocks(a.C) + (c >> 5);
-            *reinterpret_cast<unsigned*>(a.codes + block * kMxBytes + ((c >> 1) & 12)) = codes;
-            if ((c & 24) == 0) a.scales[block] = uint8_t(scale);
+            unsigned s;
+            *reinterpret_cast<unsigned*>(codes) = mxQuantise(v, s);
+            if ((threadIdx.x & 3) == 0) *scaleOf = uint8_t(s);         // rows of threads are whole blocks
         }
-        else if (a.stream && m == kVec) streamOut8(static_cast<T*>(a.out) + pixel * a.C + c, v);
-        else storeUpTo8(static_cast<T*>(a.out) + pixel * a.C + c, m, v);
+        else if (a.stream && m == kVec) streamOut8(out, v);
+        else storeUpTo8(out, m, v);
+    }
+};
+
+// Where a thread's eight channels from c on of a pixel (counted over all images) go, and of the pixels `rows` further on.
+template <typename T>
+struct Target
+{
+    T* out;
+    uint8_t *codes, *scales;
+    int64_t step, blocks;
+    __device__ __forceinline__ Target(const NormArgs& a, int64_t pixel, int c, int rows)
+        : out(static_cast<T*>(a.out) + pixel * a.C + c), codes(a.codes + (pixel * mxBlocks(a.C) + (c >> 5)) * kMxBytes + ((c >> 1) & 12)),
+          scales(a.scales + pixel * mxBlocks(a.C) + (c >> 5)), step(int64_t(rows) * a.C), blocks(rows * mxBlocks(a.C)) {}
+    template <bool MX4, int ACT>
+    __device__ __forceinline__ void store(const NormArgs& a, const Finish<T>& f, const Held<T>& x, int m, int u) const
+    {
+        f.template store<MX4, ACT>(a, x, m, out + u * step, codes + u * blocks * kMxBytes, scales + u * blocks);
+    }
+    __device__ __forceinline__ void advance(int u)
+    {
+        out += u * step;
+        codes += u * blocks * kMxBytes;
+        scales += u * blocks;
     }
 };
 
@@ -284,10 +305,11 @@ __global__ __launch_bounds__(THREADS) void NormSlabKernel(const NormArgs a)
     __syncthreads();
     if (row >= rows) return;
     f.prepare(a, sStat, g0, m, c);
+    const Target<T> to(a, int64_t(n) * pixels + row, c, rows);
     forActivation(a.activation, [&](auto act) {
 #pragma unroll
         for (int i = 0; i < R; ++i)
-            if (row + i * rows < pixels) f.template store<MX4, act.value>(a, x[i], m, c, int64_t(n) * pixels + row + i * rows);
+            if (row + i * rows < pixels) to.template store<MX4, act.value>(a, f, x[i], m, i);
     });
 }
 
@@ -408,23 +430,25 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
     // Join the rows and channels of each group: row r has `whole` pixels, and one more below `rest`.
     const int stride = vecs * kVec, whole = count / rows, rest = count - whole * rows, used = min(rows, count);
     const int lanes = lanesPerGroup(groups, kThreads), lane = tid & (lanes - 1);
-    const int dr = int(a.byGroupC(unsigned(lanes))), dc = lanes - dr * a.groupC;
-    const int firstR = int(a.byGroupC(unsigned(lane))), firstC = lane - firstR * a.groupC;
+    const int entries = used * a.groupC;
     for (int g = tid / lanes; g < groups; g += kThreads / lanes)
     {
         float mean = 0.0f, m2 = 0.0f;
         const auto each = [&](auto&& f) {
-            for (int r = firstR, c = firstC; r < used;)
+            for (int e0 = lane; e0 < entries; e0 += 4 * lanes)
             {
-                f(float(whole + (r < rest ? 1 : 0)), r * stride + g * a.groupC + c);
-                r += dr;
-                c += dc;
-                if (c >= a.groupC) { c -= a.groupC; ++r; }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                {
+                    const int e = min(e0 + u * lanes, entries - 1), r = int(a.byGroupC(unsigned(e)));
+                    const float n = e0 + u * lanes < entries ? float(whole + (r < rest ? 1 : 0)) : 0.0f;
+                    f(n, r * stride + g * a.groupC + e - r * a.groupC);
+                }
             }
         };
         each([&](float n, int at) { mean = fmaf(n, sMean[at], mean); });
         mean = sumLanes(mean, lanes) / (float(count) * float(a.groupC));
-        each([&](float n, int at) { const float d = sMean[at] - mean; m2 += fmaf(n * d, d, sM2[at]); });
+        each([&](float n, int at) { const float d = sMean[at] - mean; m2 += n > 0.0f ? fmaf(n * d, d, sM2[at]) : 0.0f; });
         m2 = sumLanes(m2, lanes);
         if (lane == 0) out[int64_t(g) * a.chunks] = float2{mean, m2};
     }
@@ -517,7 +541,7 @@ __global__ __launch_bounds__(kThreads) void NormApplyKernel(const NormArgs a)
     __syncthreads();
     if (row >= rows) return;
     f.prepare(a, sStat, g0, m, c);
-    const int64_t pixel0 = n * a.pixels + p0;
+    Target<T> to(a, n * a.pixels + p0 + row, c, rows);
     forActivation(a.activation, [&](auto act) {
         int p = row;
         for (; p + (2 * kFlight - 1) * rows < count; p += kFlight * rows)
@@ -530,7 +554,8 @@ __global__ __launch_bounds__(kThreads) void NormApplyKernel(const NormArgs a)
                 for (int u = 0; u < kFlight; ++u) load(next[u], at + u * step);
             }
 #pragma unroll
-            for (int u = 0; u < kFlight; ++u) f.template store<MX4, act.value>(a, x[u], m, c, pixel0 + p + u * rows);
+            for (int u = 0; u < kFlight; ++u) to.template store<MX4, act.value>(a, f, x[u], m, u);
+            to.advance(kFlight);
 #pragma unroll
             for (int u = 0; u < kFlight; ++u) x[u] = next[u];
         }
@@ -543,7 +568,8 @@ __global__ __launch_bounds__(kThreads) void NormApplyKernel(const NormArgs a)
                 if (m > 0 && p + (kFlight + u) * rows < count) load(next[u], at + u * step);
 #pragma unroll
             for (int u = 0; u < kFlight; ++u)
-                if (p + u * rows < count) f.template store<MX4, act.value>(a, x[u], m, c, pixel0 + p + u * rows);
+                if (p + u * rows < count) to.template store<MX4, act.value>(a, f, x[u], m, u);
+            to.advance(kFlight);
 #pragma unroll
             for (int u = 0; u < kFlight; ++u) x[u] = next[u];
         }
@@ -707,11 +733,11 @@ NormPlan planNorm(const ML::Operator& op, bool mx4)
 
     a.tileGroups = a.groupC >= kTileC ? 1 : (kTileC / a.groupC < a.G ? kTileC / a.groupC : a.G);
     a.tiles = (a.G + a.tileGroups - 1) / a.tileGroups;
-    // Statistics: parts of 64 KB at least, about 1024 workgroups at most.  Up to kJoin parts of an image spare the kernel
-    // that joins them (4.6 us), which pays while they stay below 192 KB.
+    // Statistics: parts of 32 KB for small images, of 64 KB for others, about 1024 workgroups at most.  Up to kJoin parts of
+    // an image spare the kernel that joins them (4.6 us), which pays while they stay below 192 KB.
     const int64_t imageBytes = a.pixels * a.C * (op.dataType == ML::TensorDataType::FLOAT16 ? 2 : 4);
-    int64_t chunks = (imageBytes + (64 << 10) - 1) / (64 << 10);
-    if (chunks > kJoin && imageBytes <= int64_t(kJoin) * (192 << 10)) chunks = kJoin;
+    int64_t chunks = (imageBytes + (32 << 10) - 1) / (32 << 10);
+    if (chunks > kJoin) chunks = imageBytes <= int64_t(kJoin) * (192 << 10) ? kJoin : (imageBytes + (64 << 10) - 1) / (64 << 10);
     const int64_t most = (1024 + n * a.tiles - 1) / (n * a.tiles);
     if (chunks > most) chunks = most;
     // (no part is longer than 2^22 pixels: a thread's sums stay short)
