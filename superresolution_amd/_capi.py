@@ -316,8 +316,11 @@ class FramePipe:
         return out.copy() if copy else out
 
 
+_U32x4 = C.c_uint32 * 4
+
+
 def _sizes(v):
-    return (C.c_uint32 * 4)(*[int(x) for x in v])
+    return _U32x4(*map(int, v))
 
 
 def layer_plan(kind, dtype, in_sizes, param, in_bytes=0, out_bytes=0):

@@ -829,18 +829,28 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
         return rows == 4 ? launchRows<4>(half, a, s) : rows == 2 ? launchRows<2>(half, a, s) : launchRows<1>(half, a, s);
     // Up to 64 channels on large images: the window kernel.  64 -> 64 channels, 3x3: 92 instead of 139 us for 1920x1080, 17.8
     // instead of 20 for 640x360 (900 tiles), but 8.4 instead of 7.2 for 320x180 (240); 1x1, 1920x1080: 74 instead of 104.
-    // 96 -> 96, 3x3, 960x540: 83 instead of 78.  fp32 results leave room for 32 channels at a time only (34 instead of 43 us).
-    if (a.blocks <= 2 && a.W >= kWinW && a.H >= kWinH && tiles(64, 256) >= 768)
+    // 96 -> 96, 3x3, 960x540: 83 instead of 78.  32 -> 128, 3x3, 512x512: 22 instead of 29; 64 -> 256, 3x3, 256x256: 17.2
+    // instead of 15.6.  fp32 results leave room for 32 channels at a time only (34 instead of 43 us).
+    if (a.blocks <= 2 && a.O <= 128 && a.W >= kWinW && a.H >= kWinH && tiles(64, 256) >= 768)
     {
         const hipError_t e = !half ? launchWindow<float, 1>(a, s) : a.O <= 32 ? launchWindow<f16, 1>(a, s) : launchWindow<f16, 2>(a, s);
         if (e != hipErrorInvalidConfiguration) return e;
     }
     // The largest tile that leaves no CU without one: 256x256 reads a quarter of what 64x64 does (512 -> 512 channels, 3x3,
-    // 256x256: 90 instead of 158 us), but 64 such tiles for 2048 -> 2048 channels, 1x1, 2048 pixels take 19 instead of 11.7.
-    if (a.O > 128 && tiles(256, 256) >= 256) return launch<512, 256, 256, 4, 2>(half, a, s);
-    if (a.O > 64 && tiles(128, 64) >= 512) return launch<256, 128, 64, 2, 1>(half, a, s);
+    // 256x256: 90 instead of 158 us), but 64 such tiles for 2048 -> 2048 channels, 1x1, 2048 pixels take 19 instead of 12.
+    // 128x128: 12.7 instead of 14.3 us with 128x64 for 96 -> 96, 3x3, 256x256; 12.4 instead of 12.2 for 256 tiles.
+    // Channels that only fill up a tile count: 160 -> 160, 3x3, 256x256 in 256: 22.4 instead of 24.1 us, but 8 -> 416, 1x7,
+    // 100500 pixels in 512: 39 instead of 29 (nothing but the output takes time there).
+    const auto padded = [&](int64_t o) { return (a.O + o - 1) / o * o; };
+    const bool deep = a.total > 2 * kChunk;
+    if (a.O > 128 && tiles(256, 256) >= 256 && padded(256) * 10 <= padded(64) * (deep ? 14 : 10)) return launch<512, 256, 256, 4, 2>(half, a, s);
+    if (a.O > 64 && padded(128) * 10 <= padded(64) * 14)
+    {
+        if (tiles(128, 128) >= 512) return launch<256, 128, 128, 2, 2>(half, a, s);
+        if (tiles(128, 64) >= 512) return launch<256, 128, 64, 2, 1>(half, a, s);
+    }
     if (a.O <= 32 && tiles(32, 128) >= 256) return launch<256, 32, 128, 1, 1>(half, a, s);
-    if (a.O <= 64 && tiles(64, 128) >= 1024) return launch<256, 64, 128, 1, 2>(half, a, s);
+    if (tiles(64, 128) >= 1024) return launch<256, 64, 128, 1, 2>(half, a, s);
     return launch<256, 64, 64, 1, 1>(half, a, s);
 }
 
