@@ -28,6 +28,7 @@ struct ConvMxArgs
     Divider byW, byH, byBlocks, byKw, byTilesO;
     int tilesO, tilesP;
     int activation;
+    int stream;                       // the output passes by the caches
 };
 
 constexpr int kChunk = 8;             // blocks staged at a time: four instructions' worth
@@ -108,7 +109,9 @@ __device__ __forceinline__ void finishAs(const ConvMxArgs& a, const f32x16 (&acc
             if (channels >= kN)
             {
                 typedef unsigned u32x4_at __attribute__((ext_vector_type(4), aligned(2)));
-                *reinterpret_cast<u32x4_at*>(dst) = u32x4_at{v.x, v.y, v.z, v.w};
+                const u32x4_at w = {v.x, v.y, v.z, v.w};
+                if (a.stream) __builtin_nontemporal_store(w, reinterpret_cast<u32x4_at*>(dst));
+                else *reinterpret_cast<u32x4_at*>(dst) = w;
             }
             else
             {
@@ -817,6 +820,7 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
     a.byBlocks = Divider(unsigned(a.blocks));
     a.byKw = Divider(unsigned(a.kw));
     a.activation = int(op.activation);
+    a.stream = int64_t(a.pixels) * a.O * (op.dataType == ML::TensorDataType::FLOAT16 ? 2 : 4) > kStreamBytes;
     const bool half = op.dataType == ML::TensorDataType::FLOAT16;
     const auto tiles = [&](int64_t o, int64_t p) { return (a.O + o - 1) / o * ((a.pixels + p - 1) / p); };
 

@@ -17,7 +17,6 @@ namespace {
 
 constexpr int kVec = 8;               // channels of one thread
 constexpr int kTileC = kThreads * kVec;
-constexpr int64_t kStreamBytes = int64_t(96) << 20;   // a tensor that would fill the last-level cache (256 MB) passes by it
 constexpr int kJoin = 64;             // parts of an image that every workgroup of NormApplyKernel joins by itself
 
 struct NormArgs
