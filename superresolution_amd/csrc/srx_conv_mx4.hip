@@ -67,12 +67,29 @@ __device__ __forceinline__ unsigned loadByte(i32x4 from, unsigned offset)
     return __builtin_amdgcn_raw_buffer_load_b8(__builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(uint64_t(unsigned(from[0])) | uint64_t(unsigned(from[1])) << 32), 0, from[2], from[3]), offset, 0, 0);
 }
 
-// Bias, activation and stores of a wave's 32 * FO channels of 32 * FP pixels.  A lane holds, for its pixel, output channels
+// Every sum starts with its channel's bias.
+template <int FO, int FP>
+__device__ __forceinline__ void startAt(f32x16 (&acc)[FO][FP], const float* bias, int h)
+{
+#pragma unroll
+    for (int i = 0; i < FO; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+        {
+            const f32x4 b = *reinterpret_cast<const f32x4*>(bias + 32 * i + 8 * g + 4 * h);
+#pragma unroll
+            for (int j = 0; j < FP; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[i][j][4 * g + k] = b[k];
+        }
+}
+
+// Activation and stores of a wave's 32 * FO channels of 32 * FP pixels.  A lane holds, for its pixel, output channels
 // 8 * (r >> 2) + 4 * h + (r & 3) of every 32; the wave turns 32 pixels at a time in its own part of LDS, so that whole
 // rows of channels are stored.  place(j, to, count): where channel o0 of the first of the j-th 32 pixels goes, and how many
 // of them exist (both the same for all lanes).
 template <typename T, int FO, int FP, int ACT, typename Place>
-__device__ __forceinline__ void finishAs(const ConvMxArgs& a, const f32x16 (&acc)[FO][FP], const float* bias, uint8_t* mine, int o0, int lane, Place&& place)
+__device__ __forceinline__ void finishAs(const ConvMxArgs& a, const f32x16 (&acc)[FO][FP], uint8_t* mine, int o0, int lane, Place&& place)
 {
     constexpr int kOutRow = 32 * FO * int(sizeof(T)) + 16;
     constexpr int kN = 16 / int(sizeof(T)), kPerRow = 32 * FO / kN;   // elements of a store, stores of a pixel
@@ -90,10 +107,10 @@ __device__ __forceinline__ void finishAs(const ConvMxArgs& a, const f32x16 (&acc
             for (int g = 0; g < 4; ++g)
             {
                 const int o = 32 * i + 8 * g + 4 * h;
-                const f32x4 b = *reinterpret_cast<const f32x4*>(bias + o);
                 T4 v4;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v4[k] = (T)activate(acc[i][j][4 * g + k] + b[k], ACT);
+                for (int k = 0; k < 4; ++k) v4[k] = (T)(ACT == 1 ? acc[i][j][4 * g + k] : activate(acc[i][j][4 * g + k], ACT));
+                if (ACT == 1) v4 = __builtin_elementwise_maximum(v4, T4{0, 0, 0, 0});     // rounding keeps the sign: two at a time in fp16
                 *reinterpret_cast<T4*>(mine + l * kOutRow + o * int(sizeof(T))) = v4;
             }
         __builtin_amdgcn_wave_barrier();
@@ -126,11 +143,11 @@ __device__ __forceinline__ void finishAs(const ConvMxArgs& a, const f32x16 (&acc
     }
 }
 template <typename T, int FO, int FP, typename Place>
-__device__ __forceinline__ void finish(const ConvMxArgs& a, const f32x16 (&acc)[FO][FP], const float* bias, uint8_t* mine, int o0, int lane, Place&& place)
+__device__ __forceinline__ void finish(const ConvMxArgs& a, const f32x16 (&acc)[FO][FP], uint8_t* mine, int o0, int lane, Place&& place)
 {
-    if (a.activation == 0) finishAs<T, FO, FP, 0>(a, acc, bias, mine, o0, lane, place);
-    else if (a.activation == 1) finishAs<T, FO, FP, 1>(a, acc, bias, mine, o0, lane, place);
-    else finishAs<T, FO, FP, 2>(a, acc, bias, mine, o0, lane, place);
+    if (a.activation == 0) finishAs<T, FO, FP, 0>(a, acc, mine, o0, lane, place);
+    else if (a.activation == 1) finishAs<T, FO, FP, 1>(a, acc, mine, o0, lane, place);
+    else finishAs<T, FO, FP, 2>(a, acc, mine, o0, lane, place);
 }
 
 // A workgroup makes BO output channels of BP pixels; a wave makes 32 * FO channels of 32 * FP pixels.
@@ -140,7 +157,7 @@ __device__ __forceinline__ void finish(const ConvMxArgs& a, const f32x16 (&acc)[
 //           tap is found once for all; otherwise blocks are numbered through and every thread finds its own tap.
 //   WORDS:  the blocks of a pixel come in fours, so that scales are staged in words of four; otherwise byte by byte.
 template <typename T, int THREADS, int BO, int BP, int FO, int FP, bool WITHIN, bool WORDS>
-__global__ __launch_bounds__(THREADS) void ConvMxKernel(const ConvMxArgs a)
+__global__ __launch_bounds__(THREADS, 2) void ConvMxKernel(const ConvMxArgs a)
 {
     static_assert(BO * BP == THREADS / 64 * 32 * FO * 32 * FP, "the waves' tiles make the workgroup's");
     constexpr int kPass = THREADS / 8;                                // rows of codes that a pass of all threads stages
@@ -294,13 +311,6 @@ __global__ __launch_bounds__(THREADS) void ConvMxKernel(const ConvMxArgs a)
         for (int i = 0; i < kXRows; ++i) lds[stage + kXScales + (sr + kPass * i) * kChunk + sb] = xz[i];
     };
 
-    f32x16 acc[FO][FP];
-#pragma unroll
-    for (int i = 0; i < FO; ++i)
-#pragma unroll
-        for (int j = 0; j < FP; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
     // Step s multiplies the blocks s (lanes 0-31) and 4 + s (lanes 32-63) of the chunk: a lane's four scales are one word.
     uint4 wf[2][FO], xf[2][FP];
@@ -329,6 +339,8 @@ __global__ __launch_bounds__(THREADS) void ConvMxKernel(const ConvMxArgs a)
         sBias[o] = a.bias && o0 + o < a.O ? (float)static_cast<const T*>(a.bias)[o0 + o] : 0.0f;
     if (!WORDS) settle(0);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    f32x16 acc[FO][FP];
+    startAt<FO, FP>(acc, sBias + wo, h);
     read(0, 0, 0);
     readScales(0);
     if (chunks > 1)
@@ -409,7 +421,7 @@ __global__ __launch_bounds__(THREADS) void ConvMxKernel(const ConvMxArgs a)
     // (also the loads of the chunk after the last, which write zeros)
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     uint8_t* mine = lds + wave * 32 * kOutRow;
-    finish<T, FO, FP>(a, acc, sBias + wo, mine, o0 + wo, lane, [&](int j, uint8_t*& to, int& count) {
+    finish<T, FO, FP>(a, acc, mine, o0 + wo, lane, [&](int j, uint8_t*& to, int& count) {
         const int64_t m = m0 + wp + 32 * j;
         to = static_cast<uint8_t*>(a.out) + (m * a.O + o0 + wo) * int64_t(sizeof(T));
         count = int(min(int64_t(32), a.pixels - m));
@@ -579,7 +591,7 @@ struct WindowLds
 };
 
 template <typename T, int FO, int NL>
-__global__ __launch_bounds__(kThreads) void ConvMxWindowKernel(const ConvMxArgs a, const WindowArgs w)
+__global__ __launch_bounds__(kThreads, 2) void ConvMxWindowKernel(const ConvMxArgs a, const WindowArgs w)
 {
     using L = WindowLds<T, FO, NL>;
     constexpr int kBO = L::kBO, FP = 2;
@@ -653,12 +665,7 @@ __global__ __launch_bounds__(kThreads) void ConvMxWindowKernel(const ConvMxArgs 
         if (tile + w.slots < w.tiles) fetch(tile + w.slots, L::kWindow - window);
 
         f32x16 acc[FO][FP];
-#pragma unroll
-        for (int i = 0; i < FO; ++i)
-#pragma unroll
-            for (int j = 0; j < FP; ++j)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+        startAt<FO, FP>(acc, reinterpret_cast<const float*>(dyn + L::kBias), h);
 
         // the next step's operands are read while one is multiplied
         uint4 wf[2][FO], xf[2][FP];
@@ -713,7 +720,7 @@ __global__ __launch_bounds__(kThreads) void ConvMxWindowKernel(const ConvMxArgs 
 
         const unsigned q = w.byTilesX(unsigned(tile)), n = w.byTilesY(q);
         const int x0 = int(unsigned(tile) - q * unsigned(w.tilesX)) * kWinW, y0 = int(q - n * unsigned(w.tilesY)) * kWinH + 2 * wave;
-        finish<T, FO, FP>(a, acc, reinterpret_cast<const float*>(dyn + L::kBias), dyn + L::kTurn + wave * 32 * L::kOutRow, o0, lane, [&](int j, uint8_t*& to, int& count) {
+        finish<T, FO, FP>(a, acc, dyn + L::kTurn + wave * 32 * L::kOutRow, o0, lane, [&](int j, uint8_t*& to, int& count) {
             to = static_cast<uint8_t*>(a.out) + (((int64_t(n) * a.H + y0 + j) * a.W + x0) * a.O + o0) * int64_t(sizeof(T));
             count = y0 + j < a.H ? min(32, a.W - x0) : 0;
         });

@@ -183,11 +183,10 @@ __device__ __forceinline__ void storeUpTo8(T* p, int count, const float (&v)[8])
 }
 
 // 0 none, 1 ReLU, 2 SiLU: y / (1 + exp(-y)), with the exponential and the reciprocal of the special function unit
-// (an error of one part in 2^22 at most for the |y| where the result is not zero).  ReLU passes a NaN on, as the
-// comparison y < 0 is false for it.
+// (an error of one part in 2^22 at most for the |y| where the result is not zero).  ReLU is the maximum that passes a NaN on.
 __device__ __forceinline__ float activate(float y, int activation)
 {
-    if (activation == 1) return y < 0.0f ? 0.0f : y;
+    if (activation == 1) return __builtin_elementwise_maximum(y, 0.0f);
     if (activation == 2) return y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y * -1.44269504088896340736f));
     return y;
 }
