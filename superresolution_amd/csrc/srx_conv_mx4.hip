@@ -543,6 +543,16 @@ __global__ __launch_bounds__(64 * kRowWaves) void ConvMxRowsKernel(const ConvMxA
     }
 }
 
+// Whether all taps of all pixels of a tile (of 256 pixels at most) lie within the range of one descriptor.
+bool tapsInRange(const ConvMxArgs& a)
+{
+    return ((int64_t(a.taps / a.kw) * a.W + a.kw + 256) * a.blocks + a.total) * kMxBytes < int64_t(kRange);
+}
+bool scalesInWords(const ConvMxArgs& a)
+{
+    return a.blocks % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.scales) | reinterpret_cast<uintptr_t>(a.wScales)) & 3) == 0;
+}
+
 template <typename T, int FP>
 hipError_t launchRows(const ConvMxArgs& args, bool words, hipStream_t s)
 {
@@ -559,8 +569,7 @@ hipError_t launchRows(const ConvMxArgs& args, bool words, hipStream_t s)
 template <int FP>
 hipError_t launchRows(bool half, const ConvMxArgs& a, hipStream_t s)
 {
-    const bool words = a.blocks % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.scales) | reinterpret_cast<uintptr_t>(a.wScales)) & 3) == 0;
-    return half ? launchRows<f16, FP>(a, words, s) : launchRows<float, FP>(a, words, s);
+    return half ? launchRows<f16, FP>(a, scalesInWords(a), s) : launchRows<float, FP>(a, scalesInWords(a), s);
 }
 
 // Up to two blocks a pixel: the tiles above would read every pixel once for each tap.  Here a workgroup
@@ -754,6 +763,7 @@ hipError_t launchWindow(const ConvMxArgs& args, WindowArgs w, hipStream_t s)
 template <typename T, int FO>
 hipError_t launchWindow(const ConvMxArgs& a, hipStream_t s)
 {
+    // (the rows of a window are eight more than the taps')
     if (a.blocks > 2 || (int64_t(a.taps / a.kw + kWinH) * a.W + a.kw + kWinW) * a.blocks * kMxBytes >= int64_t(kRange)) return hipErrorInvalidConfiguration;
     WindowArgs w{};
     const int winH = kWinH + a.taps / a.kw - 1;
@@ -783,10 +793,7 @@ hipError_t launch(const ConvMxArgs& args, hipStream_t s)
     const int64_t grid = int64_t(a.tilesO) * (a.tilesP >= 64 ? (a.tilesP + 7) / 8 * 8 : a.tilesP);
     if (grid > INT32_MAX) return hipErrorInvalidValue;
     const dim3 g(static_cast<unsigned>(grid)), block(THREADS);
-    // Numbered-through blocks need all taps of a tile within the range of one descriptor.
-    const int64_t span = ((int64_t(a.taps / a.kw) * a.W + a.kw + BP) * a.blocks + a.total) * kMxBytes;
-    const bool within = a.taps == 1 || a.blocks % kChunk == 0 || span >= int64_t(kRange);
-    const bool words = a.blocks % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.scales) | reinterpret_cast<uintptr_t>(a.wScales)) & 3) == 0;
+    const bool within = a.taps == 1 || a.blocks % kChunk == 0 || !tapsInRange(a), words = scalesInWords(a);
     if (within && words) hipLaunchKernelGGL((ConvMxKernel<T, THREADS, BO, BP, FO, FP, true, true>), g, block, 0, s, a);
     else if (within) hipLaunchKernelGGL((ConvMxKernel<T, THREADS, BO, BP, FO, FP, true, false>), g, block, 0, s, a);
     else if (words) hipLaunchKernelGGL((ConvMxKernel<T, THREADS, BO, BP, FO, FP, false, true>), g, block, 0, s, a);
@@ -836,7 +843,7 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
     // 4096 -> 4096 channels, 1x1: 4.1 (1 pixel), 9.2 (64) us instead of 9.9, 10.2 with tiles of 64x64; 26.8 instead of 13.5
     // for 256 pixels.  256 -> 256 channels, 3x3, 16x16: 3.8 instead of 6.9.
     const int rows = tiles(16, 64) >= 256 ? 4 : tiles(16, 32) >= 256 ? 2 : 1;
-    if (tiles(16, 16 * rows) * (1 + rows) < 1560)
+    if (tiles(16, 16 * rows) * (1 + rows) < 1560 && tapsInRange(a))
         return rows == 4 ? launchRows<4>(half, a, s) : rows == 2 ? launchRows<2>(half, a, s) : launchRows<1>(half, a, s);
     // Up to 64 channels on large images: the window kernel.  64 -> 64 channels, 3x3: 92 instead of 139 us for 1920x1080, 17.8
     // instead of 20 for 640x360 (900 tiles), but 8.4 instead of 7.2 for 320x180 (240); 1x1, 1920x1080: 74 instead of 104.

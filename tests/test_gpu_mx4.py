@@ -439,6 +439,32 @@ def test_conv_of_large_images(dtype, n, c, h, w, o, kh, kw):
     assert (ok | ref.isnan()).all()
 
 
+@pytest.mark.parametrize("c,h,w,o,kh,kw", [(1 << 20, 2, 1400, 2, 3, 1), (4000, 2, 360000, 8, 3, 1), (64, 2, 15000000, 3, 2, 2)])
+def test_conv_taps_far_apart(c, h, w, o, kh, kw):
+    """Rows of pixels so long that a window's taps are more than 2^31 bytes of codes apart."""
+    b = -(-c // 32)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(c)
+    codes = torch.randint(0, 256, (h, w, b, 16), generator=g, device="cuda", dtype=torch.uint8)
+    if c % 32:
+        codes[:, :, -1, (c % 32) // 2:] = 0                       # what a block is filled up with
+    scales = torch.randint(120, 130, (h, w, b), generator=g, device="cuda", dtype=torch.uint8)
+    fc = torch.randint(0, 256, (o, kh, kw, b, 16), generator=g, device="cuda", dtype=torch.uint8)
+    fs = torch.randint(115, 120, (o, kh, kw, b), generator=g, device="cuda", dtype=torch.uint8)
+    out = torch.empty(h, w, o, device="cuda")
+    S.layer_conv2d_mx4(1, codes.data_ptr(), scales.data_ptr(), (1, c, h, w), fc.data_ptr(), fs.data_ptr(), (o, c, kh, kw), None, 0, out.data_ptr(), stream())
+    torch.cuda.synchronize()
+    f64 = values64(fc, fs, c)
+    for x0 in (0, w // 2 - 3, w - 7):                             # seven columns and a border of one on either side
+        x1, left = x0 + 7, 1 if x0 else 0
+        right = 1 if x1 < w else 0
+        part = values64(codes[:, x0 - left:x1 + right].contiguous(), scales[:, x0 - left:x1 + right].contiguous(), c)
+        ref, size, y = conv64(part[None], f64, None, 0)
+        ref, size, y = (v[0, :, left:left + 7] for v in (ref, size, y))
+        got = out[:, x0:x1].double()
+        assert ((got - ref).abs() <= step(1, ref) + conv_tolerance(size, y, kh * kw * b)).all()
+
+
 @pytest.mark.parametrize("dtype", [0, 1])
 def test_tensors_anywhere(dtype):
     """Tensors at multiples of their element, scales at odd addresses: the same results as aligned ones, bit for bit."""
