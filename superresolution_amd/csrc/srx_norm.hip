@@ -208,7 +208,8 @@ __host__ __device__ __forceinline__ int vecsFor(int channels)
 template <typename T, bool MX4, int THREADS, int R>
 __global__ __launch_bounds__(THREADS) void NormSlabKernel(const NormArgs a)
 {
-    __shared__ float sPart[THREADS * kVec];
+    __shared__ __attribute__((aligned(16))) float sPart[THREADS * kVec];
+    __shared__ float sTeam[THREADS];
     __shared__ float2 sStat[THREADS * kVec];
     const int tid = threadIdx.x, n = int(a.byTiles(blockIdx.x)), tile = int(blockIdx.x) - n * a.tiles;
     const int g0 = tile * a.tileGroups, groups = min(a.tileGroups, a.G - g0);
@@ -226,36 +227,69 @@ __global__ __launch_bounds__(THREADS) void NormSlabKernel(const NormArgs a)
     Finish<T> f;
     f.load(a, m, c);
 
-    const int lanes = lanesPerGroup(a.tileGroups, THREADS), lane = tid & (lanes - 1);
     const float inv = 1.0f / (float(pixels) * float(a.groupC));
+    // put(g, sum of v over group g): by one thread for each group, seen by all afterwards.  One group: sums of waves.
+    // Several: lanes x slices threads add up each group's values, then the slices are added up.
+    const int lanes = lanesPerGroup(a.tileGroups, THREADS), lane = tid & (lanes - 1), team = tid / lanes;
+    const int slices = max(1, THREADS / lanes / a.tileGroups), slice = slices > 1 ? team / a.tileGroups : 0;
     // Where a group is whole eighths, a thread adds up its eight channels first.
     const int per = a.groupC % kVec == 0 ? 1 : kVec;
     const int rowValues = vecs * per, groupValues = per == 1 ? a.groupC / kVec : a.groupC;
-    const auto reduce = [&](int g) -> float {
-        // every thread's values are in sPart; this thread's lane group adds up those of group g
-        float sum = 0.0f;
-        int r = lane / groupValues, k = lane - r * groupValues;
-        const int dr = lanes / groupValues, dk = lanes - dr * groupValues;
-        while (r < rows)
+    const int first = slice * lanes + lane, step = slices * lanes;
+    const int r0 = first / groupValues, k0 = first - r0 * groupValues, dr = step / groupValues, dk = step - dr * groupValues;
+    const auto total = [&](const float (&v)[kVec], auto&& put) {
+        const float own = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        if (a.tileGroups == 1)
         {
-            sum += sPart[r * rowValues + g * groupValues + k];
-            k += dk;
-            r += dr;
-            if (k >= groupValues) { k -= groupValues; ++r; }
-        }
-        return sumLanes(sum, lanes);
-    };
-    const auto publish = [&](const float (&v)[kVec]) {
-        if (row >= rows) return;
-        if (per == 1)
-            sPart[tid] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-        else
-        {
+            const float w = sumLanes(own, 64);
+            __syncthreads();                                            // (sTeam of the call before has been read)
+            if ((tid & 63) == 0) sTeam[tid >> 6] = w;
+            __syncthreads();
+            float all = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) sPart[tid * kVec + i] = v[i];
+            for (int i = 0; i < THREADS / 64; ++i) all += sTeam[i];
+            if (tid == 0) put(0, all);
+            __syncthreads();
+            return;
+        }
+        if (row < rows)
+        {
+            if (per == 1) sPart[tid] = own;
+            else
+            {
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) sPart[tid * kVec + i] = v[i];
+            }
+        }
+        __syncthreads();
+        if (slice < slices)
+            for (int g = team - slice * a.tileGroups; g < groups; g += THREADS / lanes)
+            {
+                float sum = 0.0f;
+                for (int r = r0, k = k0; r < rows;)
+                {
+                    sum += sPart[r * rowValues + g * groupValues + k];
+                    k += dk;
+                    r += dr;
+                    if (k >= groupValues) { k -= groupValues; ++r; }
+                }
+                sum = sumLanes(sum, lanes);
+                if (lane == 0 && slices == 1) put(g, sum);
+                if (lane == 0 && slices > 1) sTeam[slice * a.tileGroups + g] = sum;
+            }
+        __syncthreads();
+        if (slices > 1)
+        {
+            if (tid < groups)
+            {
+                float all = 0.0f;
+                for (int i = 0; i < slices; ++i) all += sTeam[i * a.tileGroups + tid];
+                put(tid, all);
+            }
+            __syncthreads();
         }
     };
-    float s[kVec];
+    float s[kVec], mean[kVec];
 #pragma unroll
     for (int k = 0; k < kVec; ++k) s[k] = 0.0f;
 #pragma unroll
@@ -265,15 +299,7 @@ __global__ __launch_bounds__(THREADS) void NormSlabKernel(const NormArgs a)
 #pragma unroll
             for (int k = 0; k < kVec; ++k) s[k] += k < m ? x[i].get(k) : 0.0f;
         }
-    publish(s);
-    __syncthreads();
-    for (int g = tid / lanes; g < groups; g += THREADS / lanes)
-    {
-        const float sum = reduce(g);
-        if (lane == 0) sStat[g].x = sum * inv;
-    }
-    __syncthreads();
-    float mean[kVec];
+    total(s, [&](int g, float sum) { sStat[g].x = sum * inv; });
     if (m > 0)
     {
         int g = int(a.byGroupC(unsigned(col * kVec))), left = (g + 1) * a.groupC - col * kVec;
@@ -297,14 +323,7 @@ __global__ __launch_bounds__(THREADS) void NormSlabKernel(const NormArgs a)
                 s[k] = fmaf(d, d, s[k]);
             }
         }
-    publish(s);
-    __syncthreads();
-    for (int g = tid / lanes; g < groups; g += THREADS / lanes)
-    {
-        const float sum = reduce(g);
-        if (lane == 0) sStat[g].y = inverseRoot(fmaf(sum, inv, a.epsilon));
-    }
-    __syncthreads();
+    total(s, [&](int g, float sum) { sStat[g].y = inverseRoot(fmaf(sum, inv, a.epsilon)); });
     if (row >= rows) return;
     f.prepare(a, sStat, g0, m, c);
     const Target<T> to(a, int64_t(n) * pixels + row, c, rows);
@@ -708,17 +727,16 @@ NormPlan planNorm(const ML::Operator& op, bool mx4)
     a.byGroupC = Divider(unsigned(a.groupC));
     a.groupsInAll = int(n * a.G < INT32_MAX ? n * a.G : INT32_MAX);
 
-    // slabs: the fewest groups that are a whole number of 64-byte lines (of blocks of 32 channels)
-    const int unit = mx4 || op.dataType == ML::TensorDataType::FLOAT16 ? 32 : 16;
-    int groups = 1;
-    while (groups < a.G && (groups * a.groupC) % unit != 0) ++groups;
-    if (a.pixels <= 1 << 20 && (!mx4 || groups == a.G || (groups * a.groupC) % 32 == 0))
-    {
+    // Slabs of the fewest groups that are a whole number of 64-byte lines (of blocks of 32 channels), or of single groups.  A
+    // slab has one CU's arithmetic: with SiLU 8192 values take 4.2 us, 32768 take 8.5, 131072 take 25, against 10 us for
+    // the two kernels below on images up to 1 MB.  Single groups, whose pixels are pieces of lines: 32768 values take 15.6 us.
+    const bool half = op.dataType == ML::TensorDataType::FLOAT16;
+    const int64_t imageBytes = a.pixels * a.C * (half ? 2 : 4);
+    const auto slab = [&](int groups, int most) {
         const int64_t vecs = mx4 ? vecsFor<true>(groups * a.groupC) : vecsFor<false>(groups * a.groupC);
-        const int most = op.dataType == ML::TensorDataType::FLOAT16 ? 16 : 8;
         for (const int threads : {256, 1024})
         {
-            if (vecs > threads) continue;
+            if (vecs > threads || a.pixels > 1 << 20) continue;
             const int64_t rows = threads / vecs, held = (a.pixels + rows - 1) / rows;
             if (held > (threads == 256 ? 4 : most)) continue;
             p.slabThreads = threads;
@@ -728,16 +746,22 @@ NormPlan planNorm(const ML::Operator& op, bool mx4)
             a.slabRows = int(rows);
             a.byTiles = Divider(unsigned(a.tiles));
             a.byVecs = Divider(unsigned(vecs));
-            if (n * a.tiles <= INT32_MAX) return p;
+            return n * a.tiles <= INT32_MAX;
         }
-    }
+        return false;
+    };
+    const int unit = mx4 || half ? 32 : 16;
+    int lines = 1;
+    while (lines < a.G && (lines * a.groupC) % unit != 0) ++lines;
+    // few slabs of whole lines: single groups make more of them (4 x 32x32 pixels of 128 channels: 7.8 instead of 10.9 us)
+    if (!mx4 && n * ((a.G + lines - 1) / lines) < 32 && slab(1, 2)) return p;
+    if (slab(lines, 4)) return p;
     p.slabThreads = 0;
 
     a.tileGroups = a.groupC >= kTileC ? 1 : (kTileC / a.groupC < a.G ? kTileC / a.groupC : a.G);
     a.tiles = (a.G + a.tileGroups - 1) / a.tileGroups;
     // Statistics: parts of 32 KB for small images, of 64 KB for others, about 1024 workgroups at most.  Up to kJoin parts of
     // an image spare the kernel that joins them (4.6 us), which pays while they stay below 192 KB.
-    const int64_t imageBytes = a.pixels * a.C * (op.dataType == ML::TensorDataType::FLOAT16 ? 2 : 4);
     int64_t chunks = (imageBytes + (32 << 10) - 1) / (32 << 10);
     if (chunks > kJoin) chunks = imageBytes <= int64_t(kJoin) * (192 << 10) ? kJoin : (imageBytes + (64 << 10) - 1) / (64 << 10);
     const int64_t most = (1024 + n * a.tiles - 1) / (n * a.tiles);
@@ -773,12 +797,10 @@ hipError_t launchNorm(const NormPlan& p, hipStream_t s)
     if (p.slabThreads)
     {
         const dim3 grid(static_cast<unsigned>(p.images * a.tiles));
-        constexpr bool kHalf = sizeof(T) == 2;
         if (p.slabThreads == 256 && p.slabHeld == 1) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 256, 1>), grid, dim3(256), 0, s, a);
         else if (p.slabThreads == 256) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 256, 4>), grid, dim3(256), 0, s, a);
-        else if (p.slabHeld <= 4) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 1024, 4>), grid, dim3(1024), 0, s, a);
-        else if (p.slabHeld <= 8) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 1024, 8>), grid, dim3(1024), 0, s, a);
-        else if constexpr (kHalf) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 1024, 16>), grid, dim3(1024), 0, s, a);
+        else if (p.slabHeld <= 2) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 1024, 2>), grid, dim3(1024), 0, s, a);
+        else hipLaunchKernelGGL((NormSlabKernel<T, MX4, 1024, 4>), grid, dim3(1024), 0, s, a);
         return hipGetLastError();
     }
     const int64_t statsGrid = p.images * a.chunks * a.tiles, applyGrid = p.images * a.applyChunks * a.applyTiles;
