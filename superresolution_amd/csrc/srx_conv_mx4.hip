@@ -441,14 +441,13 @@ __device__ __forceinline__ unsigned loadWord(i32x4 from, unsigned offset)
 }
 
 // Few pixels: a workgroup makes 16 output channels of 16 * FP pixels on v_mfma_scale_f32_16x16x128_f8f6f4, and its waves
-// share the reduction: wave w takes the chunks w, w + 8, .. of sixteen blocks, straight from memory into registers, and the
+// share the reduction: wave w takes the chunks w, w + WAVES, .. of sixteen blocks, straight from memory into registers, and the
 // partial sums are added up in LDS in the waves' order.  Lane l holds row (or column) l & 15; step s multiplies the
 // blocks 4 * (l >> 4) + s, so that a lane's four scales are one word and its codes 64 bytes in a row.
-constexpr int kRowWaves = 8;
-template <typename T, int FP, bool WORDS>
-__global__ __launch_bounds__(64 * kRowWaves) void ConvMxRowsKernel(const ConvMxArgs a)
+template <typename T, int FP, bool WORDS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void ConvMxRowsKernel(const ConvMxArgs a)
 {
-    __shared__ __attribute__((aligned(16))) f32x4 part[kRowWaves][FP][64];
+    __shared__ __attribute__((aligned(16))) f32x4 part[WAVES][FP][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), q = lane >> 4, l = lane & 15;
     const unsigned tileP = a.byTilesO(blockIdx.x);
     const int o0 = int(blockIdx.x - tileP * a.tilesO) * 16;
@@ -470,24 +469,24 @@ __global__ __launch_bounds__(64 * kRowWaves) void ConvMxRowsKernel(const ConvMxA
     const i32x4 wd = descriptor(a.wCodes + int64_t(o0) * a.total * kMxBytes, kRange), vd = descriptor(a.wScales + int64_t(o0) * a.total, kRange >> 4);
     const unsigned wRow = o0 + l < a.O ? unsigned(l * a.total) * kMxBytes : kRange;
 
-    f32x4 acc[FP];
-#pragma unroll
-    for (int j = 0; j < FP; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k0 = wave * 16; k0 < a.total; k0 += kRowWaves * 16)
+    struct Operands
     {
-        uint4 wf[4], xf[FP][4];
-        unsigned ws = 0, xs[FP];
-#pragma unroll
-        for (int j = 0; j < FP; ++j) xs[j] = 0;
+        uint4 w[4], x[FP][4];
+        unsigned ws, xs[FP];
+    };
+    const auto load = [&](Operands& to, int k0) {
         const int kb = k0 + 4 * q;
         unsigned off[FP];
+        to.ws = 0;
+#pragma unroll
+        for (int j = 0; j < FP; ++j) to.xs[j] = 0;
 #pragma unroll
         for (int s = 0; s < 4; ++s)
         {
             const unsigned out = kb + s < a.total ? 0u : kRange;
             const unsigned at = (wRow + unsigned(kb + s) * kMxBytes) | out;
-            wf[s] = loadCodes(wd, at);
-            if (!WORDS) ws |= unsigned(loadByte(vd, at / kMxBytes)) << (8 * s);
+            to.w[s] = loadCodes(wd, at);
+            if (!WORDS) to.ws |= unsigned(loadByte(vd, at / kMxBytes)) << (8 * s);
             if (!WORDS || s == 0)
             {
                 const int t = int(a.byBlocks(unsigned(kb + s))), ky = int(a.byKw(unsigned(t))), kx = t - ky * a.kw;
@@ -498,24 +497,43 @@ __global__ __launch_bounds__(64 * kRowWaves) void ConvMxRowsKernel(const ConvMxA
 #pragma unroll
             for (int j = 0; j < FP; ++j)
             {
-                xf[j][s] = loadCodes(xd, WORDS ? off[j] + s * kMxBytes : off[j]);
-                if (!WORDS) xs[j] |= unsigned(loadByte(zd, off[j] / kMxBytes)) << (8 * s);
+                to.x[j][s] = loadCodes(xd, WORDS ? off[j] + s * kMxBytes : off[j]);
+                if (!WORDS) to.xs[j] |= unsigned(loadByte(zd, off[j] / kMxBytes)) << (8 * s);
             }
         }
         if (WORDS)
         {
-            ws = loadWord(vd, ((wRow + unsigned(kb) * kMxBytes) | (kb < a.total ? 0u : kRange)) / kMxBytes);
+            to.ws = loadWord(vd, ((wRow + unsigned(kb) * kMxBytes) | (kb < a.total ? 0u : kRange)) / kMxBytes);
 #pragma unroll
-            for (int j = 0; j < FP; ++j) xs[j] = loadWord(zd, off[j] / kMxBytes);
+            for (int j = 0; j < FP; ++j) to.xs[j] = loadWord(zd, off[j] / kMxBytes);
         }
+    };
+    f32x4 acc[FP];
+#pragma unroll
+    for (int j = 0; j < FP; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const auto multiply = [&](const Operands& o) {
 #define SRX_STEP(S)                                                                                                    \
         _Pragma("unroll") for (int j = 0; j < FP; ++j)                                                                 \
-            acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(wf[S]), widen(xf[j][S]), acc[j], 4, 4, S, ws, S, xs[j]);
+            acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(o.w[S]), widen(o.x[j][S]), acc[j], 4, 4, S, o.ws, S, o.xs[j]);
         SRX_STEP(0)
         SRX_STEP(1)
         SRX_STEP(2)
         SRX_STEP(3)
 #undef SRX_STEP
+    };
+    // the next chunk's operands are asked for before the current one is multiplied
+    int k0 = wave * 16;
+    if (k0 < a.total)
+    {
+        Operands now, next;
+        load(now, k0);
+        for (k0 += WAVES * 16; k0 < a.total; k0 += WAVES * 16)
+        {
+            load(next, k0);
+            multiply(now);
+            now = next;
+        }
+        multiply(now);
     }
 #pragma unroll
     for (int j = 0; j < FP; ++j) part[wave][j][lane] = acc[j];
@@ -523,7 +541,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void ConvMxRowsKernel(const ConvMxA
     if (wave >= FP) return;
     // a lane holds, for its pixel, output channels 4 * (lane >> 4) ..
     f32x4 sum = part[0][wave][lane];
-    const int waves = min(kRowWaves, (a.total + 15) / 16);
+    const int waves = min(WAVES, (a.total + 15) / 16);
     for (int w = 1; w < waves; ++w) sum += part[w][wave][lane];
     const int64_t m = m0 + 16 * wave + l;
     if (m >= a.pixels) return;
@@ -561,9 +579,18 @@ hipError_t launchRows(const ConvMxArgs& args, bool words, hipStream_t s)
     a.byTilesO = Divider(unsigned(a.tilesO));
     const int64_t grid = int64_t(a.tilesO) * ((int64_t(a.pixels) + 16 * FP - 1) / (16 * FP));
     if (grid > INT32_MAX) return hipErrorInvalidValue;
-    const dim3 g(static_cast<unsigned>(grid)), block(64 * kRowWaves);
-    if (words) hipLaunchKernelGGL((ConvMxRowsKernel<T, FP, true>), g, block, 0, s, a);
-    else hipLaunchKernelGGL((ConvMxRowsKernel<T, FP, false>), g, block, 0, s, a);
+    const dim3 g(static_cast<unsigned>(grid));
+    // Sixteen waves where eight would take several chunks each (1024 -> 1024 channels, 3x3, 8x8: 7.8 us), but for 64 pixels,
+    // whose operands do not fit a sixteenth of the registers twice.
+    if constexpr (FP < 4)
+        if (a.total > 8 * 16)
+        {
+            if (words) hipLaunchKernelGGL((ConvMxRowsKernel<T, FP, true, 16>), g, dim3(1024), 0, s, a);
+            else hipLaunchKernelGGL((ConvMxRowsKernel<T, FP, false, 16>), g, dim3(1024), 0, s, a);
+            return hipGetLastError();
+        }
+    if (words) hipLaunchKernelGGL((ConvMxRowsKernel<T, FP, true, 8>), g, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((ConvMxRowsKernel<T, FP, false, 8>), g, dim3(512), 0, s, a);
     return hipGetLastError();
 }
 template <int FP>
@@ -862,7 +889,7 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
     const auto padded = [&](int64_t o) { return (a.O + o - 1) / o * o; };
     const bool deep = a.total > 2 * kChunk;
     if (a.O > 128 && tiles(256, 256) >= 256 && padded(256) * 10 <= padded(64) * (deep ? 14 : 10)) return launch<512, 256, 256, 4, 2>(half, a, s);
-    if (a.O > 64 && padded(128) * 10 <= padded(64) * 14)
+    if (a.O > 64 && padded(128) * 10 <= padded(64) * (deep ? 14 : 10))
     {
         if (tiles(128, 128) >= 512) return launch<256, 128, 128, 2, 2>(half, a, s);
         if (tiles(128, 64) >= 512) return launch<256, 128, 64, 2, 1>(half, a, s);
