@@ -150,6 +150,17 @@ __device__ __forceinline__ void finish(const ConvMxArgs& a, const f32x16 (&acc)[
     else finishAs<T, FO, FP, 2>(a, acc, mine, o0, lane, place);
 }
 
+// LDS of a tile: the bias, and one or two chunks (rows of codes, words of scales), later the turn of the results.
+template <typename T, int THREADS, int BO, int BP, int FO>
+struct TileLds
+{
+    static constexpr int kXWords = (BP * 2 + THREADS - 1) / THREADS, kWWords = (BO * 2 + THREADS - 1) / THREADS;
+    static constexpr int kCodes = (BO + BP) * kRow, kXScales = kCodes + kWWords * THREADS * 4, kStage = kXScales + kXWords * THREADS * 4;
+    static constexpr int kOutRow = 32 * FO * int(sizeof(T)) + 16;     // bytes of a pixel in the epilogue, padded
+    static constexpr int kOut = THREADS / 64 * 32 * kOutRow, kBias = (BO * 4 + 1023) / 1024 * 1024;
+    static constexpr int bytes(int chunks) { return kBias + (chunks * kStage > kOut ? chunks * kStage : kOut); }
+};
+
 // A workgroup makes BO output channels of BP pixels; a wave makes 32 * FO channels of 32 * FP pixels.
 // The reduction goes in chunks of eight blocks through two buffers in LDS: while one is multiplied, the next is on its
 // way from memory to the other (one barrier a chunk).
@@ -163,11 +174,11 @@ __global__ __launch_bounds__(THREADS, 2) void ConvMxKernel(const ConvMxArgs a)
     constexpr int kPass = THREADS / 8;                                // rows of codes that a pass of all threads stages
     constexpr int kXRows = BP / kPass, kWRows = BO / kPass;
     constexpr int kXWords = (BP * 2 + THREADS - 1) / THREADS, kWWords = (BO * 2 + THREADS - 1) / THREADS;
-    constexpr int kCodes = (BO + BP) * kRow, kStage = kCodes + (kXWords + kWWords) * THREADS * 4, kXScales = kCodes + kWWords * THREADS * 4;
-    constexpr int kOutRow = 32 * FO * int(sizeof(T)) + 16;            // bytes of a pixel in the epilogue, padded
-    constexpr int kOut = THREADS / 64 * 32 * kOutRow, kLds = 2 * kStage > kOut ? 2 * kStage : kOut;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
-    __shared__ __attribute__((aligned(16))) float sBias[BO];
+    using L = TileLds<T, THREADS, BO, BP, FO>;
+    constexpr int kCodes = L::kCodes, kStage = L::kStage, kXScales = L::kXScales, kOutRow = L::kOutRow;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
+    uint8_t* const lds = dyn + L::kBias;
+    float* const sBias = reinterpret_cast<float*>(dyn);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
     // Workgroups are dealt round-robin over the 8 XCDs.  Where there are enough pixel tiles, all channel tiles of the same
     // pixels go to one XCD and share its L2 (256 -> 256 channels, 1x1, 65536 pixels, 64x64 tiles: 13.4 instead of 16.5 us);
@@ -821,11 +832,19 @@ hipError_t launch(const ConvMxArgs& args, hipStream_t s)
     if (grid > INT32_MAX) return hipErrorInvalidValue;
     const dim3 g(static_cast<unsigned>(grid)), block(THREADS);
     const bool within = a.taps == 1 || a.blocks % kChunk == 0 || !tapsInRange(a), words = scalesInWords(a);
-    if (within && words) hipLaunchKernelGGL((ConvMxKernel<T, THREADS, BO, BP, FO, FP, true, true>), g, block, 0, s, a);
-    else if (within) hipLaunchKernelGGL((ConvMxKernel<T, THREADS, BO, BP, FO, FP, true, false>), g, block, 0, s, a);
-    else if (words) hipLaunchKernelGGL((ConvMxKernel<T, THREADS, BO, BP, FO, FP, false, true>), g, block, 0, s, a);
-    else hipLaunchKernelGGL((ConvMxKernel<T, THREADS, BO, BP, FO, FP, false, false>), g, block, 0, s, a);
-    return hipGetLastError();
+    // one chunk needs one buffer: more workgroups fit a CU (8 -> 416 channels, 1x7, 100500 pixels: 23.3 instead of 26.2 us)
+    const int chunks = within ? a.taps * ((a.blocks + kChunk - 1) / kChunk) : (a.total + kChunk - 1) / kChunk;
+    const int lds = TileLds<T, THREADS, BO, BP, FO>::bytes(chunks > 1 ? 2 : 1);
+    const auto launchAs = [&](auto kernel) {
+        const hipError_t e = dev::ensureDynamicLds(reinterpret_cast<const void*>(kernel), TileLds<T, THREADS, BO, BP, FO>::bytes(2));
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL(kernel, g, block, lds, s, a);
+        return hipGetLastError();
+    };
+    if (within && words) return launchAs(ConvMxKernel<T, THREADS, BO, BP, FO, FP, true, true>);
+    if (within) return launchAs(ConvMxKernel<T, THREADS, BO, BP, FO, FP, true, false>);
+    if (words) return launchAs(ConvMxKernel<T, THREADS, BO, BP, FO, FP, false, true>);
+    return launchAs(ConvMxKernel<T, THREADS, BO, BP, FO, FP, false, false>);
 }
 
 template <int THREADS, int BO, int BP, int FO, int FP>
