@@ -325,8 +325,8 @@ srx_status srx_layer_add(int32_t dtype, const void* a, const void* b, void* out,
  *     may overlap on different streams as long as their outputs and workspaces are different memory.
  *   - Results do not depend on what runs beside a call: no atomics, fixed orders of summation.
  *   - A call that is refused (SRX_ERR_INVALID) has launched nothing.  Sizes of zero are refused.
- *   - At most 2^20 channels and filters; in srx_layer_conv2d_mx4 N*H*W is at most 2^31 - 1 and kh * kw * ceil(C / 32)
- *     below 2^19.
+ *   - At most 2^20 channels and filters; in srx_layer_group_norm* N * groups is at most 2^31 - 1; in
+ *     srx_layer_conv2d_mx4 N*H*W is at most 2^31 - 1 and kh * kw * ceil(C / 32) below 2^19.
  *
  * Activations: 0 = none, 1 = ReLU, 2 = SiLU, y / (1 + exp(-y)).
  *
@@ -355,8 +355,10 @@ srx_status srx_layer_group_norm_workspace(int32_t dtype, const uint32_t sizes[4]
 /* Group normalisation with an activation.  The channels are taken in `groups` groups of C / groups neighbours; with the
  * mean and the (uncorrected) variance of an image's group over all its pixels,
  *     out = act((in - mean) / sqrt(variance + epsilon) * scale[c] + bias[c]).
- * epsilon is a positive normal number; scale and bias are C values of the tensor's type, NULL stands for 1 and 0.  `out` may be `in`.  The workspace may be
- * reused by the next call on the same stream. */
+ * epsilon is a positive normal number; scale and bias are C values of the tensor's type, NULL stands for 1 and 0.
+ * `out` may be `in` (no other operands of these layers may overlap an output).  A NaN or an infinity makes NaN of its
+ * group, and so do fp32 values whose sum, or whose squared deviations' sum, passes the range of fp32.  The workspace may
+ * be reused by the next call on the same stream. */
 srx_status srx_layer_group_norm(int32_t dtype, const void* in, const uint32_t sizes[4], uint32_t groups,
                                 const void* scale, const void* bias, float epsilon, int32_t activation, void* out,
                                 void* workspace, size_t workspace_bytes, void* stream);

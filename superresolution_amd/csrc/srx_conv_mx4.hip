@@ -184,17 +184,18 @@ __global__ __launch_bounds__(THREADS, 2) void ConvMxKernel(const ConvMxArgs a)
     // pixels go to one XCD and share its L2 (256 -> 256 channels, 1x1, 65536 pixels, 64x64 tiles: 13.4 instead of 16.5 us);
     // pixels are dealt out singly (one long run of them for each XCD: 163 instead of 134 us for 64 -> 64 channels, 3x3,
     // 1920x1080).
+    const unsigned number = blockNumber();
     unsigned tileO, tileP;
     if (a.tilesP >= 64)
     {
-        const unsigned turn = blockIdx.x >> 3, round = a.byTilesO(turn);
+        const unsigned turn = number >> 3, round = a.byTilesO(turn);
         tileO = turn - round * a.tilesO;
-        tileP = round * 8 + (blockIdx.x & 7);
+        tileP = round * 8 + (number & 7);
     }
     else
     {
-        tileP = a.byTilesO(blockIdx.x);
-        tileO = blockIdx.x - tileP * a.tilesO;
+        tileP = a.byTilesO(number);
+        tileO = number - tileP * a.tilesO;
     }
     if (tileP >= unsigned(a.tilesP)) return;
     const int o0 = int(tileO) * BO;
@@ -830,7 +831,7 @@ hipError_t launch(const ConvMxArgs& args, hipStream_t s)
     a.tilesP = int((int64_t(a.pixels) + BP - 1) / BP);
     const int64_t grid = int64_t(a.tilesO) * (a.tilesP >= 64 ? (a.tilesP + 7) / 8 * 8 : a.tilesP);
     if (grid > INT32_MAX) return hipErrorInvalidValue;
-    const dim3 g(static_cast<unsigned>(grid)), block(THREADS);
+    const dim3 g = gridOf(grid), block(THREADS);
     const bool within = a.taps == 1 || a.blocks % kChunk == 0 || !tapsInRange(a), words = scalesInWords(a);
     // one chunk needs one buffer: more workgroups fit a CU (8 -> 416 channels, 1x7, 100500 pixels: 23.3 instead of 26.2 us)
     const int chunks = within ? a.taps * ((a.blocks + kChunk - 1) / kChunk) : (a.total + kChunk - 1) / kChunk;

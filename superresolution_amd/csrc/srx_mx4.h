@@ -23,6 +23,15 @@ struct Divider
     __device__ __forceinline__ unsigned operator()(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
 };
 
+// Grids of up to 2^31 - 1 workgroups: one dimension has to stay below 2^32 threads, so they come in rows of 2^21.
+constexpr unsigned kGridRow = 1u << 21;
+inline dim3 gridOf(int64_t blocks)
+{
+    return blocks <= int64_t(kGridRow) ? dim3(unsigned(blocks)) : dim3(kGridRow, unsigned((blocks + kGridRow - 1) / kGridRow));
+}
+// Number of this workgroup; those behind the last one of the grid asked for leave at once.
+__device__ __forceinline__ unsigned blockNumber() { return blockIdx.y * kGridRow + blockIdx.x; }
+
 constexpr int kMxBlock = 32;                          // values that share a scale
 constexpr int kMxBytes = kMxBlock / 2;                // bytes of a block's codes
 
@@ -183,7 +192,8 @@ __device__ __forceinline__ void storeUpTo8(T* p, int count, const float (&v)[8])
 }
 
 // 0 none, 1 ReLU, 2 SiLU: y / (1 + exp(-y)), with the exponential and the reciprocal of the special function unit
-// (an error of one part in 2^22 at most for the |y| where the result is not zero).  ReLU is the maximum that passes a NaN on.
+// (one part in 2^22 each; the product of y and log2(e) adds |y| parts in 2^24 where y is negative, and results below 1e-36
+// in magnitude may become zero).  ReLU is the maximum that passes a NaN on.
 __device__ __forceinline__ float activate(float y, int activation)
 {
     if (activation == 1) return __builtin_elementwise_maximum(y, 0.0f);

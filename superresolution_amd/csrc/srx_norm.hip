@@ -32,6 +32,7 @@ struct NormArgs
     int tileGroups, tiles;            // whole groups per workgroup (statistics, slabs)
     int applyChunks, applyPixels, applyTiles;
     int groupsInAll;                  // N * G
+    int blocks;                       // workgroups of this launch
     int slabRows;                     // pixels that the threads of a slab hold at a time
     Divider byTiles, byChunks, byGroupC, byVecs;
     float epsilon;
@@ -211,7 +212,9 @@ __global__ __launch_bounds__(THREADS) void NormSlabKernel(const NormArgs a)
     __shared__ __attribute__((aligned(16))) float sPart[THREADS * kVec];
     __shared__ float sTeam[THREADS];
     __shared__ float2 sStat[THREADS * kVec];
-    const int tid = threadIdx.x, n = int(a.byTiles(blockIdx.x)), tile = int(blockIdx.x) - n * a.tiles;
+    const unsigned number = blockNumber();
+    if (number >= unsigned(a.blocks)) return;
+    const int tid = threadIdx.x, n = int(a.byTiles(number)), tile = int(number) - n * a.tiles;
     const int g0 = tile * a.tileGroups, groups = min(a.tileGroups, a.G - g0);
     const int c0 = g0 * a.groupC, tileC = groups * a.groupC;
     // (the last tile may be narrower: its threads keep the others' places)
@@ -341,7 +344,9 @@ template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
 {
     __shared__ __attribute__((aligned(16))) float sMean[kTileC], sM2[kTileC];
-    const int b = int(a.byTiles(blockIdx.x)), tile = int(blockIdx.x) - b * a.tiles;
+    const unsigned number = blockNumber();
+    if (number >= unsigned(a.blocks)) return;
+    const int b = int(a.byTiles(number)), tile = int(number) - b * a.tiles;
     const int n = int(a.byChunks(unsigned(b))), chunk = b - n * a.chunks;
     const int g0 = tile * a.tileGroups, groups = min(a.tileGroups, a.G - g0);
     const int c0 = g0 * a.groupC, tileC = groups * a.groupC;
@@ -516,7 +521,9 @@ __global__ __launch_bounds__(kThreads) void NormApplyKernel(const NormArgs a)
 {
     __shared__ float2 sStat[kTileC];
     // from the last part to the first: the statistics kernel read the last ones last, so they are still cached
-    const int b0 = int(gridDim.x - 1 - blockIdx.x), b = int(a.byTiles(unsigned(b0))), tile = b0 - b * a.tiles;
+    const unsigned number = blockNumber();
+    if (number >= unsigned(a.blocks)) return;
+    const int b0 = a.blocks - 1 - int(number), b = int(a.byTiles(unsigned(b0))), tile = b0 - b * a.tiles;
     const int n = int(a.byChunks(unsigned(b))), chunk = b - n * a.applyChunks;
     const int c0 = tile * kTileC, tileC = min(kTileC, a.C - c0);
     const int g0 = int(a.byGroupC(unsigned(c0))), groups = int(a.byGroupC(unsigned(c0 + tileC - 1))) + 1 - g0;
@@ -629,7 +636,7 @@ struct Unit
 template <typename T>
 __global__ __launch_bounds__(kThreads) void QuantizeKernel(const MxArgs a)
 {
-    const int64_t base = int64_t(blockIdx.x) * (kThreads * kUnits);
+    const int64_t base = int64_t(blockNumber()) * (kThreads * kUnits);
     const int64_t row0 = base / a.rowUnits;
     const unsigned rem = unsigned(base - row0 * a.rowUnits);
     const T* in = static_cast<const T*>(a.in);
@@ -667,7 +674,7 @@ __global__ __launch_bounds__(kThreads) void QuantizeKernel(const MxArgs a)
 template <typename T>
 __global__ __launch_bounds__(kThreads) void DequantizeKernel(const MxArgs a)
 {
-    const int64_t base = int64_t(blockIdx.x) * (kThreads * kUnits);
+    const int64_t base = int64_t(blockNumber()) * (kThreads * kUnits);
     const int64_t row0 = base / a.rowUnits;
     const unsigned rem = unsigned(base - row0 * a.rowUnits);
     unsigned codes[kUnits], scale[kUnits];
@@ -725,7 +732,7 @@ NormPlan planNorm(const ML::Operator& op, bool mx4)
     p.images = op.inputSizes[0];
     const int64_t n = p.images;
     a.byGroupC = Divider(unsigned(a.groupC));
-    a.groupsInAll = int(n * a.G < INT32_MAX ? n * a.G : INT32_MAX);
+    a.groupsInAll = int(n * a.G);          // (the factory refuses more than 2^31 - 1)
 
     // Slabs of the fewest groups that are a whole number of 64-byte lines (of blocks of 32 channels), or of single groups.  A
     // slab has one CU's arithmetic: with SiLU 8192 values take 4.2 us, 32768 take 8.5, 131072 take 25, against 10 us for
@@ -766,8 +773,11 @@ NormPlan planNorm(const ML::Operator& op, bool mx4)
     if (chunks > kJoin) chunks = imageBytes <= int64_t(kJoin) * (192 << 10) ? kJoin : (imageBytes + (64 << 10) - 1) / (64 << 10);
     const int64_t most = (1024 + n * a.tiles - 1) / (n * a.tiles);
     if (chunks > most) chunks = most;
-    // (no part is longer than 2^22 pixels: a thread's sums stay short)
-    if (chunks < (a.pixels + (1 << 22) - 1) >> 22) chunks = (a.pixels + (1 << 22) - 1) >> 22;
+    // No thread adds up more than 256 values of a channel (parts of 1 MB in fp16): the rounding of its sums, about a first value
+    // that may be far from the others, grows with their number.
+    const int64_t longest = kThreads * int64_t(256) / vecsFor<false>(a.tileGroups * a.groupC);
+    const int64_t least = longest > 1 ? (a.pixels + longest - 1) / longest : a.pixels;
+    if (chunks < least) chunks = least;
     a.chunkPixels = int((a.pixels + chunks - 1) / chunks);
     a.chunks = int((a.pixels + a.chunkPixels - 1) / a.chunkPixels);
     // Output: about 1024 workgroups (256x256 pixels of 256 channels in 4 bits: 13.0 us; 2048: 14.6), four batches of pixels
@@ -796,7 +806,9 @@ hipError_t launchNorm(const NormPlan& p, hipStream_t s)
     const NormArgs& a = p.a;
     if (p.slabThreads)
     {
-        const dim3 grid(static_cast<unsigned>(p.images * a.tiles));
+        NormArgs a = p.a;
+        a.blocks = int(p.images * a.tiles);
+        const dim3 grid = gridOf(a.blocks);
         if (p.slabThreads == 256 && p.slabHeld == 1) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 256, 1>), grid, dim3(256), 0, s, a);
         else if (p.slabThreads == 256) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 256, 4>), grid, dim3(256), 0, s, a);
         else if (p.slabHeld <= 2) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 1024, 2>), grid, dim3(1024), 0, s, a);
@@ -812,9 +824,11 @@ hipError_t launchNorm(const NormPlan& p, hipStream_t s)
     ap.tiles = a.applyTiles;
     ap.byTiles = Divider(unsigned(a.applyTiles));
     ap.byChunks = Divider(unsigned(a.applyChunks));
+    st.blocks = int(statsGrid);
+    ap.blocks = int(applyGrid);
     const bool whole = a.C % kVec == 0 && (a.tileGroups == a.G || (a.tileGroups * a.groupC) % kVec == 0);
-    if (whole) hipLaunchKernelGGL((NormStatsKernel<T, true>), dim3(unsigned(statsGrid)), block, 0, s, st);
-    else hipLaunchKernelGGL((NormStatsKernel<T, false>), dim3(unsigned(statsGrid)), block, 0, s, st);
+    if (whole) hipLaunchKernelGGL((NormStatsKernel<T, true>), gridOf(statsGrid), block, 0, s, st);
+    else hipLaunchKernelGGL((NormStatsKernel<T, false>), gridOf(statsGrid), block, 0, s, st);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (a.chunks > kJoin)
@@ -822,8 +836,8 @@ hipError_t launchNorm(const NormPlan& p, hipStream_t s)
         hipLaunchKernelGGL(NormJoinKernel, dim3(unsigned(a.groupsInAll)), dim3(64), 0, s, a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    if (a.C % kVec == 0) hipLaunchKernelGGL((NormApplyKernel<T, MX4, true>), dim3(unsigned(applyGrid)), block, 0, s, ap);
-    else hipLaunchKernelGGL((NormApplyKernel<T, MX4, false>), dim3(unsigned(applyGrid)), block, 0, s, ap);
+    if (a.C % kVec == 0) hipLaunchKernelGGL((NormApplyKernel<T, MX4, true>), gridOf(applyGrid), block, 0, s, ap);
+    else hipLaunchKernelGGL((NormApplyKernel<T, MX4, false>), gridOf(applyGrid), block, 0, s, ap);
     return hipGetLastError();
 }
 
@@ -863,7 +877,7 @@ bool planMx(int64_t rows, int64_t columns, int bytes, MxArgs& a, dim3& grid)
     a.byRow = Divider(a.rowUnits);
     a.stream = a.values * bytes > kStreamBytes;
     const int64_t blocks = (a.units + kThreads * kUnits - 1) / (kThreads * kUnits);
-    grid = dim3(unsigned(blocks));
+    grid = gridOf(blocks);
     return blocks <= INT32_MAX;
 }
 }  // namespace

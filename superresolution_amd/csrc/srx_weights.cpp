@@ -165,6 +165,7 @@ bool Util::CreateGroupNormLayer(const uint32_t inputSizes[4], uint32_t groups, f
 {
     if (!validSizes(inputSizes) || m_dataType == TensorDataType::UNKNOWN || m_layout != TensorLayout::NHWC) return false;
     if (groups == 0 || inputSizes[1] % groups != 0 || inputSizes[1] > kMaxChannels) return false;
+    if (uint64_t(inputSizes[0]) * groups > uint64_t(INT32_MAX)) return false;
     if (!(epsilon >= FLT_MIN) || !std::isfinite(epsilon) || activation > uint32_t(Activation::SILU)) return false;
     opOut = Operator{};
     opOut.kind = Operator::Kind::GROUP_NORM;

@@ -85,7 +85,7 @@ public:
                                 uint32_t outputSizes[4], Operator& opOut) const;
     bool CreateAdditionLayer(const uint32_t inputSizes[4], Operator& opOut) const;
     // No counterparts in the reference.  Both take channels-last tensors only (the NHWC layout).  Group normalisation:
-    // `groups` must divide the channels, epsilon must be a positive normal number.  Convolution of an input and a filter in
+    // `groups` must divide the channels (at most 2^31 - 1 groups in all images), epsilon must be a positive normal number.  Convolution of an input and a filter in
     // the 4-bit block form: sizes and padding as in CreateConvolutionLayer, filter sides up to 7, the output in the
     // tensor data type; at most 2^31 - 1 pixels in all.
     bool CreateGroupNormLayer(const uint32_t inputSizes[4], uint32_t groups, float epsilon, uint32_t activation,

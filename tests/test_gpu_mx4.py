@@ -301,6 +301,69 @@ def test_offsets_past_32_bits():
         assert ((x[at:at + 96].cpu().double() - want).abs() <= step(0, want) + U * 200 * (want.abs() + 1)).all()
 
 
+def test_more_threads_than_one_grid_dimension_holds():
+    """2^32 rows of one value, 2^31 - 1 pixels, 2^24 images of one pixel: workgroups whose threads number 2^32 and more."""
+    rows, pixels = (1 << 32) + 3, (1 << 31) - 1
+    tail = rnd((40, 1), 11)
+    x = torch.zeros(rows, 1, dtype=torch.float16, device="cuda")
+    at = (rows - 40, (1 << 31) - 41, 12345)
+    for a in at:
+        x[a:a + 40] = tail.cuda()
+    codes = torch.empty(rows, 16, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(rows, dtype=torch.uint8, device="cuda")
+    S.layer_quantize_mx4(0, x.data_ptr(), rows, 1, codes.data_ptr(), scales.data_ptr(), stream())
+    x.fill_(9)
+    S.layer_dequantize_mx4(0, codes.data_ptr(), scales.data_ptr(), rows, 1, x.data_ptr(), stream())
+    f = rnd((4, 1), 12)
+    wc, ws = quantise(f, 0)
+    y = torch.empty(pixels, 4, dtype=torch.float16, device="cuda")
+    S.layer_conv2d_mx4(0, codes.data_ptr(), scales.data_ptr(), (1, 1, 1, pixels), wc.ptr(), ws.ptr(), (4, 1, 1, 1), None, 0, y.data_ptr(), stream())
+    torch.cuda.synchronize()
+    want, want_s = quantise64(tail)
+    v = values64(want, want_s, 1)
+    product = (v * values64(wc.whole(), ws.whole(), 1).reshape(1, 4)).half()   # 4 bits of fraction at most: exact in fp16
+    for a in at:
+        assert torch.equal(codes[a:a + 40].cpu(), want[:, 0]) and torch.equal(scales[a:a + 40].cpu(), want_s[:, 0])
+        assert torch.equal(x[a:a + 40].cpu(), v.half())
+        if a + 40 <= pixels:
+            assert torch.equal(y[a:a + 40].cpu(), product)
+    assert float(x[rows - 41]) == 0 and float(y[1 << 30:(1 << 30) + 4096].abs().max()) == 0
+    del x, y, codes, scales
+    images = (1 << 24) + 3
+    x = torch.randn(images, 1, 1, 8, dtype=torch.float16, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    out = torch.empty_like(x)
+    need = S.layer_group_norm_workspace(0, (images, 8, 1, 1), 2)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    S.layer_group_norm(0, x.data_ptr(), (images, 8, 1, 1), 2, None, None, 1e-5, 0, out.data_ptr(), work.data_ptr(), need, stream())
+    torch.cuda.synchronize()
+    for a in (0, (1 << 21) - 20, (1 << 23) - 20, images - 40):
+        ref, *parts = norm64(x[a:a + 40].cpu(), 2, None, None, 1e-5, 0)
+        assert ((out[a:a + 40].cpu().double() - ref).abs() <= step(0, ref) + norm_tolerance(*parts)).all()
+
+
+def test_group_norm_first_value_far_from_the_others():
+    """Large parts of few channels, whose sums are taken about the first value: its distance must not drown the spread."""
+    n, h, w, c, d = 1, 8192, 8192, 4, 300.0
+    x = torch.randn(n, h, w, c, device="cuda", generator=torch.Generator("cuda").manual_seed(2))
+    x.view(-1, c)[::65536] += d
+    v = x.double().view(-1, 2, 2)
+    mean = v.mean(dim=(0, 2))
+    v = v - mean[:, None]
+    rstd = 1 / torch.sqrt((v ** 2).mean(dim=(0, 2)) + 1e-5)
+    want = (v * rstd[:, None]).view(n, h, w, c)
+    out = torch.empty_like(x)
+    need = S.layer_group_norm_workspace(1, (n, c, h, w), 2)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    S.layer_group_norm(1, x.data_ptr(), (n, c, h, w), 2, None, None, 1e-5, 0, out.data_ptr(), work.data_ptr(), need, stream())
+    torch.cuda.synchronize()
+    # A thread adds up 256 values at most; the one of 256 threads whose first value is the far one adds up squares of d:
+    # U * i * d^2 at term i, 256^2 / 2 in all, and twice that in the square of its sum.  Its part's variance times the part's pixels
+    # is 65536 (1 + d^2 / 65536); the result has half the variance's relative error.  Its mean is off by 256 U d, the
+    # part's by d U, the other sums by 80 half steps of the spread and the mean as in norm_tolerance.
+    off = 1.5 * 256 ** 2 * U * d ** 2 / (65536 + d ** 2) / 2
+    assert ((out.double() - want).abs() <= off * want.abs() + U * (80 * (want.abs() + 1) + d)).all()
+
+
 # ---------------------------------------------------------------------------
 # Group normalisation
 # ---------------------------------------------------------------------------

@@ -62,6 +62,13 @@ def test_group_norm_arguments_refused(change):
     refused(S.layer_group_norm_mx4, dtype, x, sizes, groups, scale, bias, epsilon, act, codes, P, work, nbytes)
 
 
+def test_group_norm_counts_groups_in_31_bits():
+    refused(S.layer_group_norm, *norm(sizes=(1 << 31, 1, 1, 1), groups=1))
+    refused(S.layer_group_norm, *norm(sizes=(1 << 28, 8, 1, 1), groups=8))
+    refused(S.layer_group_norm_workspace, 0, (1 << 28, 8, 1, 1), 8)
+    assert S.layer_group_norm_workspace(0, ((1 << 28) - 1, 8, 1, 1), 8) == 0
+
+
 def test_group_norm_mx4_needs_both_outputs():
     refused(S.layer_group_norm_mx4, 0, P, (1, 8, 4, 4), 2, P, P, 1e-5, 0, P, None, P, 1 << 20)
 
