@@ -6,6 +6,17 @@
 // reduction over the blocks of 32 channels of every tap, numbered kb = tap * (blocks of a pixel) + block.  One
 // instruction multiplies two blocks: lanes 0-31 hold one of them for 32 rows (or columns), lanes 32-63 the other, 16
 // bytes and one scale byte each, so that the two blocks may come from different taps.  fp32 accumulation.
+//
+// Three kernels, chosen by LaunchConvMx4; times of the kernels themselves, fp16 results (they differ by 5 % between devices,
+// and by as much between operands of all bit patterns and those of a normalised layer: the power limit):
+//   ConvMxRowsKernel    few pixels; bound by the latency of one trip to memory and of the join.  One row times 4096 x 4096: 6.0 us
+//                       (8.9 MB of filter: 1.5 TB/s).
+//   ConvMxWindowKernel  up to 64 channels on large images; bound by the output's bytes.  64 -> 64 channels, 3x3, 1920x1080:
+//                       74 us (336 MB: 4.5 TB/s; 2.1 PFLOP/s).
+//   ConvMxKernel        everything else.  512 -> 512 channels, 3x3, 256x256: 80 - 84 us, 3.7 - 3.9 PFLOP/s.  The matrix units
+//                       alone reach 6.2 on such operands held in registers (at the power limit; 7.7 on constants), 5.5 where
+//                       every operand is read from LDS; without its loads from memory this kernel takes 66 of 102 us, without
+//                       its reads from LDS 87: L2, LDS and power together bound it.
 #include "srx_mx4.h"
 
 namespace srx {
@@ -181,9 +192,9 @@ __global__ __launch_bounds__(THREADS, 2) void ConvMxKernel(const ConvMxArgs a)
     float* const sBias = reinterpret_cast<float*>(dyn);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
     // Workgroups are dealt round-robin over the 8 XCDs.  Where there are enough pixel tiles, all channel tiles of the same
-    // pixels go to one XCD and share its L2 (256 -> 256 channels, 1x1, 65536 pixels, 64x64 tiles: 13.4 instead of 16.5 us);
-    // pixels are dealt out singly (one long run of them for each XCD: 163 instead of 134 us for 64 -> 64 channels, 3x3,
-    // 1920x1080).
+    // pixels go to one XCD and share its L2 (512 -> 512 channels, 3x3, 256x256: 95 instead of 98 us; 128 -> 512, 1x1: 18.3
+    // instead of 18.6); pixels are dealt out singly (one long run of them for each XCD: 95, and 12.2 instead of 11.8 for 256 ->
+    // 256, 1x1).
     const unsigned number = blockNumber();
     unsigned tileO, tileP;
     if (a.tilesP >= 64)
@@ -833,7 +844,7 @@ hipError_t launch(const ConvMxArgs& args, hipStream_t s)
     if (grid > INT32_MAX) return hipErrorInvalidValue;
     const dim3 g = gridOf(grid), block(THREADS);
     const bool within = a.taps == 1 || a.blocks % kChunk == 0 || !tapsInRange(a), words = scalesInWords(a);
-    // one chunk needs one buffer: more workgroups fit a CU (8 -> 416 channels, 1x7, 100500 pixels: 23.3 instead of 26.2 us)
+    // one chunk needs one buffer: more workgroups fit a CU (8 -> 416 channels, 1x7, 100500 pixels: 24 instead of 33 us)
     const int chunks = within ? a.taps * ((a.blocks + kChunk - 1) / kChunk) : (a.total + kChunk - 1) / kChunk;
     const int lds = TileLds<T, THREADS, BO, BP, FO>::bytes(chunks > 1 ? 2 : 1);
     const auto launchAs = [&](auto kernel) {
@@ -887,25 +898,27 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
 
     // Few pixels: the shared reduction (ConvMxRowsKernel), as wide as 256 workgroups allow, while what its workgroups read
     // (their number times 1 + FP rows of 16) takes less time than the chunks of a tile take one after the other.
-    // 4096 -> 4096 channels, 1x1: 4.1 (1 pixel), 9.2 (64) us instead of 9.9, 10.2 with tiles of 64x64; 26.8 instead of 13.5
-    // for 256 pixels.  256 -> 256 channels, 3x3, 16x16: 3.8 instead of 6.9.
+    // 4096 -> 4096 channels, 1x1: 5.3 (1 pixel), 8.9 (64) us instead of 9.4, 9.6 with tiles; 31 instead of 10.3 for 256
+    // pixels.  256 -> 256 channels, 3x3, 16x16: 4.0 instead of 6.6; 1024 -> 1024, 3x3, 8x8: 8.0 instead of 18.
     const int rows = tiles(16, 64) >= 256 ? 4 : tiles(16, 32) >= 256 ? 2 : 1;
     if (tiles(16, 16 * rows) * (1 + rows) < 1560 && tapsInRange(a))
         return rows == 4 ? launchRows<4>(half, a, s) : rows == 2 ? launchRows<2>(half, a, s) : launchRows<1>(half, a, s);
-    // Up to 64 channels on large images: the window kernel.  64 -> 64 channels, 3x3: 92 instead of 139 us for 1920x1080, 17.8
-    // instead of 20 for 640x360 (900 tiles), but 8.4 instead of 7.2 for 320x180 (240); 1x1, 1920x1080: 74 instead of 104.
-    // 96 -> 96, 3x3, 960x540: 83 instead of 78.  32 -> 128, 3x3, 512x512: 22 instead of 29; 64 -> 256, 3x3, 256x256: 17.2
-    // instead of 15.6.  fp32 results leave room for 32 channels at a time only (34 instead of 43 us).
+    // Up to 64 channels on large images: the window kernel.  64 -> 64 channels, 3x3: 90 instead of 162 us for 1920x1080
+    // (codes of all bit patterns; 74 - 78 for those of a normalised layer), 15 instead of 22 for 640x360 (900 tiles), 7.3
+    // and 7.4 for 320x180 (240); 1x1, 1920x1080: 65 instead of 88.  32 -> 128, 3x3, 512x512: 18 instead of 26; with more
+    // channel tiles the window is read as often as the tiles read it (64 -> 256, 3x3, 256x256: 14.7 and 15.9).  fp32 results
+    // leave room for 32 channels at a time only (960x540: 33 instead of 46).
     if (a.blocks <= 2 && a.O <= 128 && a.W >= kWinW && a.H >= kWinH && tiles(64, 256) >= 768)
     {
         const hipError_t e = !half ? launchWindow<float, 1>(a, s) : a.O <= 32 ? launchWindow<f16, 1>(a, s) : launchWindow<f16, 2>(a, s);
         if (e != hipErrorInvalidConfiguration) return e;
     }
     // The largest tile that leaves no CU without one: 256x256 reads a quarter of what 64x64 does (512 -> 512 channels, 3x3,
-    // 256x256: 90 instead of 158 us), but 64 such tiles for 2048 -> 2048 channels, 1x1, 2048 pixels take 19 instead of 12.
-    // 128x128: 12.7 instead of 14.3 us with 128x64 for 96 -> 96, 3x3, 256x256; 12.4 instead of 12.2 for 256 tiles.
-    // Channels that only fill up a tile count: 160 -> 160, 3x3, 256x256 in 256: 22.4 instead of 24.1 us, but 8 -> 416, 1x7,
-    // 100500 pixels in 512: 39 instead of 29 (nothing but the output takes time there).
+    // 256x256: 95 instead of 164 us), but 64 such tiles for 2048 -> 2048 channels, 1x1, 2048 pixels take 19 instead of 12.
+    // 128x128: 12.7 instead of 14.5 us with 128x64 for 96 -> 96, 3x3, 256x256; 8.7 instead of 8.1 for half as many pixels
+    // (256 tiles).  32x128: 19 instead of 24 with 64x64 for 96 -> 32, 3x3, 512x512.
+    // Channels that only fill up a tile count: 160 -> 160, 3x3, 256x256 in 256: 22.5 instead of 27.5 us, but 8 -> 416, 1x7,
+    // 100500 pixels in 512: 34 instead of 24 (nothing but the output takes time there).
     const auto padded = [&](int64_t o) { return (a.O + o - 1) / o * o; };
     const bool deep = a.total > 2 * kChunk;
     if (a.O > 128 && tiles(256, 256) >= 256 && padded(256) * 10 <= padded(64) * (deep ? 14 : 10)) return launch<512, 256, 256, 4, 2>(half, a, s);
