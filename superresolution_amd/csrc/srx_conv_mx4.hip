@@ -7,12 +7,14 @@
 // instruction multiplies two blocks: lanes 0-31 hold one of them for 32 rows (or columns), lanes 32-63 the other, 16
 // bytes and one scale byte each, so that the two blocks may come from different taps.  fp32 accumulation.
 //
-// Three kernels, chosen by LaunchConvMx4; times of the kernels themselves, fp16 results (they differ by 5 % between devices,
+// Four kernels, chosen by LaunchConvMx4; times of the kernels themselves, fp16 results (they differ by 5 % between devices,
 // and by as much between operands of all bit patterns and those of a normalised layer: the power limit):
 //   ConvMxRowsKernel    few pixels; bound by the latency of one trip to memory and of the join.  One row times 4096 x 4096: 6.0 us
 //                       (8.9 MB of filter: 1.5 TB/s).
 //   ConvMxWindowKernel  up to 64 channels on large images; bound by the output's bytes.  64 -> 64 channels, 3x3, 1920x1080:
 //                       74 us (336 MB: 4.5 TB/s; 2.1 PFLOP/s).
+//   ConvMxTapsKernel    several taps, up to 256 channels.  96 -> 96, 3x3, 960x540: 47 us (126 MB, 86 GFLOP: 2.7 TB/s, 1.8 PFLOP/s), bound
+//                       by the start and end of its tiles as much as by the products; 256 -> 256, 256x256: 27 us, 2.8 PFLOP/s.
 //   ConvMxKernel        everything else.  512 -> 512 channels, 3x3, 256x256: 80 - 84 us, 3.7 - 3.9 PFLOP/s.  The matrix units
 //                       alone reach 6.2 on such operands held in registers (at the power limit; 7.7 on constants), 5.5 where
 //                       every operand is read from LDS; without its loads from memory this kernel takes 66 of 102 us, without
@@ -104,10 +106,11 @@ __device__ __forceinline__ void finishAs(const ConvMxArgs& a, const f32x16 (&acc
 {
     constexpr int kOutRow = 32 * FO * int(sizeof(T)) + 16;
     constexpr int kN = 16 / int(sizeof(T)), kPerRow = 32 * FO / kN;   // elements of a store, stores of a pixel
-    constexpr int kPass = 64 / kPerRow;                               // pixels stored at a time
+    constexpr bool kEven = 64 % kPerRow == 0;
+    constexpr int kPass = 64 / kPerRow, kStores = kPerRow / 2;        // pixels stored at a time (kEven), times for 32 pixels
     typedef T T4 __attribute__((ext_vector_type(4)));
-    const int h = lane >> 5, l = lane & 31, px = lane / kPerRow, part = lane % kPerRow;
-    const int channels = a.O - o0 - part * kN;                        // that exist from this lane's first on
+    const int h = lane >> 5, l = lane & 31;
+    int px = lane / kPerRow, part = lane % kPerRow, channels = a.O - o0 - part * kN;   // channels that exist from this lane's first on
     const unsigned lanes = unsigned(px) * unsigned(a.O) * unsigned(sizeof(T)) + part * 16, pass = unsigned(kPass) * unsigned(a.O) * unsigned(sizeof(T));
 #pragma unroll
     for (int j = 0; j < FP; ++j)
@@ -129,11 +132,18 @@ __device__ __forceinline__ void finishAs(const ConvMxArgs& a, const f32x16 (&acc
         int count;
         place(j, to, count);
 #pragma unroll
-        for (int u = 0; u < 32 / kPass; ++u)
+        for (int u = 0; u < kStores; ++u)
         {
-            const uint4 v = *reinterpret_cast<const uint4*>(mine + (u * kPass + px) * kOutRow + part * 16);
-            if (u * kPass + px >= count) continue;
-            uint8_t* dst = to + (lanes + u * pass);
+            if (!kEven)
+            {
+                px = (u * 64 + lane) / kPerRow;
+                part = (u * 64 + lane) % kPerRow;
+                channels = a.O - o0 - part * kN;
+            }
+            const int row = kEven ? u * kPass + px : px;
+            const uint4 v = *reinterpret_cast<const uint4*>(mine + row * kOutRow + part * 16);
+            if (row >= count) continue;
+            uint8_t* dst = to + (kEven ? lanes + u * pass : unsigned(px) * unsigned(a.O) * unsigned(sizeof(T)) + part * 16);
             if (channels >= kN)
             {
                 typedef unsigned u32x4_at __attribute__((ext_vector_type(4), aligned(2)));
@@ -833,6 +843,323 @@ hipError_t launchWindow(const ConvMxArgs& a, hipStream_t s)
     return hipErrorInvalidConfiguration;
 }
 
+// Filters of several taps and up to eight blocks a pixel: a tile's pixels are eight rows of 32, and the window that all its
+// taps see is staged once, so that only the filters come from memory chunk by chunk (ConvMxKernel reads every pixel once for each
+// tap, more than L2 delivers while tiles of 128 channels are multiplied).  A workgroup makes 32 * FO channels, a wave
+// two rows of them.
+struct TapsArgs
+{
+    int winW, winPixels;
+    int scales;                       // place of the window's scales behind its codes
+    int down, mask;                   // place of a pixel's block: block ^ (pixel >> down & mask); neighbouring 16 pixels lie in all banks
+    int tilesX, tilesY;
+    Divider byTilesX, byTilesY, byWinW;
+};
+
+template <typename T, int FO>
+struct TapsLds
+{
+    static constexpr int kBO = 32 * FO, kStage = kBO * kRow + kThreads * 4;
+    static constexpr int kOutRow = 32 * FO * int(sizeof(T)) + 16, kOut = kThreads / 64 * 32 * kOutRow;
+    // two chunks of filters (codes, scales; the bias in the second one's place at first) and the window, later the turn of the results
+    static int bytes(int window) { return 2 * kStage + window > kOut ? 2 * kStage + window : kOut; }
+};
+
+constexpr int kTapsLoads = 16;        // of a window, at most
+
+// WORDS: four or eight blocks a pixel, whose scales are staged in words; otherwise byte by byte.
+// As many waves a SIMD as the accumulators leave room for (96 -> 96 channels, 960x540: 49 us with three, 53 with two).
+template <typename T, int FO, bool WORDS>
+__global__ __launch_bounds__(kThreads, FO > 3 ? 2 : FO > 2 ? 3 : 4) void ConvMxTapsKernel(const ConvMxArgs a, const TapsArgs w)
+{
+    using L = TapsLds<T, FO>;
+    constexpr int kBO = L::kBO, kStage = L::kStage, kScales = kBO * kRow, kWindow = 2 * kStage, FP = 2, kPass = kThreads / 8, kWRows = kBO / kPass;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
+    const unsigned ldsAt = unsigned(uintptr_t((__attribute__((address_space(3))) uint8_t*)dyn));
+    // as in ConvMxKernel
+    const unsigned number = blockNumber(), turn = number >> 3, round = a.byTilesO(turn), tileP = round * 8 + (number & 7);
+    if (tileP >= unsigned(a.tilesP)) return;
+    const int o0 = int(turn - round * unsigned(a.tilesO)) * kBO;
+    const unsigned tileY = w.byTilesX(tileP), n = w.byTilesY(tileY);
+    const int x0 = int(tileP - tileY * unsigned(w.tilesX)) * kWinW, y0 = int(tileY - n * unsigned(w.tilesY)) * kWinH;
+    const int r0 = 2 * wave;
+    const auto place = [&](unsigned p, unsigned block) { return block ^ ((p >> w.down) & unsigned(w.mask)); };
+
+    // The filters' next chunk of eight blocks; beyond the last, nothing is read.
+    const int sr = tid >> 3, sb = (tid & 7) ^ ((sr >> 1) & 7), zr = tid >> 1, zb = (tid & 1) * 4;
+    i32x4 wd, vd;
+    unsigned wOff[kWRows], off[kWRows], zOff = 0;
+    uint8_t wz[kWRows];
+#pragma unroll
+    for (int i = 0; i < kWRows; ++i) wOff[i] = o0 + sr + kPass * i < a.O ? unsigned((sr + kPass * i) * a.total + sb) * kMxBytes : kRange;
+    const unsigned vOff = zr < kBO && o0 + zr < a.O ? unsigned(zr * a.total + zb) : kRange;
+    int next = 0;
+    const auto prepare = [&]() {
+        wd = descriptor(a.wCodes + (int64_t(o0) * a.total + next) * kMxBytes, kRange);
+        vd = descriptor(a.wScales + int64_t(o0) * a.total + next, WORDS ? kRange : kRange >> 4);
+        const unsigned out = next + sb < a.total ? 0u : kRange;
+#pragma unroll
+        for (int i = 0; i < kWRows; ++i) off[i] = wOff[i] | out;
+        zOff = vOff | (next + zb < a.total ? 0u : kRange);
+        next += kChunk;
+    };
+    constexpr int kLoads = kWRows + (WORDS ? 1 : 0);
+    const auto load = [&](int i, int stage) {
+        if (i < kWRows) loadToLds(wd, off[i], ldsAt + stage + wave * 1024 + i * kThreads * 16);
+        else loadWordToLds(vd, zOff, ldsAt + stage + kScales + wave * 256);
+    };
+    const auto loadBytes = [&]() {
+#pragma unroll
+        for (int i = 0; i < kWRows; ++i) wz[i] = uint8_t(loadByte(vd, off[i] / kMxBytes));
+    };
+    const auto settle = [&](int stage) {
+#pragma unroll
+        for (int i = 0; i < kWRows; ++i) dyn[stage + kScales + (sr + kPass * i) * kChunk + sb] = wz[i];
+    };
+
+    // Operands of step s of the current chunk: blocks s (lanes 0-31) and 4 + s (lanes 32-63).  Behind the last block the filters
+    // are zeros, and the last block's pixels, which are in the sum anyway, stand in.
+    int chunk = 0;
+    uint4 wf[2][FO], xf[2][FP];
+    unsigned ws[FO], oldW[FO], xs[2][FP], oldX[FP], xAt[FP];
+    // window pixel, counted from the wave's own, that each half of the wave reads for blocks kb0 and kb1; first pixel of a lane
+    const auto pixelOf = [&](int kb0, int kb1, int& b) {
+        int at[2], block[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+        {
+            const int kb = min(k ? kb1 : kb0, a.total - 1), tap = int(a.byBlocks(unsigned(kb))), ky = int(a.byKw(unsigned(tap)));
+            at[k] = ky * w.winW + tap - ky * a.kw;
+            block[k] = kb - tap * a.blocks;
+        }
+        b = h ? block[1] : block[0];
+        return r0 * w.winW + l + (h ? at[1] : at[0]);
+    };
+    const auto read = [&](int set, int stage, int s) {
+#pragma unroll
+        for (int i = 0; i < FO; ++i) wf[set][i] = *reinterpret_cast<const uint4*>(dyn + stage + slot(32 * i + l, 4 * h + s));
+        int b;
+        if (WORDS)
+        {
+            // a lane's four blocks are of one pixel: their places differ in two bits, and their scales are a word
+            if (s == 0)
+            {
+                const int p0 = pixelOf(chunk * kChunk, chunk * kChunk + 4, b);
+                b &= ~3;
+#pragma unroll
+                for (int j = 0; j < FP; ++j)
+                {
+                    const int p = p0 + j * w.winW;
+                    xAt[j] = kWindow + (unsigned(p * a.blocks) + place(unsigned(p), unsigned(b))) * 16;
+                    xs[0][j] = *reinterpret_cast<const unsigned*>(dyn + kWindow + w.scales + p * a.blocks + b);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < FP; ++j) xf[set][j] = *reinterpret_cast<const uint4*>(dyn + (xAt[j] ^ unsigned(s * 16)));
+        }
+        else
+        {
+            const int p0 = pixelOf(chunk * kChunk + s, chunk * kChunk + 4 + s, b);
+#pragma unroll
+            for (int j = 0; j < FP; ++j)
+            {
+                const int p = p0 + j * w.winW;
+                xf[set][j] = *reinterpret_cast<const uint4*>(dyn + kWindow + (unsigned(p * a.blocks) + place(unsigned(p), unsigned(b))) * 16);
+                xs[set][j] = dyn[kWindow + w.scales + p * a.blocks + b];
+            }
+        }
+    };
+    const auto readScales = [&](int stage) {
+#pragma unroll
+        for (int i = 0; i < FO; ++i) ws[i] = *reinterpret_cast<const unsigned*>(dyn + stage + kScales + (32 * i + l) * kChunk + 4 * h);
+    };
+#define SRX_STEP(S, SET, I, J, WS, XS)                                                                                 \
+    acc[I][J] = WORDS ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(wf[SET][I]), widen(xf[SET][J]), acc[I][J], 4, 4, S, WS[I], S, XS[J])   \
+                      : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(wf[SET][I]), widen(xf[SET][J]), acc[I][J], 4, 4, S, WS[I], 0, xs[SET][J]);
+#define SRX_MULTIPLY(S, SET)                                                                                           \
+    _Pragma("unroll") for (int i = 0; i < FO; ++i)                                                                     \
+        _Pragma("unroll") for (int j = 0; j < FP; ++j) { SRX_STEP(S, SET, i, j, ws, xs[0]) }
+
+    prepare();
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) load(i, 0);
+    if (!WORDS) loadBytes();
+    // the window: codes unit by unit, scales in words or with their codes
+    {
+        const int pixelBytes = a.blocks * kMxBytes;
+        const unsigned rowBytes = unsigned(a.W) * unsigned(pixelBytes);
+        const int64_t first = (int64_t(n) * a.H + y0 - a.padTop) * a.W + x0 - a.padLeft;
+        const i32x4 xd = descriptor(a.codes + first * pixelBytes, kRange), zd = descriptor(a.scales + first * a.blocks, WORDS ? kRange : kRange >> 4);
+        const auto offsetOf = [&](unsigned p) {                         // of a window's pixel, in codes; or kRange
+            const unsigned row = w.byWinW(p), col = p - row * unsigned(w.winW);
+            const bool in = unsigned(y0 - a.padTop + int(row)) < unsigned(a.H) && unsigned(x0 - a.padLeft + int(col)) < unsigned(a.W);
+            return in && p < unsigned(w.winPixels) ? row * rowBytes + col * unsigned(pixelBytes) : kRange;
+        };
+        const int units = w.winPixels * a.blocks;
+        uint8_t z[kTapsLoads];
+#pragma unroll
+        for (int i = 0; i < kTapsLoads; ++i)
+        {
+            if (i * kThreads + wave * 64 >= units) continue;
+            const unsigned u = i * kThreads + tid, p = a.byBlocks(u), o = offsetOf(p);
+            const unsigned from = o == kRange ? kRange : o + place(p, u - p * unsigned(a.blocks)) * kMxBytes;
+            loadToLds(xd, from, ldsAt + kWindow + (i * kThreads + wave * 64) * 16);
+            if (!WORDS) z[i] = uint8_t(loadByte(zd, from / kMxBytes));
+        }
+        if (WORDS)
+        {
+#pragma unroll
+            for (int i = 0; i < kTapsLoads / 4; ++i)
+            {
+                if (i * kThreads + wave * 64 >= units / 4) continue;
+                const unsigned u = i * kThreads + tid, p = a.blocks == 8 ? u >> 1 : u, o = offsetOf(p);
+                loadWordToLds(zd, o == kRange ? kRange : o / kMxBytes + (a.blocks == 8 ? (u & 1) * 4 : 0), ldsAt + kWindow + w.scales + (i * kThreads + wave * 64) * 4);
+            }
+        }
+        else
+        {
+#pragma unroll
+            for (int i = 0; i < kTapsLoads; ++i)
+            {
+                const unsigned u = i * kThreads + tid, p = a.byBlocks(u);
+                if (u < unsigned(units)) dyn[kWindow + w.scales + p * unsigned(a.blocks) + place(p, u - p * unsigned(a.blocks))] = z[i];
+            }
+            settle(0);
+        }
+    }
+    float* const bias = reinterpret_cast<float*>(dyn + kStage);
+    if (tid < kBO) bias[tid] = a.bias && o0 + tid < a.O ? (float)static_cast<const T*>(a.bias)[o0 + tid] : 0.0f;
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    f32x16 acc[FO][FP];
+    startAt<FO, FP>(acc, bias, h);
+    read(0, 0, 0);
+    readScales(0);
+    // the bias has been read by every wave: its place is the second chunk's
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const int chunks = (a.total + kChunk - 1) / kChunk;
+    if (chunks > 1)
+    {
+        prepare();
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) load(i, kStage);
+        if (!WORDS) loadBytes();
+    }
+    int stage = 0;
+    for (int c = 1; c < chunks; ++c)
+    {
+        // (no branch in here: the compiler would move the products behind it)
+        read(1, stage, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        SRX_MULTIPLY(0, 0)
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < FP; ++j) oldX[j] = xs[0][j];
+        read(0, stage, 2);
+        __builtin_amdgcn_sched_barrier(0);
+        prepare();
+        SRX_MULTIPLY(1, 1)
+        __builtin_amdgcn_sched_barrier(0);
+        read(1, stage, 3);
+        __builtin_amdgcn_sched_barrier(0);
+        SRX_MULTIPLY(2, 0)
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < FO; ++i) oldW[i] = ws[i];
+        stage = kStage - stage;
+        if (!WORDS) settle(stage);
+        // after this the next chunk is there, and this one is in registers in every wave: its place is free
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        ++chunk;
+        read(0, stage, 0);
+        readScales(stage);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < FO; ++i)
+#pragma unroll
+            for (int j = 0; j < FP; ++j)
+            {
+                SRX_STEP(3, 1, i, j, oldW, oldX)
+                __builtin_amdgcn_sched_barrier(0);
+                constexpr int kN = FO * FP;
+#pragma unroll
+                for (int k = kLoads * (i * FP + j) / kN; k < kLoads * (i * FP + j + 1) / kN; ++k) load(k, kStage - stage);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        if (!WORDS) loadBytes();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    const int left = a.total - chunk * kChunk;
+    SRX_MULTIPLY(0, 0)
+    if (left > 1)
+    {
+        read(1, stage, 1);
+        SRX_MULTIPLY(1, 1)
+        if (left > 2)
+        {
+            read(0, stage, 2);
+            SRX_MULTIPLY(2, 0)
+            if (left > 3)
+            {
+                read(1, stage, 3);
+                SRX_MULTIPLY(3, 1)
+            }
+        }
+    }
+#undef SRX_MULTIPLY
+#undef SRX_STEP
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    finish<T, FO, FP>(a, acc, dyn + wave * 32 * L::kOutRow, o0, lane, [&](int j, uint8_t*& to, int& count) {
+        to = static_cast<uint8_t*>(a.out) + (((int64_t(n) * a.H + y0 + r0 + j) * a.W + x0) * a.O + o0) * int64_t(sizeof(T));
+        count = y0 + r0 + j < a.H ? min(32, a.W - x0) : 0;
+    });
+}
+
+// hipErrorInvalidConfiguration, and no launch, where the window does not fit half a CU's LDS, where the tiles at the images' edges
+// are a quarter empty, or where there are too few (96 -> 96 channels, 3x3, 200x200, 175 tiles: 9.9 instead of 11.9 us;
+// 180x180, 138: 9.6 instead of 8.3).
+template <typename T, int FO>
+hipError_t launchTaps(const ConvMxArgs& args, hipStream_t s)
+{
+    using L = TapsLds<T, FO>;
+    ConvMxArgs a = args;
+    TapsArgs w{};
+    const int winH = kWinH + a.taps / a.kw - 1;
+    if ((int64_t(winH) * a.W + a.kw + kWinW) * a.blocks * kMxBytes >= int64_t(kRange)) return hipErrorInvalidConfiguration;
+    w.tilesX = (a.W + kWinW - 1) / kWinW;
+    w.tilesY = (a.H + kWinH - 1) / kWinH;
+    a.tilesO = (a.O + L::kBO - 1) / L::kBO;
+    a.tilesP = a.pixels / (a.H * a.W) * w.tilesX * w.tilesY;
+    if (int64_t(a.tilesP) * a.tilesO < 160 || int64_t(a.tilesP) * (kWinW * kWinH * 4) > int64_t(a.pixels) * 5) return hipErrorInvalidConfiguration;
+    const bool words = a.blocks % 4 == 0 && scalesInWords(a);
+    w.winW = kWinW + a.kw - 1;
+    w.winPixels = winH * w.winW;
+    const int units = w.winPixels * a.blocks;
+    w.scales = (units + 63) / 64 * 1024;
+    const int lds = L::bytes(w.scales + (words ? (units / 4 + 63) / 64 * 256 : units)), most = 80 << 10;
+    if (units > kTapsLoads * kThreads || lds > most) return hipErrorInvalidConfiguration;
+    w.down = a.blocks == 8 ? 1 : a.blocks == 4 ? 2 : 3;
+    w.mask = a.blocks == 8 ? 7 : a.blocks == 4 ? 3 : a.blocks % 2 ? 0 : 1;
+    w.byTilesX = Divider(unsigned(w.tilesX));
+    w.byTilesY = Divider(unsigned(w.tilesY));
+    w.byWinW = Divider(unsigned(w.winW));
+    a.byTilesO = Divider(unsigned(a.tilesO));
+    const int64_t grid = int64_t(a.tilesO) * ((int64_t(a.tilesP) + 7) / 8 * 8);
+    if (grid > INT32_MAX) return hipErrorInvalidConfiguration;
+    const auto launchAs = [&](auto kernel) {
+        const hipError_t e = dev::ensureDynamicLds(reinterpret_cast<const void*>(kernel), most);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL(kernel, gridOf(grid), dim3(kThreads), lds, s, a, w);
+        return hipGetLastError();
+    };
+    return words ? launchAs(ConvMxTapsKernel<T, FO, true>) : launchAs(ConvMxTapsKernel<T, FO, false>);
+}
+template <int FO>
+hipError_t launchTaps(bool half, const ConvMxArgs& a, hipStream_t s)
+{
+    return half ? launchTaps<f16, FO>(a, s) : launchTaps<float, FO>(a, s);
+}
+
 template <typename T, int THREADS, int BO, int BP, int FO, int FP>
 hipError_t launch(const ConvMxArgs& args, hipStream_t s)
 {
@@ -903,23 +1230,37 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
     const int rows = tiles(16, 64) >= 256 ? 4 : tiles(16, 32) >= 256 ? 2 : 1;
     if (tiles(16, 16 * rows) * (1 + rows) < 1560 && tapsInRange(a))
         return rows == 4 ? launchRows<4>(half, a, s) : rows == 2 ? launchRows<2>(half, a, s) : launchRows<1>(half, a, s);
+    const auto padded = [&](int64_t o) { return (a.O + o - 1) / o * o; };
     // Up to 64 channels on large images: the window kernel.  64 -> 64 channels, 3x3: 90 instead of 162 us for 1920x1080
     // (codes of all bit patterns; 74 - 78 for those of a normalised layer), 15 instead of 22 for 640x360 (900 tiles), 7.3
     // and 7.4 for 320x180 (240); 1x1, 1920x1080: 65 instead of 88.  32 -> 128, 3x3, 512x512: 18 instead of 26; with more
     // channel tiles the window is read as often as the tiles read it (64 -> 256, 3x3, 256x256: 14.7 and 15.9).  fp32 results
     // leave room for 32 channels at a time only (960x540: 33 instead of 46).
-    if (a.blocks <= 2 && a.O <= 128 && a.W >= kWinW && a.H >= kWinH && tiles(64, 256) >= 768)
+    if (a.blocks <= 2 && a.O <= 128 && (a.taps == 1 || padded(64) <= padded(96)) && a.W >= kWinW && a.H >= kWinH && tiles(64, 256) >= 768)
     {
         const hipError_t e = !half ? launchWindow<float, 1>(a, s) : a.O <= 32 ? launchWindow<f16, 1>(a, s) : launchWindow<f16, 2>(a, s);
         if (e != hipErrorInvalidConfiguration) return e;
     }
+    // Several taps, up to 256 channels: the window staged once (launchTaps refuses where tiles are few or empty), with the tile that
+    // computes least beyond what is needed; a tile of 96 channels takes a tenth longer for a channel than one of 128, one of 64 a
+    // quarter.  3x3, with tiles that read every pixel for every tap: 96 -> 96, 960x540: 47 instead of 75 us; 128 -> 128, 512x512: 33
+    // instead of 42; 96 -> 64: 19 instead of 27; 96 -> 32: 14.6 instead of 20.8; 160 -> 160, 256x256: 19.8 instead of 22.7; 256 ->
+    // 256: 27.5 instead of 28.8; 64 -> 96, 512x512: 21 instead of 25 with the window kernel.
+    if (a.taps > 1 && a.blocks <= kChunk)
+    {
+        const int64_t by128 = padded(128) * 20, by96 = padded(96) * 22, by64 = padded(64) * 25;
+        const hipError_t e = a.O <= 32                          ? launchTaps<1>(half, a, s)
+                             : by128 <= by96 && by128 <= by64 ? launchTaps<4>(half, a, s)
+                             : by96 <= by64                     ? launchTaps<3>(half, a, s)
+                                                                : launchTaps<2>(half, a, s);
+        if (e != hipErrorInvalidConfiguration) return e;
+    }
     // The largest tile that leaves no CU without one: 256x256 reads a quarter of what 64x64 does (512 -> 512 channels, 3x3,
     // 256x256: 95 instead of 164 us), but 64 such tiles for 2048 -> 2048 channels, 1x1, 2048 pixels take 19 instead of 12.
-    // 128x128: 12.7 instead of 14.5 us with 128x64 for 96 -> 96, 3x3, 256x256; 8.7 instead of 8.1 for half as many pixels
-    // (256 tiles).  32x128: 19 instead of 24 with 64x64 for 96 -> 32, 3x3, 512x512.
-    // Channels that only fill up a tile count: 160 -> 160, 3x3, 256x256 in 256: 22.5 instead of 27.5 us, but 8 -> 416, 1x7,
+    // 128x128: 25.8 instead of 30.8 us with 128x64 for 288 -> 96, 3x3, 256x256; 16.3 instead of 15.7 for half as many pixels
+    // (256 tiles).  32x128: 42 instead of 54 with 64x64 for 288 -> 32, 3x3, 512x512.
+    // Channels that only fill up a tile count: 288 -> 160, 3x3, 256x256 in 256: 32 instead of 40 us, but 8 -> 416, 1x7, one row of
     // 100500 pixels in 512: 34 instead of 24 (nothing but the output takes time there).
-    const auto padded = [&](int64_t o) { return (a.O + o - 1) / o * o; };
     const bool deep = a.total > 2 * kChunk;
     if (a.O > 128 && tiles(256, 256) >= 256 && padded(256) * 10 <= padded(64) * (deep ? 14 : 10)) return launch<512, 256, 256, 4, 2>(half, a, s);
     if (a.O > 64 && padded(128) * 10 <= padded(64) * (deep ? 14 : 10))

@@ -502,6 +502,47 @@ def test_conv_of_large_images(dtype, n, c, h, w, o, kh, kw):
     assert (ok | ref.isnan()).all()
 
 
+TAPS = [(1, 96, 200, 215, 96, 3, 3), (1, 128, 203, 211, 128, 3, 3), (2, 256, 130, 160, 65, 3, 3), (1, 224, 250, 190, 33, 2, 3),
+        (1, 75, 230, 215, 30, 5, 2), (1, 130, 215, 220, 100, 1, 7), (1, 170, 127, 190, 230, 3, 3), (1, 50, 215, 210, 90, 5, 5),
+        (3, 7, 125, 127, 75, 7, 1), (1, 160, 8, 6000, 70, 2, 2), (1, 128, 1500, 33, 200, 4, 1), (1, 128, 900, 64, 60, 7, 7),
+        (1, 250, 310, 190, 2, 3, 3), (5, 96, 91, 91, 85, 3, 3)]
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("n,c,h,w,o,kh,kw", TAPS)
+def test_conv_of_several_taps(dtype, n, c, h, w, o, kh, kw):
+    """Up to 256 channels, windows with several taps: every number of blocks and channels of a tile, with NaN in the first and in the
+    last block of a pixel."""
+    x, f = rnd((n * h * w, c), c + o), rnd((o * kh * kw, c), c * o + 1) / 8
+    x[(n * h * w) // 2, 0] = x[(n * h * w) // 3, c - 1] = x[n * h * w - 1, c // 2] = float("nan")
+    xc, xs = quantise(x, 0)
+    wc, ws = quantise(f, 0)
+    x64 = values64(xc.t, xs.t, c).reshape(n, h, w, c)
+    w64 = values64(wc.t, ws.t, c).reshape(o, kh, kw, c)
+    act = (c + o) % 3
+    bias = rnd((o,), 7, dtype) if act else None
+    ref, size, y = conv64(x64, w64, bias, act)
+    got = convolve(xc, xs, (n, c, h, w), wc, ws, (o, c, kh, kw), bias, act, dtype).cuda().double()
+    assert int(ref.isnan().sum()) > 0 and torch.equal(got.isnan(), ref.isnan())
+    ok = (got - ref).abs() <= step(dtype, ref) + conv_tolerance(size, y, kh * kw * -(-c // 32))
+    assert (ok | ref.isnan()).all()
+
+
+@pytest.mark.parametrize("c,h,w,o,kh,kw", [(128, 203, 211, 128, 3, 3), (256, 150, 190, 200, 3, 2), (128, 310, 190, 20, 3, 3), (64, 450, 450, 64, 3, 3)])
+def test_conv_scales_at_odd_addresses(c, h, w, o, kh, kw):
+    """Scales that cannot be read in words: the same results, bit for bit."""
+    xc, xs = quantise(rnd((h * w, c), 1), 0)
+    wc, ws = quantise(rnd((o * kh * kw, c), 2) / 30, 0)
+    ref = convolve(xc, xs, (1, c, h, w), wc, ws, (o, c, kh, kw), None, 2, 0)
+    b = c // 32
+    for by in (1, 3):
+        ms, mf = Guarded((h * w * b + 4,), torch.uint8), Guarded((o * kh * kw * b + 4,), torch.uint8)
+        ms.t[by:by + h * w * b], mf.t[by:by + o * kh * kw * b] = xs.t.view(-1), ws.t.view(-1)
+        out = Guarded((1, h, w, o), torch.float16)
+        S.layer_conv2d_mx4(0, xc.ptr(), ms.ptr() + by, (1, c, h, w), wc.ptr(), mf.ptr() + by, (o, c, kh, kw), None, 2, out.ptr(), stream())
+        assert torch.equal(out.whole(), ref)
+
+
 @pytest.mark.parametrize("c,h,w,o,kh,kw", [(1 << 20, 2, 1400, 2, 3, 1), (4000, 2, 360000, 8, 3, 1), (64, 2, 15000000, 3, 2, 2)])
 def test_conv_taps_far_apart(c, h, w, o, kh, kw):
     """Rows of pixels so long that a window's taps are more than 2^31 bytes of codes apart."""
