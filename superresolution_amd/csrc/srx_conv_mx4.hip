@@ -13,12 +13,14 @@
 //                       (8.9 MB of filter: 1.5 TB/s).
 //   ConvMxWindowKernel  up to 64 channels on large images; bound by the output's bytes.  64 -> 64 channels, 3x3, 1920x1080:
 //                       74 us (336 MB: 4.5 TB/s; 2.1 PFLOP/s).
-//   ConvMxTapsKernel    several taps, up to 256 channels.  96 -> 96, 3x3, 960x540: 47 us (126 MB, 86 GFLOP: 2.7 TB/s, 1.8 PFLOP/s), bound
-//                       by the start and end of its tiles as much as by the products; 256 -> 256, 256x256: 27 us, 2.8 PFLOP/s.
-//   ConvMxKernel        everything else.  512 -> 512 channels, 3x3, 256x256: 80 - 84 us, 3.7 - 3.9 PFLOP/s.  The matrix units
-//                       alone reach 6.2 on such operands held in registers (at the power limit; 7.7 on constants), 5.5 where
-//                       every operand is read from LDS; without its loads from memory this kernel takes 66 of 102 us, without
-//                       its reads from LDS 87: L2, LDS and power together bound it.
+//   ConvMxTapsKernel    several taps.  512 -> 512 channels, 3x3, 256x256: 76 - 81 us, 3.8 - 4.0 PFLOP/s; 256 -> 256: 26, 3.0; 96 -> 96,
+//                       960x540: 47 us (126 MB: 2.7 TB/s; 1.8 PFLOP/s), bound by the start and end of its tiles as much as by the
+//                       products.
+//   ConvMxKernel        everything else.  2048 -> 2048 channels, 1x1, 16384 pixels: 55 us, 2.5 PFLOP/s; 512 -> 512, 65536 pixels:
+//                       24 us (103 MB: 4.3 TB/s).
+// The matrix units alone reach 6.2 PFLOP/s on operands of all bit patterns held in registers (at the power limit; 7.7 on
+// constants), 5.5 where every operand is read from LDS.  Of 102 us that ConvMxKernel takes for 512 -> 512, 3x3, its loads from memory
+// cost 36 and its reads from LDS 15: L2, LDS and power together bound the wide layers.
 #include "srx_mx4.h"
 
 namespace srx {
@@ -203,7 +205,7 @@ __global__ __launch_bounds__(THREADS, 2) void ConvMxKernel(const ConvMxArgs a)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
     // Workgroups are dealt round-robin over the 8 XCDs.  Where there are enough pixel tiles, all channel tiles of the same
     // pixels go to one XCD and share its L2 (512 -> 512 channels, 3x3, 256x256: 95 instead of 98 us; 128 -> 512, 1x1: 18.3
-    // instead of 18.6); pixels are dealt out singly (one long run of them for each XCD: 95, and 12.2 instead of 11.8 for 256 ->
+    // and 18.6); pixels are dealt out singly (one long run of them for each XCD: 95, and 12.2 instead of 11.8 for 256 ->
     // 256, 1x1).
     const unsigned number = blockNumber();
     unsigned tileO, tileP;
@@ -843,17 +845,17 @@ hipError_t launchWindow(const ConvMxArgs& a, hipStream_t s)
     return hipErrorInvalidConfiguration;
 }
 
-// Filters of several taps and up to eight blocks a pixel: a tile's pixels are eight rows of 32, and the window that all its
-// taps see is staged once, so that only the filters come from memory chunk by chunk (ConvMxKernel reads every pixel once for each
-// tap, more than L2 delivers while tiles of 128 channels are multiplied).  A workgroup makes 32 * FO channels, a wave
-// two rows of them.
+// Filters of several taps: a tile's pixels are eight rows of 32, and the window that all its taps see is staged once, eight
+// blocks of each pixel (a part) at a time, so that only the filters come from memory chunk by chunk (ConvMxKernel reads every pixel
+// once for each tap, more than L2 delivers while tiles of 128 channels are multiplied).  A workgroup makes 32 * FO channels, a
+// wave two rows of them; while one workgroup of a CU waits for its window, the others multiply.
 struct TapsArgs
 {
     int winW, winPixels;
     int scales;                       // place of the window's scales behind its codes
-    int down, mask;                   // place of a pixel's block: block ^ (pixel >> down & mask); neighbouring 16 pixels lie in all banks
+    int parts, last;                  // parts of a pixel's blocks, blocks of the last one
     int tilesX, tilesY;
-    Divider byTilesX, byTilesY, byWinW;
+    Divider byTilesX, byTilesY, byWinW, byLast;
 };
 
 template <typename T, int FO>
@@ -867,10 +869,10 @@ struct TapsLds
 
 constexpr int kTapsLoads = 16;        // of a window, at most
 
-// WORDS: four or eight blocks a pixel, whose scales are staged in words; otherwise byte by byte.
-// As many waves a SIMD as the accumulators leave room for (96 -> 96 channels, 960x540: 49 us with three, 53 with two).
-template <typename T, int FO, bool WORDS>
-__global__ __launch_bounds__(kThreads, FO > 3 ? 2 : FO > 2 ? 3 : 4) void ConvMxTapsKernel(const ConvMxArgs a, const TapsArgs w)
+// WORDS: all parts are of four or eight blocks, whose scales are staged in words; otherwise byte by byte.  PARTS: more than one.
+// As many waves a SIMD as the accumulators, and whole windows in LDS (PARTS), leave room for (96 -> 96 channels, 960x540: 49 us with three, 53 with two).
+template <typename T, int FO, bool WORDS, bool PARTS>
+__global__ __launch_bounds__(kThreads, FO > 3 || PARTS ? 2 : FO > 2 ? 3 : 4) void ConvMxTapsKernel(const ConvMxArgs a, const TapsArgs w)
 {
     using L = TapsLds<T, FO>;
     constexpr int kBO = L::kBO, kStage = L::kStage, kScales = kBO * kRow, kWindow = 2 * kStage, FP = 2, kPass = kThreads / 8, kWRows = kBO / kPass;
@@ -884,24 +886,42 @@ __global__ __launch_bounds__(kThreads, FO > 3 ? 2 : FO > 2 ? 3 : 4) void ConvMxT
     const unsigned tileY = w.byTilesX(tileP), n = w.byTilesY(tileY);
     const int x0 = int(tileP - tileY * unsigned(w.tilesX)) * kWinW, y0 = int(tileY - n * unsigned(w.tilesY)) * kWinH;
     const int r0 = 2 * wave;
-    const auto place = [&](unsigned p, unsigned block) { return block ^ ((p >> w.down) & unsigned(w.mask)); };
 
-    // The filters' next chunk of eight blocks; beyond the last, nothing is read.
+    // Of the current part: its blocks, all of them in the reduction, division by its blocks (as Divider), and the place of a
+    // pixel's block: block ^ (pixel >> down & mask), with which neighbouring 16 pixels lie in all banks.
+    int part = 0, blocks, total;
+    unsigned mul, shift, down, mask;
+    const auto begin = [&]() {
+        const bool last = !PARTS || part == w.parts - 1;
+        blocks = last ? w.last : kChunk;
+        total = a.taps * blocks;
+        mul = last ? w.byLast.mul : 1u;
+        shift = last ? w.byLast.shift : 3u;
+        down = blocks == 8 ? 1 : blocks == 4 ? 2 : 3;
+        mask = blocks == 8 ? 7 : blocks == 4 ? 3 : ~unsigned(blocks) & 1u;
+    };
+    const auto byBlocks = [&](unsigned n) { return (__umulhi(n, mul) + n) >> shift; };
+    const auto place = [&](unsigned p, unsigned block) { return block ^ ((p >> down) & mask); };
+
+    // The filters' next chunk of eight blocks of the part; beyond the last, nothing is read.
     const int sr = tid >> 3, sb = (tid & 7) ^ ((sr >> 1) & 7), zr = tid >> 1, zb = (tid & 1) * 4;
     i32x4 wd, vd;
     unsigned wOff[kWRows], off[kWRows], zOff = 0;
     uint8_t wz[kWRows];
 #pragma unroll
-    for (int i = 0; i < kWRows; ++i) wOff[i] = o0 + sr + kPass * i < a.O ? unsigned((sr + kPass * i) * a.total + sb) * kMxBytes : kRange;
-    const unsigned vOff = zr < kBO && o0 + zr < a.O ? unsigned(zr * a.total + zb) : kRange;
+    for (int i = 0; i < kWRows; ++i) wOff[i] = o0 + sr + kPass * i < a.O ? unsigned((sr + kPass * i) * a.total) * kMxBytes : kRange;
+    const unsigned vOff = zr < kBO && o0 + zr < a.O ? unsigned(zr * a.total) : kRange;
     int next = 0;
     const auto prepare = [&]() {
-        wd = descriptor(a.wCodes + (int64_t(o0) * a.total + next) * kMxBytes, kRange);
-        vd = descriptor(a.wScales + int64_t(o0) * a.total + next, WORDS ? kRange : kRange >> 4);
-        const unsigned out = next + sb < a.total ? 0u : kRange;
+        // number kb of the part is number kb + tap * (a pixel's other blocks) of a filter, from the part's first on
+        const int64_t first = int64_t(o0) * a.total + part * kChunk + next;
+        wd = descriptor(a.wCodes + first * kMxBytes, kRange);
+        vd = descriptor(a.wScales + first, WORDS ? kRange : kRange >> 4);
+        const unsigned others = PARTS ? unsigned(a.blocks - blocks) : 0u;
+        const unsigned at = (byBlocks(unsigned(next + sb)) * others + unsigned(sb)) * kMxBytes, out = next + sb < total ? 0u : kRange;
 #pragma unroll
-        for (int i = 0; i < kWRows; ++i) off[i] = wOff[i] | out;
-        zOff = vOff | (next + zb < a.total ? 0u : kRange);
+        for (int i = 0; i < kWRows; ++i) off[i] = (wOff[i] + at) | out;
+        if (WORDS) zOff = (vOff + byBlocks(unsigned(next + zb)) * others + unsigned(zb)) | (next + zb < total ? 0u : kRange);
         next += kChunk;
     };
     constexpr int kLoads = kWRows + (WORDS ? 1 : 0);
@@ -929,9 +949,9 @@ __global__ __launch_bounds__(kThreads, FO > 3 ? 2 : FO > 2 ? 3 : 4) void ConvMxT
 #pragma unroll
         for (int k = 0; k < 2; ++k)
         {
-            const int kb = min(k ? kb1 : kb0, a.total - 1), tap = int(a.byBlocks(unsigned(kb))), ky = int(a.byKw(unsigned(tap)));
+            const int kb = min(k ? kb1 : kb0, total - 1), tap = int(byBlocks(unsigned(kb))), ky = int(a.byKw(unsigned(tap)));
             at[k] = ky * w.winW + tap - ky * a.kw;
-            block[k] = kb - tap * a.blocks;
+            block[k] = kb - tap * blocks;
         }
         b = h ? block[1] : block[0];
         return r0 * w.winW + l + (h ? at[1] : at[0]);
@@ -951,8 +971,8 @@ __global__ __launch_bounds__(kThreads, FO > 3 ? 2 : FO > 2 ? 3 : 4) void ConvMxT
                 for (int j = 0; j < FP; ++j)
                 {
                     const int p = p0 + j * w.winW;
-                    xAt[j] = kWindow + (unsigned(p * a.blocks) + place(unsigned(p), unsigned(b))) * 16;
-                    xs[0][j] = *reinterpret_cast<const unsigned*>(dyn + kWindow + w.scales + p * a.blocks + b);
+                    xAt[j] = kWindow + (unsigned(p * blocks) + place(unsigned(p), unsigned(b))) * 16;
+                    xs[0][j] = *reinterpret_cast<const unsigned*>(dyn + kWindow + w.scales + p * blocks + b);
                 }
             }
 #pragma unroll
@@ -965,8 +985,8 @@ __global__ __launch_bounds__(kThreads, FO > 3 ? 2 : FO > 2 ? 3 : 4) void ConvMxT
             for (int j = 0; j < FP; ++j)
             {
                 const int p = p0 + j * w.winW;
-                xf[set][j] = *reinterpret_cast<const uint4*>(dyn + kWindow + (unsigned(p * a.blocks) + place(unsigned(p), unsigned(b))) * 16);
-                xs[set][j] = dyn[kWindow + w.scales + p * a.blocks + b];
+                xf[set][j] = *reinterpret_cast<const uint4*>(dyn + kWindow + (unsigned(p * blocks) + place(unsigned(p), unsigned(b))) * 16);
+                xs[set][j] = dyn[kWindow + w.scales + p * blocks + b];
             }
         }
     };
@@ -981,134 +1001,145 @@ __global__ __launch_bounds__(kThreads, FO > 3 ? 2 : FO > 2 ? 3 : 4) void ConvMxT
     _Pragma("unroll") for (int i = 0; i < FO; ++i)                                                                     \
         _Pragma("unroll") for (int j = 0; j < FP; ++j) { SRX_STEP(S, SET, i, j, ws, xs[0]) }
 
-    prepare();
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) load(i, 0);
-    if (!WORDS) loadBytes();
-    // the window: codes unit by unit, scales in words or with their codes
+    f32x16 acc[FO][FP];
+    for (;;)
     {
-        const int pixelBytes = a.blocks * kMxBytes;
-        const unsigned rowBytes = unsigned(a.W) * unsigned(pixelBytes);
-        const int64_t first = (int64_t(n) * a.H + y0 - a.padTop) * a.W + x0 - a.padLeft;
-        const i32x4 xd = descriptor(a.codes + first * pixelBytes, kRange), zd = descriptor(a.scales + first * a.blocks, WORDS ? kRange : kRange >> 4);
-        const auto offsetOf = [&](unsigned p) {                         // of a window's pixel, in codes; or kRange
-            const unsigned row = w.byWinW(p), col = p - row * unsigned(w.winW);
-            const bool in = unsigned(y0 - a.padTop + int(row)) < unsigned(a.H) && unsigned(x0 - a.padLeft + int(col)) < unsigned(a.W);
-            return in && p < unsigned(w.winPixels) ? row * rowBytes + col * unsigned(pixelBytes) : kRange;
-        };
-        const int units = w.winPixels * a.blocks;
-        uint8_t z[kTapsLoads];
+        begin();
+        next = chunk = 0;
+        prepare();
 #pragma unroll
-        for (int i = 0; i < kTapsLoads; ++i)
+        for (int i = 0; i < kLoads; ++i) load(i, 0);
+        if (!WORDS) loadBytes();
+        // the window: codes unit by unit, scales in words or with their codes
         {
-            if (i * kThreads + wave * 64 >= units) continue;
-            const unsigned u = i * kThreads + tid, p = a.byBlocks(u), o = offsetOf(p);
-            const unsigned from = o == kRange ? kRange : o + place(p, u - p * unsigned(a.blocks)) * kMxBytes;
-            loadToLds(xd, from, ldsAt + kWindow + (i * kThreads + wave * 64) * 16);
-            if (!WORDS) z[i] = uint8_t(loadByte(zd, from / kMxBytes));
-        }
-        if (WORDS)
-        {
-#pragma unroll
-            for (int i = 0; i < kTapsLoads / 4; ++i)
-            {
-                if (i * kThreads + wave * 64 >= units / 4) continue;
-                const unsigned u = i * kThreads + tid, p = a.blocks == 8 ? u >> 1 : u, o = offsetOf(p);
-                loadWordToLds(zd, o == kRange ? kRange : o / kMxBytes + (a.blocks == 8 ? (u & 1) * 4 : 0), ldsAt + kWindow + w.scales + (i * kThreads + wave * 64) * 4);
-            }
-        }
-        else
-        {
-#pragma unroll
+            const int pixelBytes = a.blocks * kMxBytes;
+            const unsigned rowBytes = unsigned(a.W) * unsigned(pixelBytes);
+            const int64_t first = ((int64_t(n) * a.H + y0 - a.padTop) * a.W + x0 - a.padLeft) * a.blocks + part * kChunk;
+            const i32x4 xd = descriptor(a.codes + first * kMxBytes, kRange), zd = descriptor(a.scales + first, WORDS ? kRange : kRange >> 4);
+            const auto offsetOf = [&](unsigned p) {                     // of a window's pixel, in codes; or kRange
+                const unsigned row = w.byWinW(p), col = p - row * unsigned(w.winW);
+                const bool in = unsigned(y0 - a.padTop + int(row)) < unsigned(a.H) && unsigned(x0 - a.padLeft + int(col)) < unsigned(a.W);
+                return in && p < unsigned(w.winPixels) ? row * rowBytes + col * unsigned(pixelBytes) : kRange;
+            };
+            const int units = w.winPixels * blocks;
+            uint8_t z[kTapsLoads];
+            // (PARTS: the sums are in registers meanwhile)
+#pragma unroll PARTS ? 1 : kTapsLoads
             for (int i = 0; i < kTapsLoads; ++i)
             {
-                const unsigned u = i * kThreads + tid, p = a.byBlocks(u);
-                if (u < unsigned(units)) dyn[kWindow + w.scales + p * unsigned(a.blocks) + place(p, u - p * unsigned(a.blocks))] = z[i];
+                if (i * kThreads + wave * 64 >= units) continue;
+                const unsigned u = i * kThreads + tid, p = byBlocks(u), o = offsetOf(p);
+                const unsigned from = o == kRange ? kRange : o + place(p, u - p * unsigned(blocks)) * kMxBytes;
+                loadToLds(xd, from, ldsAt + kWindow + (i * kThreads + wave * 64) * 16);
+                if (!WORDS) z[i] = uint8_t(loadByte(zd, from / kMxBytes));
             }
-            settle(0);
+            if (WORDS)
+            {
+#pragma unroll PARTS ? 1 : kTapsLoads / 4
+                for (int i = 0; i < kTapsLoads / 4; ++i)
+                {
+                    if (i * kThreads + wave * 64 >= units / 4) continue;
+                    const unsigned u = i * kThreads + tid, p = blocks == 8 ? u >> 1 : u, o = offsetOf(p);
+                    loadWordToLds(zd, o == kRange ? kRange : o / kMxBytes + (blocks == 8 ? (u & 1) * 4 : 0), ldsAt + kWindow + w.scales + (i * kThreads + wave * 64) * 4);
+                }
+            }
+            else
+            {
+#pragma unroll
+                for (int i = 0; i < kTapsLoads; ++i)
+                {
+                    const unsigned u = i * kThreads + tid, p = byBlocks(u);
+                    if (u < unsigned(units)) dyn[kWindow + w.scales + p * unsigned(blocks) + place(p, u - p * unsigned(blocks))] = z[i];
+                }
+                settle(0);
+            }
         }
-    }
-    float* const bias = reinterpret_cast<float*>(dyn + kStage);
-    if (tid < kBO) bias[tid] = a.bias && o0 + tid < a.O ? (float)static_cast<const T*>(a.bias)[o0 + tid] : 0.0f;
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    f32x16 acc[FO][FP];
-    startAt<FO, FP>(acc, bias, h);
-    read(0, 0, 0);
-    readScales(0);
-    // the bias has been read by every wave: its place is the second chunk's
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const int chunks = (a.total + kChunk - 1) / kChunk;
-    if (chunks > 1)
-    {
-        prepare();
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) load(i, kStage);
-        if (!WORDS) loadBytes();
-    }
-    int stage = 0;
-    for (int c = 1; c < chunks; ++c)
-    {
-        // (no branch in here: the compiler would move the products behind it)
-        read(1, stage, 1);
-        __builtin_amdgcn_sched_barrier(0);
-        SRX_MULTIPLY(0, 0)
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int j = 0; j < FP; ++j) oldX[j] = xs[0][j];
-        read(0, stage, 2);
-        __builtin_amdgcn_sched_barrier(0);
-        prepare();
-        SRX_MULTIPLY(1, 1)
-        __builtin_amdgcn_sched_barrier(0);
-        read(1, stage, 3);
-        __builtin_amdgcn_sched_barrier(0);
-        SRX_MULTIPLY(2, 0)
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < FO; ++i) oldW[i] = ws[i];
-        stage = kStage - stage;
-        if (!WORDS) settle(stage);
-        // after this the next chunk is there, and this one is in registers in every wave: its place is free
+        float* const bias = reinterpret_cast<float*>(dyn + kStage);
+        if ((!PARTS || part == 0) && tid < kBO) bias[tid] = a.bias && o0 + tid < a.O ? (float)static_cast<const T*>(a.bias)[o0 + tid] : 0.0f;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        ++chunk;
-        read(0, stage, 0);
-        readScales(stage);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < FO; ++i)
-#pragma unroll
-            for (int j = 0; j < FP; ++j)
-            {
-                SRX_STEP(3, 1, i, j, oldW, oldX)
-                __builtin_amdgcn_sched_barrier(0);
-                constexpr int kN = FO * FP;
-#pragma unroll
-                for (int k = kLoads * (i * FP + j) / kN; k < kLoads * (i * FP + j + 1) / kN; ++k) load(k, kStage - stage);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        if (!WORDS) loadBytes();
-        __builtin_amdgcn_sched_barrier(0);
-    }
-    const int left = a.total - chunk * kChunk;
-    SRX_MULTIPLY(0, 0)
-    if (left > 1)
-    {
-        read(1, stage, 1);
-        SRX_MULTIPLY(1, 1)
-        if (left > 2)
+        if (!PARTS || part == 0)
         {
+            startAt<FO, FP>(acc, bias, h);
+            // the bias has been read by every wave: its place is the second chunk's
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        }
+        read(0, 0, 0);
+        readScales(0);
+        const int chunks = (total + kChunk - 1) / kChunk;
+        if (chunks > 1)
+        {
+            prepare();
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) load(i, kStage);
+            if (!WORDS) loadBytes();
+        }
+        int stage = 0;
+        for (int c = 1; c < chunks; ++c)
+        {
+            // (no branch in here: the compiler would move the products behind it)
+            read(1, stage, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            SRX_MULTIPLY(0, 0)
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < FP; ++j) oldX[j] = xs[0][j];
             read(0, stage, 2);
+            __builtin_amdgcn_sched_barrier(0);
+            prepare();
+            SRX_MULTIPLY(1, 1)
+            __builtin_amdgcn_sched_barrier(0);
+            read(1, stage, 3);
+            __builtin_amdgcn_sched_barrier(0);
             SRX_MULTIPLY(2, 0)
-            if (left > 3)
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < FO; ++i) oldW[i] = ws[i];
+            stage = kStage - stage;
+            if (!WORDS) settle(stage);
+            // after this the next chunk is there, and this one is in registers in every wave: its place is free
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            ++chunk;
+            read(0, stage, 0);
+            readScales(stage);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < FO; ++i)
+#pragma unroll
+                for (int j = 0; j < FP; ++j)
+                {
+                    SRX_STEP(3, 1, i, j, oldW, oldX)
+                    __builtin_amdgcn_sched_barrier(0);
+                    constexpr int kN = FO * FP;
+#pragma unroll
+                    for (int k = kLoads * (i * FP + j) / kN; k < kLoads * (i * FP + j + 1) / kN; ++k) load(k, kStage - stage);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            if (!WORDS) loadBytes();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const int left = total - chunk * kChunk;
+        SRX_MULTIPLY(0, 0)
+        if (left > 1)
+        {
+            read(1, stage, 1);
+            SRX_MULTIPLY(1, 1)
+            if (left > 2)
             {
-                read(1, stage, 3);
-                SRX_MULTIPLY(3, 1)
+                read(0, stage, 2);
+                SRX_MULTIPLY(2, 0)
+                if (left > 3)
+                {
+                    read(1, stage, 3);
+                    SRX_MULTIPLY(3, 1)
+                }
             }
         }
+        // every wave has read this part's window and filters (and the loads behind the last chunk have written their zeros)
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (!PARTS || ++part == w.parts) break;
     }
 #undef SRX_MULTIPLY
 #undef SRX_STEP
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     finish<T, FO, FP>(a, acc, dyn + wave * 32 * L::kOutRow, o0, lane, [&](int j, uint8_t*& to, int& count) {
         to = static_cast<uint8_t*>(a.out) + (((int64_t(n) * a.H + y0 + r0 + j) * a.W + x0) * a.O + o0) * int64_t(sizeof(T));
         count = y0 + r0 + j < a.H ? min(32, a.W - x0) : 0;
@@ -1131,15 +1162,16 @@ hipError_t launchTaps(const ConvMxArgs& args, hipStream_t s)
     a.tilesO = (a.O + L::kBO - 1) / L::kBO;
     a.tilesP = a.pixels / (a.H * a.W) * w.tilesX * w.tilesY;
     if (int64_t(a.tilesP) * a.tilesO < 160 || int64_t(a.tilesP) * (kWinW * kWinH * 4) > int64_t(a.pixels) * 5) return hipErrorInvalidConfiguration;
-    const bool words = a.blocks % 4 == 0 && scalesInWords(a);
+    const bool words = scalesInWords(a);
+    w.parts = (a.blocks + kChunk - 1) / kChunk;
+    w.last = a.blocks - (w.parts - 1) * kChunk;
     w.winW = kWinW + a.kw - 1;
     w.winPixels = winH * w.winW;
-    const int units = w.winPixels * a.blocks;
+    const int units = w.winPixels * (w.parts > 1 ? kChunk : w.last);
     w.scales = (units + 63) / 64 * 1024;
     const int lds = L::bytes(w.scales + (words ? (units / 4 + 63) / 64 * 256 : units)), most = 80 << 10;
-    if (units > kTapsLoads * kThreads || lds > most) return hipErrorInvalidConfiguration;
-    w.down = a.blocks == 8 ? 1 : a.blocks == 4 ? 2 : 3;
-    w.mask = a.blocks == 8 ? 7 : a.blocks == 4 ? 3 : a.blocks % 2 ? 0 : 1;
+    if (units > kTapsLoads * kThreads || lds > most || (w.parts > 1 && !words)) return hipErrorInvalidConfiguration;
+    w.byLast = Divider(unsigned(w.last));
     w.byTilesX = Divider(unsigned(w.tilesX));
     w.byTilesY = Divider(unsigned(w.tilesY));
     w.byWinW = Divider(unsigned(w.winW));
@@ -1152,7 +1184,8 @@ hipError_t launchTaps(const ConvMxArgs& args, hipStream_t s)
         hipLaunchKernelGGL(kernel, gridOf(grid), dim3(kThreads), lds, s, a, w);
         return hipGetLastError();
     };
-    return words ? launchAs(ConvMxTapsKernel<T, FO, true>) : launchAs(ConvMxTapsKernel<T, FO, false>);
+    if (w.parts > 1) return launchAs(ConvMxTapsKernel<T, FO, true, true>);
+    return words ? launchAs(ConvMxTapsKernel<T, FO, true, false>) : launchAs(ConvMxTapsKernel<T, FO, false, false>);
 }
 template <int FO>
 hipError_t launchTaps(bool half, const ConvMxArgs& a, hipStream_t s)
@@ -1241,12 +1274,12 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
         const hipError_t e = !half ? launchWindow<float, 1>(a, s) : a.O <= 32 ? launchWindow<f16, 1>(a, s) : launchWindow<f16, 2>(a, s);
         if (e != hipErrorInvalidConfiguration) return e;
     }
-    // Several taps, up to 256 channels: the window staged once (launchTaps refuses where tiles are few or empty), with the tile that
-    // computes least beyond what is needed; a tile of 96 channels takes a tenth longer for a channel than one of 128, one of 64 a
-    // quarter.  3x3, with tiles that read every pixel for every tap: 96 -> 96, 960x540: 47 instead of 75 us; 128 -> 128, 512x512: 33
-    // instead of 42; 96 -> 64: 19 instead of 27; 96 -> 32: 14.6 instead of 20.8; 160 -> 160, 256x256: 19.8 instead of 22.7; 256 ->
-    // 256: 27.5 instead of 28.8; 64 -> 96, 512x512: 21 instead of 25 with the window kernel.
-    if (a.taps > 1 && a.blocks <= kChunk)
+    // Several taps: the window staged once (launchTaps refuses where tiles are few or empty), with the tile that computes least
+    // beyond what is needed; a tile of 96 channels takes a tenth longer for a channel than one of 128, one of 64 a quarter.  3x3, with
+    // tiles that read every pixel for every tap: 96 -> 96, 960x540: 47 instead of 75 us; 128 -> 128, 512x512: 33 instead of 42; 96 ->
+    // 64: 19 instead of 27; 96 -> 32: 14 instead of 20.8; 160 -> 160, 256x256: 19.8 instead of 22.7; 384 -> 384: 55 instead of 70;
+    // 512 -> 512: 88 instead of 94; 64 -> 96, 512x512: 21 instead of 25 with the window kernel.
+    if (a.taps > 1)
     {
         const int64_t by128 = padded(128) * 20, by96 = padded(96) * 22, by64 = padded(64) * 25;
         const hipError_t e = a.O <= 32                          ? launchTaps<1>(half, a, s)
@@ -1255,12 +1288,12 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
                                                                 : launchTaps<2>(half, a, s);
         if (e != hipErrorInvalidConfiguration) return e;
     }
-    // The largest tile that leaves no CU without one: 256x256 reads a quarter of what 64x64 does (512 -> 512 channels, 3x3,
-    // 256x256: 95 instead of 164 us), but 64 such tiles for 2048 -> 2048 channels, 1x1, 2048 pixels take 19 instead of 12.
-    // 128x128: 25.8 instead of 30.8 us with 128x64 for 288 -> 96, 3x3, 256x256; 16.3 instead of 15.7 for half as many pixels
-    // (256 tiles).  32x128: 42 instead of 54 with 64x64 for 288 -> 32, 3x3, 512x512.
-    // Channels that only fill up a tile count: 288 -> 160, 3x3, 256x256 in 256: 32 instead of 40 us, but 8 -> 416, 1x7, one row of
-    // 100500 pixels in 512: 34 instead of 24 (nothing but the output takes time there).
+    // The largest tile that leaves no CU without one: 256x256 reads a quarter of what 64x64 does (2048 -> 2048 channels, 1x1,
+    // 16384 pixels: 54 instead of 93 us), but 64 such tiles for 2048 pixels take 19 instead of 12.
+    // 128x128: 13.0 instead of 15.3 us with 128x64 for 1024 -> 96, 1x1, 65536 pixels; 9.5 instead of 8.0 for half as many (256
+    // tiles).  32x128: 27.5 instead of 29.4 with 64x64 for 1024 -> 32, 1x1, 262144 pixels; 42 instead of 54 for 288 -> 32, 3x3.
+    // Channels that only fill up a tile count: 1024 -> 160, 1x1, 65536 pixels in 256: 18.7 instead of 22 us, but 8 -> 416, 1x7, one
+    // row of 100500 pixels in 512: 34 instead of 24 (nothing but the output takes time there).
     const bool deep = a.total > 2 * kChunk;
     if (a.O > 128 && tiles(256, 256) >= 256 && padded(256) * 10 <= padded(64) * (deep ? 14 : 10)) return launch<512, 256, 256, 4, 2>(half, a, s);
     if (a.O > 64 && padded(128) * 10 <= padded(64) * (deep ? 14 : 10))

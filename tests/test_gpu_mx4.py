@@ -505,14 +505,15 @@ def test_conv_of_large_images(dtype, n, c, h, w, o, kh, kw):
 TAPS = [(1, 96, 200, 215, 96, 3, 3), (1, 128, 203, 211, 128, 3, 3), (2, 256, 130, 160, 65, 3, 3), (1, 224, 250, 190, 33, 2, 3),
         (1, 75, 230, 215, 30, 5, 2), (1, 130, 215, 220, 100, 1, 7), (1, 170, 127, 190, 230, 3, 3), (1, 50, 215, 210, 90, 5, 5),
         (3, 7, 125, 127, 75, 7, 1), (1, 160, 8, 6000, 70, 2, 2), (1, 128, 1500, 33, 200, 4, 1), (1, 128, 900, 64, 60, 7, 7),
-        (1, 250, 310, 190, 2, 3, 3), (5, 96, 91, 91, 85, 3, 3)]
+        (1, 250, 310, 190, 2, 3, 3), (5, 96, 91, 91, 85, 3, 3), (1, 512, 170, 160, 256, 3, 3),
+        (1, 380, 210, 213, 90, 2, 2), (1, 640, 250, 190, 20, 1, 5), (2, 290, 130, 160, 60, 3, 3), (1, 1024, 160, 256, 128, 3, 2)]
 
 
 @pytest.mark.parametrize("dtype", [0, 1])
 @pytest.mark.parametrize("n,c,h,w,o,kh,kw", TAPS)
 def test_conv_of_several_taps(dtype, n, c, h, w, o, kh, kw):
-    """Up to 256 channels, windows with several taps: every number of blocks and channels of a tile, with NaN in the first and in the
-    last block of a pixel."""
+    """Windows with several taps: every number of blocks and channels of a tile, channels in one part and in several, with NaN in the
+    first and in the last block of a pixel."""
     x, f = rnd((n * h * w, c), c + o), rnd((o * kh * kw, c), c * o + 1) / 8
     x[(n * h * w) // 2, 0] = x[(n * h * w) // 3, c - 1] = x[n * h * w - 1, c // 2] = float("nan")
     xc, xs = quantise(x, 0)
