@@ -1022,16 +1022,31 @@ __global__ __launch_bounds__(kThreads, FO > 3 || PARTS ? 2 : FO > 2 ? 3 : 4) voi
                 return in && p < unsigned(w.winPixels) ? row * rowBytes + col * unsigned(pixelBytes) : kRange;
             };
             const int units = w.winPixels * blocks;
-            uint8_t z[kTapsLoads];
-            // (PARTS: the sums are in registers meanwhile)
-#pragma unroll PARTS ? 1 : kTapsLoads
-            for (int i = 0; i < kTapsLoads; ++i)
+            // all loads first, or (PARTS: the sums are in registers meanwhile) four at a time
+            constexpr int kBatch = PARTS ? 4 : kTapsLoads;
+            uint8_t z[kBatch];
+#pragma unroll 1
+            for (int from = 0; from < kTapsLoads && from * kThreads < units; from += kBatch)
             {
-                if (i * kThreads + wave * 64 >= units) continue;
-                const unsigned u = i * kThreads + tid, p = byBlocks(u), o = offsetOf(p);
-                const unsigned from = o == kRange ? kRange : o + place(p, u - p * unsigned(blocks)) * kMxBytes;
-                loadToLds(xd, from, ldsAt + kWindow + (i * kThreads + wave * 64) * 16);
-                if (!WORDS) z[i] = uint8_t(loadByte(zd, from / kMxBytes));
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i)
+                {
+                    const int at = (from + i) * kThreads;
+                    if (at + wave * 64 >= units) continue;
+                    const unsigned u = at + tid, p = byBlocks(u), o = offsetOf(p);
+                    const unsigned off = o == kRange ? kRange : o + place(p, u - p * unsigned(blocks)) * kMxBytes;
+                    loadToLds(xd, off, ldsAt + kWindow + (at + wave * 64) * 16);
+                    if (!WORDS) z[i] = uint8_t(loadByte(zd, off / kMxBytes));
+                }
+                if (!WORDS)
+                {
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i)
+                    {
+                        const unsigned u = (from + i) * kThreads + tid, p = byBlocks(u);
+                        if (u < unsigned(units)) dyn[kWindow + w.scales + p * unsigned(blocks) + place(p, u - p * unsigned(blocks))] = z[i];
+                    }
+                }
             }
             if (WORDS)
             {
@@ -1043,16 +1058,7 @@ __global__ __launch_bounds__(kThreads, FO > 3 || PARTS ? 2 : FO > 2 ? 3 : 4) voi
                     loadWordToLds(zd, o == kRange ? kRange : o / kMxBytes + (blocks == 8 ? (u & 1) * 4 : 0), ldsAt + kWindow + w.scales + (i * kThreads + wave * 64) * 4);
                 }
             }
-            else
-            {
-#pragma unroll
-                for (int i = 0; i < kTapsLoads; ++i)
-                {
-                    const unsigned u = i * kThreads + tid, p = byBlocks(u);
-                    if (u < unsigned(units)) dyn[kWindow + w.scales + p * unsigned(blocks) + place(p, u - p * unsigned(blocks))] = z[i];
-                }
-                settle(0);
-            }
+            else settle(0);
         }
         float* const bias = reinterpret_cast<float*>(dyn + kStage);
         if ((!PARTS || part == 0) && tid < kBO) bias[tid] = a.bias && o0 + tid < a.O ? (float)static_cast<const T*>(a.bias)[o0 + tid] : 0.0f;
@@ -1170,7 +1176,7 @@ hipError_t launchTaps(const ConvMxArgs& args, hipStream_t s)
     const int units = w.winPixels * (w.parts > 1 ? kChunk : w.last);
     w.scales = (units + 63) / 64 * 1024;
     const int lds = L::bytes(w.scales + (words ? (units / 4 + 63) / 64 * 256 : units)), most = 80 << 10;
-    if (units > kTapsLoads * kThreads || lds > most || (w.parts > 1 && !words)) return hipErrorInvalidConfiguration;
+    if (units > kTapsLoads * kThreads || lds > most) return hipErrorInvalidConfiguration;
     w.byLast = Divider(unsigned(w.last));
     w.byTilesX = Divider(unsigned(w.tilesX));
     w.byTilesY = Divider(unsigned(w.tilesY));
@@ -1184,7 +1190,7 @@ hipError_t launchTaps(const ConvMxArgs& args, hipStream_t s)
         hipLaunchKernelGGL(kernel, gridOf(grid), dim3(kThreads), lds, s, a, w);
         return hipGetLastError();
     };
-    if (w.parts > 1) return launchAs(ConvMxTapsKernel<T, FO, true, true>);
+    if (w.parts > 1) return words ? launchAs(ConvMxTapsKernel<T, FO, true, true>) : launchAs(ConvMxTapsKernel<T, FO, false, true>);
     return words ? launchAs(ConvMxTapsKernel<T, FO, true, false>) : launchAs(ConvMxTapsKernel<T, FO, false, false>);
 }
 template <int FO>
