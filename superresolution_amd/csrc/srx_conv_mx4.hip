@@ -1281,13 +1281,16 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
         if (e != hipErrorInvalidConfiguration) return e;
     }
     // Several taps: the window staged once (launchTaps refuses where tiles are few or empty), with the tile that computes least
-    // beyond what is needed; a tile of 96 channels takes a tenth longer for a channel than one of 128, one of 64 a quarter.  3x3, with
-    // tiles that read every pixel for every tap: 96 -> 96, 960x540: 47 instead of 75 us; 128 -> 128, 512x512: 33 instead of 42; 96 ->
-    // 64: 19 instead of 27; 96 -> 32: 14 instead of 20.8; 160 -> 160, 256x256: 19.8 instead of 22.7; 384 -> 384: 55 instead of 70;
-    // 512 -> 512: 88 instead of 94; 64 -> 96, 512x512: 21 instead of 25 with the window kernel.
+    // beyond what is needed; a tile of 96 channels takes a twentieth longer for a channel than one of 128, one of 64 a quarter, but
+    // in short reductions, where the output takes the time, the smaller ones win (32 -> 384, 3x3, 512x512: 44 instead of 49 us;
+    // 32 -> 300: 43 instead of 52).  3x3, with tiles that read every pixel for every tap: 96 -> 96, 960x540: 47 instead of 75 us;
+    // 128 -> 128, 512x512: 33 instead of 42; 96 -> 64: 19 instead of 27; 96 -> 32: 14 instead of 20.8; 160 -> 160, 256x256: 19.8
+    // instead of 22.7; 384 -> 384: 55 instead of 70; 512 -> 512: 88 instead of 94; 64 -> 96, 512x512: 21 instead of 25 with the
+    // window kernel.
     if (a.taps > 1)
     {
-        const int64_t by128 = padded(128) * 20, by96 = padded(96) * 22, by64 = padded(64) * 25;
+        const bool brief = a.total <= 2 * kChunk;
+        const int64_t by128 = padded(128) * 20, by96 = padded(96) * (brief ? 19 : 21), by64 = padded(64) * (brief ? 18 : 25);
         const hipError_t e = a.O <= 32                          ? launchTaps<1>(half, a, s)
                              : by128 <= by96 && by128 <= by64 ? launchTaps<4>(half, a, s)
                              : by96 <= by64                     ? launchTaps<3>(half, a, s)

@@ -506,7 +506,8 @@ TAPS = [(1, 96, 200, 215, 96, 3, 3), (1, 128, 203, 211, 128, 3, 3), (2, 256, 130
         (1, 75, 230, 215, 30, 5, 2), (1, 130, 215, 220, 100, 1, 7), (1, 170, 127, 190, 230, 3, 3), (1, 50, 215, 210, 90, 5, 5),
         (3, 7, 125, 127, 75, 7, 1), (1, 160, 8, 6000, 70, 2, 2), (1, 128, 1500, 33, 200, 4, 1), (1, 128, 900, 64, 60, 7, 7),
         (1, 250, 310, 190, 2, 3, 3), (5, 96, 91, 91, 85, 3, 3), (1, 512, 170, 160, 256, 3, 3),
-        (1, 380, 210, 213, 90, 2, 2), (1, 640, 250, 190, 20, 1, 5), (2, 290, 130, 160, 60, 3, 3), (1, 1024, 160, 256, 128, 3, 2)]
+        (1, 380, 210, 213, 90, 2, 2), (1, 640, 250, 190, 20, 1, 5), (2, 290, 130, 160, 60, 3, 3), (1, 1024, 160, 256, 128, 3, 2), (1, 20, 200, 220, 384, 3, 3),
+        (2, 4, 130, 190, 290, 5, 5), (1, 500, 210, 213, 40, 2, 3)]
 
 
 @pytest.mark.parametrize("dtype", [0, 1])
