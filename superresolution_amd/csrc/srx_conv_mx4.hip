@@ -7,8 +7,9 @@
 // instruction multiplies two blocks: lanes 0-31 hold one of them for 32 rows (or columns), lanes 32-63 the other, 16
 // bytes and one scale byte each, so that the two blocks may come from different taps.  fp32 accumulation.
 //
-// Four kernels, chosen by LaunchConvMx4; times of the kernels themselves, fp16 results (they differ by 5 % between devices,
-// and by as much between operands of all bit patterns and those of a normalised layer: the power limit):
+// Four kernels, chosen by LaunchConvMx4 (ConvMxTapsKernel is in srx_conv_mx4_taps.hip); times of the kernels themselves, fp16
+// results (they differ by 5 % between devices, and by as much between operands of all bit patterns and those of a normalised
+// layer: the power limit):
 //   ConvMxRowsKernel    few pixels; bound by the latency of one trip to memory and of the join.  One row times 4096 x 4096: 6.0 us
 //                       (8.9 MB of filter: 1.5 TB/s).
 //   ConvMxWindowKernel  up to 64 channels on large images; bound by the output's bytes.  64 -> 64 channels, 3x3, 1920x1080:
@@ -21,157 +22,13 @@
 // The matrix units alone reach 6.2 PFLOP/s on operands of all bit patterns held in registers (at the power limit; 7.7 on
 // constants), 5.5 where every operand is read from LDS.  Of 102 us that ConvMxKernel takes for 512 -> 512, 3x3, its loads from memory
 // cost 36 and its reads from LDS 15: L2, LDS and power together bound the wide layers.
-#include "srx_mx4.h"
+#include "srx_conv_mx4.h"
 
 namespace srx {
 
 using namespace dev;
 
 namespace {
-
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
-struct ConvMxArgs
-{
-    const uint8_t *codes, *scales;    // [pixels][blocks][16], [pixels][blocks]
-    const uint8_t *wCodes, *wScales;  // [O][total][16], [O][total]
-    const void* bias;
-    void* out;
-    int pixels, H, W, O, kw, taps, padTop, padLeft;
-    int blocks, total;                // blocks of a pixel, blocks of the whole reduction
-    Divider byW, byH, byBlocks, byKw, byTilesO;
-    int tilesO, tilesP;
-    int activation;
-    int stream;                       // the output passes by the caches
-};
-
-constexpr int kChunk = 8;             // blocks staged at a time: four instructions' worth
-constexpr int kRow = kChunk * kMxBytes;
-
-// Position of block `b` of row `row` in LDS: rows are 128 bytes apart, and the exclusive-or spreads the 16 rows that
-// one pass of a ds_read_b128 covers over all 64 banks.
-__device__ __forceinline__ int slot(int row, int b) { return row * kRow + ((b ^ ((row >> 1) & 7)) << 4); }
-
-__device__ __forceinline__ i32x8 widen(const uint4& v)
-{
-    return i32x8{int(v.x), int(v.y), int(v.z), int(v.w), 0, 0, 0, 0};
-}
-
-// Buffer descriptors of everything from `p` on: offsets below kRange are read, others give zeros.  A lane that has
-// nothing to read takes the offset kRange.  Scales lie at a sixteenth of their codes' offsets.
-constexpr unsigned kRange = 0x80000000u;
-__device__ __forceinline__ i32x4 descriptor(const uint8_t* p, unsigned range)
-{
-    const uint64_t at = reinterpret_cast<uint64_t>(p);
-    return i32x4{int(unsigned(at)), int(unsigned(at >> 32) & 0xffffu), int(range), 0x00027000};
-}
-// 16 bytes a lane from memory to LDS, lane after lane from the address `lds` on, without registers.  The compiler does
-// not count this load: whoever reads the data waits for it (vmcnt) and for the other waves (s_barrier) first.
-__device__ __forceinline__ void loadToLds(i32x4 from, unsigned offset, unsigned lds)
-{
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(from) : "memory");
-}
-// The same with 4 bytes a lane.
-__device__ __forceinline__ void loadWordToLds(i32x4 from, unsigned offset, unsigned lds)
-{
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(from) : "memory");
-}
-__device__ __forceinline__ unsigned loadByte(i32x4 from, unsigned offset)
-{
-    return __builtin_amdgcn_raw_buffer_load_b8(__builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(uint64_t(unsigned(from[0])) | uint64_t(unsigned(from[1])) << 32), 0, from[2], from[3]), offset, 0, 0);
-}
-
-// Every sum starts with its channel's bias.
-template <int FO, int FP>
-__device__ __forceinline__ void startAt(f32x16 (&acc)[FO][FP], const float* bias, int h)
-{
-#pragma unroll
-    for (int i = 0; i < FO; ++i)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-        {
-            const f32x4 b = *reinterpret_cast<const f32x4*>(bias + 32 * i + 8 * g + 4 * h);
-#pragma unroll
-            for (int j = 0; j < FP; ++j)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) acc[i][j][4 * g + k] = b[k];
-        }
-}
-
-// Activation and stores of a wave's 32 * FO channels of 32 * FP pixels.  A lane holds, for its pixel, output channels
-// 8 * (r >> 2) + 4 * h + (r & 3) of every 32; the wave turns 32 pixels at a time in its own part of LDS, so that whole
-// rows of channels are stored.  place(j, to, count): where channel o0 of the first of the j-th 32 pixels goes, and how many
-// of them exist (both the same for all lanes).
-template <typename T, int FO, int FP, int ACT, typename Place>
-__device__ __forceinline__ void finishAs(const ConvMxArgs& a, const f32x16 (&acc)[FO][FP], uint8_t* mine, int o0, int lane, Place&& place)
-{
-    constexpr int kOutRow = 32 * FO * int(sizeof(T)) + 16;
-    constexpr int kN = 16 / int(sizeof(T)), kPerRow = 32 * FO / kN;   // elements of a store, stores of a pixel
-    constexpr bool kEven = 64 % kPerRow == 0;
-    constexpr int kPass = 64 / kPerRow, kStores = kPerRow / 2;        // pixels stored at a time (kEven), times for 32 pixels
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    const int h = lane >> 5, l = lane & 31;
-    int px = lane / kPerRow, part = lane % kPerRow, channels = a.O - o0 - part * kN;   // channels that exist from this lane's first on
-    const unsigned lanes = unsigned(px) * unsigned(a.O) * unsigned(sizeof(T)) + part * 16, pass = unsigned(kPass) * unsigned(a.O) * unsigned(sizeof(T));
-#pragma unroll
-    for (int j = 0; j < FP; ++j)
-    {
-#pragma unroll
-        for (int i = 0; i < FO; ++i)
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-            {
-                const int o = 32 * i + 8 * g + 4 * h;
-                T4 v4;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v4[k] = (T)(ACT == 1 ? acc[i][j][4 * g + k] : activate(acc[i][j][4 * g + k], ACT));
-                if (ACT == 1) v4 = __builtin_elementwise_maximum(v4, T4{0, 0, 0, 0});     // rounding keeps the sign: two at a time in fp16
-                *reinterpret_cast<T4*>(mine + l * kOutRow + o * int(sizeof(T))) = v4;
-            }
-        __builtin_amdgcn_wave_barrier();
-        uint8_t* to;
-        int count;
-        place(j, to, count);
-#pragma unroll
-        for (int u = 0; u < kStores; ++u)
-        {
-            if (!kEven)
-            {
-                px = (u * 64 + lane) / kPerRow;
-                part = (u * 64 + lane) % kPerRow;
-                channels = a.O - o0 - part * kN;
-            }
-            const int row = kEven ? u * kPass + px : px;
-            const uint4 v = *reinterpret_cast<const uint4*>(mine + row * kOutRow + part * 16);
-            if (row >= count) continue;
-            uint8_t* dst = to + (kEven ? lanes + u * pass : unsigned(px) * unsigned(a.O) * unsigned(sizeof(T)) + part * 16);
-            if (channels >= kN)
-            {
-                typedef unsigned u32x4_at __attribute__((ext_vector_type(4), aligned(2)));
-                const u32x4_at w = {v.x, v.y, v.z, v.w};
-                if (a.stream) __builtin_nontemporal_store(w, reinterpret_cast<u32x4_at*>(dst));
-                else *reinterpret_cast<u32x4_at*>(dst) = w;
-            }
-            else
-            {
-                T e[kN];
-                __builtin_memcpy(e, &v, 16);
-#pragma unroll
-                for (int k = 0; k < kN; ++k)
-                    if (k < channels) reinterpret_cast<T*>(dst)[k] = e[k];
-            }
-        }
-        __builtin_amdgcn_wave_barrier();
-    }
-}
-template <typename T, int FO, int FP, typename Place>
-__device__ __forceinline__ void finish(const ConvMxArgs& a, const f32x16 (&acc)[FO][FP], uint8_t* mine, int o0, int lane, Place&& place)
-{
-    if (a.activation == 0) finishAs<T, FO, FP, 0>(a, acc, mine, o0, lane, place);
-    else if (a.activation == 1) finishAs<T, FO, FP, 1>(a, acc, mine, o0, lane, place);
-    else finishAs<T, FO, FP, 2>(a, acc, mine, o0, lane, place);
-}
 
 // LDS of a tile: the bias, and one or two chunks (rows of codes, words of scales), later the turn of the results.
 template <typename T, int THREADS, int BO, int BP, int FO>
@@ -601,10 +458,6 @@ bool tapsInRange(const ConvMxArgs& a)
 {
     return ((int64_t(a.taps / a.kw) * a.W + a.kw + 256) * a.blocks + a.total) * kMxBytes < int64_t(kRange);
 }
-bool scalesInWords(const ConvMxArgs& a)
-{
-    return a.blocks % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.scales) | reinterpret_cast<uintptr_t>(a.wScales)) & 3) == 0;
-}
 
 template <typename T, int FP>
 hipError_t launchRows(const ConvMxArgs& args, bool words, hipStream_t s)
@@ -647,7 +500,6 @@ struct WindowArgs
     int tilesX, tilesY, tiles, slots; // tiles of all images; workgroups for each channel tile
     Divider byTilesX, byTilesY, byWinRow;
 };
-constexpr int kWinH = 8, kWinW = 32;  // pixels of a tile
 
 template <typename T, int FO, int NL>
 struct WindowLds
@@ -845,360 +697,6 @@ hipError_t launchWindow(const ConvMxArgs& a, hipStream_t s)
     return hipErrorInvalidConfiguration;
 }
 
-// Filters of several taps: a tile's pixels are eight rows of 32, and the window that all its taps see is staged once, eight
-// blocks of each pixel (a part) at a time, so that only the filters come from memory chunk by chunk (ConvMxKernel reads every pixel
-// once for each tap, more than L2 delivers while tiles of 128 channels are multiplied).  A workgroup makes 32 * FO channels, a
-// wave two rows of them; while one workgroup of a CU waits for its window, the others multiply.
-struct TapsArgs
-{
-    int winW, winPixels;
-    int scales;                       // place of the window's scales behind its codes
-    int parts, last;                  // parts of a pixel's blocks, blocks of the last one
-    int tilesX, tilesY;
-    Divider byTilesX, byTilesY, byWinW, byLast;
-};
-
-template <typename T, int FO>
-struct TapsLds
-{
-    static constexpr int kBO = 32 * FO, kStage = kBO * kRow + kThreads * 4;
-    static constexpr int kOutRow = 32 * FO * int(sizeof(T)) + 16, kOut = kThreads / 64 * 32 * kOutRow;
-    // two chunks of filters (codes, scales; the bias in the second one's place at first) and the window, later the turn of the results
-    static int bytes(int window) { return 2 * kStage + window > kOut ? 2 * kStage + window : kOut; }
-};
-
-constexpr int kTapsLoads = 16;        // of a window, at most
-
-// WORDS: all parts are of four or eight blocks, whose scales are staged in words; otherwise byte by byte.  PARTS: more than one.
-// As many waves a SIMD as the accumulators, and whole windows in LDS (PARTS), leave room for (96 -> 96 channels, 960x540: 49 us with three, 53 with two).
-template <typename T, int FO, bool WORDS, bool PARTS>
-__global__ __launch_bounds__(kThreads, FO > 3 || PARTS ? 2 : FO > 2 ? 3 : 4) void ConvMxTapsKernel(const ConvMxArgs a, const TapsArgs w)
-{
-    using L = TapsLds<T, FO>;
-    constexpr int kBO = L::kBO, kStage = L::kStage, kScales = kBO * kRow, kWindow = 2 * kStage, FP = 2, kPass = kThreads / 8, kWRows = kBO / kPass;
-    extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
-    const unsigned ldsAt = unsigned(uintptr_t((__attribute__((address_space(3))) uint8_t*)dyn));
-    // as in ConvMxKernel
-    const unsigned number = blockNumber(), turn = number >> 3, round = a.byTilesO(turn), tileP = round * 8 + (number & 7);
-    if (tileP >= unsigned(a.tilesP)) return;
-    const int o0 = int(turn - round * unsigned(a.tilesO)) * kBO;
-    const unsigned tileY = w.byTilesX(tileP), n = w.byTilesY(tileY);
-    const int x0 = int(tileP - tileY * unsigned(w.tilesX)) * kWinW, y0 = int(tileY - n * unsigned(w.tilesY)) * kWinH;
-    const int r0 = 2 * wave;
-
-    // Of the current part: its blocks, all of them in the reduction, division by its blocks (as Divider), and the place of a
-    // pixel's block: block ^ (pixel >> down & mask), with which neighbouring 16 pixels lie in all banks.
-    int part = 0, blocks, total;
-    unsigned mul, shift, down, mask;
-    const auto begin = [&]() {
-        const bool last = !PARTS || part == w.parts - 1;
-        blocks = last ? w.last : kChunk;
-        total = a.taps * blocks;
-        mul = last ? w.byLast.mul : 1u;
-        shift = last ? w.byLast.shift : 3u;
-        down = blocks == 8 ? 1 : blocks == 4 ? 2 : 3;
-        mask = blocks == 8 ? 7 : blocks == 4 ? 3 : ~unsigned(blocks) & 1u;
-    };
-    const auto byBlocks = [&](unsigned n) { return (__umulhi(n, mul) + n) >> shift; };
-    const auto place = [&](unsigned p, unsigned block) { return block ^ ((p >> down) & mask); };
-
-    // The filters' next chunk of eight blocks of the part; beyond the last, nothing is read.
-    const int sr = tid >> 3, sb = (tid & 7) ^ ((sr >> 1) & 7), zr = tid >> 1, zb = (tid & 1) * 4;
-    i32x4 wd, vd;
-    unsigned wOff[kWRows], off[kWRows], zOff = 0;
-    uint8_t wz[kWRows];
-#pragma unroll
-    for (int i = 0; i < kWRows; ++i) wOff[i] = o0 + sr + kPass * i < a.O ? unsigned((sr + kPass * i) * a.total) * kMxBytes : kRange;
-    const unsigned vOff = zr < kBO && o0 + zr < a.O ? unsigned(zr * a.total) : kRange;
-    int next = 0;
-    const auto prepare = [&]() {
-        // number kb of the part is number kb + tap * (a pixel's other blocks) of a filter, from the part's first on
-        const int64_t first = int64_t(o0) * a.total + part * kChunk + next;
-        wd = descriptor(a.wCodes + first * kMxBytes, kRange);
-        vd = descriptor(a.wScales + first, WORDS ? kRange : kRange >> 4);
-        const unsigned others = PARTS ? unsigned(a.blocks - blocks) : 0u;
-        const unsigned at = (byBlocks(unsigned(next + sb)) * others + unsigned(sb)) * kMxBytes, out = next + sb < total ? 0u : kRange;
-#pragma unroll
-        for (int i = 0; i < kWRows; ++i) off[i] = (wOff[i] + at) | out;
-        if (WORDS) zOff = (vOff + byBlocks(unsigned(next + zb)) * others + unsigned(zb)) | (next + zb < total ? 0u : kRange);
-        next += kChunk;
-    };
-    constexpr int kLoads = kWRows + (WORDS ? 1 : 0);
-    const auto load = [&](int i, int stage) {
-        if (i < kWRows) loadToLds(wd, off[i], ldsAt + stage + wave * 1024 + i * kThreads * 16);
-        else loadWordToLds(vd, zOff, ldsAt + stage + kScales + wave * 256);
-    };
-    const auto loadBytes = [&]() {
-#pragma unroll
-        for (int i = 0; i < kWRows; ++i) wz[i] = uint8_t(loadByte(vd, off[i] / kMxBytes));
-    };
-    const auto settle = [&](int stage) {
-#pragma unroll
-        for (int i = 0; i < kWRows; ++i) dyn[stage + kScales + (sr + kPass * i) * kChunk + sb] = wz[i];
-    };
-
-    // Operands of step s of the current chunk: blocks s (lanes 0-31) and 4 + s (lanes 32-63).  Behind the last block the filters
-    // are zeros, and the last block's pixels, which are in the sum anyway, stand in.
-    int chunk = 0;
-    uint4 wf[2][FO], xf[2][FP];
-    unsigned ws[FO], oldW[FO], xs[2][FP], oldX[FP], xAt[FP];
-    // window pixel, counted from the wave's own, that each half of the wave reads for blocks kb0 and kb1; first pixel of a lane
-    const auto pixelOf = [&](int kb0, int kb1, int& b) {
-        int at[2], block[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-        {
-            const int kb = min(k ? kb1 : kb0, total - 1), tap = int(byBlocks(unsigned(kb))), ky = int(a.byKw(unsigned(tap)));
-            at[k] = ky * w.winW + tap - ky * a.kw;
-            block[k] = kb - tap * blocks;
-        }
-        b = h ? block[1] : block[0];
-        return r0 * w.winW + l + (h ? at[1] : at[0]);
-    };
-    const auto read = [&](int set, int stage, int s) {
-#pragma unroll
-        for (int i = 0; i < FO; ++i) wf[set][i] = *reinterpret_cast<const uint4*>(dyn + stage + slot(32 * i + l, 4 * h + s));
-        int b;
-        if (WORDS)
-        {
-            // a lane's four blocks are of one pixel: their places differ in two bits, and their scales are a word
-            if (s == 0)
-            {
-                const int p0 = pixelOf(chunk * kChunk, chunk * kChunk + 4, b);
-                b &= ~3;
-#pragma unroll
-                for (int j = 0; j < FP; ++j)
-                {
-                    const int p = p0 + j * w.winW;
-                    xAt[j] = kWindow + (unsigned(p * blocks) + place(unsigned(p), unsigned(b))) * 16;
-                    xs[0][j] = *reinterpret_cast<const unsigned*>(dyn + kWindow + w.scales + p * blocks + b);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < FP; ++j) xf[set][j] = *reinterpret_cast<const uint4*>(dyn + (xAt[j] ^ unsigned(s * 16)));
-        }
-        else
-        {
-            const int p0 = pixelOf(chunk * kChunk + s, chunk * kChunk + 4 + s, b);
-#pragma unroll
-            for (int j = 0; j < FP; ++j)
-            {
-                const int p = p0 + j * w.winW;
-                xf[set][j] = *reinterpret_cast<const uint4*>(dyn + kWindow + (unsigned(p * blocks) + place(unsigned(p), unsigned(b))) * 16);
-                xs[set][j] = dyn[kWindow + w.scales + p * blocks + b];
-            }
-        }
-    };
-    const auto readScales = [&](int stage) {
-#pragma unroll
-        for (int i = 0; i < FO; ++i) ws[i] = *reinterpret_cast<const unsigned*>(dyn + stage + kScales + (32 * i + l) * kChunk + 4 * h);
-    };
-#define SRX_STEP(S, SET, I, J, WS, XS)                                                                                 \
-    acc[I][J] = WORDS ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(wf[SET][I]), widen(xf[SET][J]), acc[I][J], 4, 4, S, WS[I], S, XS[J])   \
-                      : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(widen(wf[SET][I]), widen(xf[SET][J]), acc[I][J], 4, 4, S, WS[I], 0, xs[SET][J]);
-#define SRX_MULTIPLY(S, SET)                                                                                           \
-    _Pragma("unroll") for (int i = 0; i < FO; ++i)                                                                     \
-        _Pragma("unroll") for (int j = 0; j < FP; ++j) { SRX_STEP(S, SET, i, j, ws, xs[0]) }
-
-    f32x16 acc[FO][FP];
-    for (;;)
-    {
-        begin();
-        next = chunk = 0;
-        prepare();
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) load(i, 0);
-        if (!WORDS) loadBytes();
-        // the window: codes unit by unit, scales in words or with their codes
-        {
-            const int pixelBytes = a.blocks * kMxBytes;
-            const unsigned rowBytes = unsigned(a.W) * unsigned(pixelBytes);
-            const int64_t first = ((int64_t(n) * a.H + y0 - a.padTop) * a.W + x0 - a.padLeft) * a.blocks + part * kChunk;
-            const i32x4 xd = descriptor(a.codes + first * kMxBytes, kRange), zd = descriptor(a.scales + first, WORDS ? kRange : kRange >> 4);
-            const auto offsetOf = [&](unsigned p) {                     // of a window's pixel, in codes; or kRange
-                const unsigned row = w.byWinW(p), col = p - row * unsigned(w.winW);
-                const bool in = unsigned(y0 - a.padTop + int(row)) < unsigned(a.H) && unsigned(x0 - a.padLeft + int(col)) < unsigned(a.W);
-                return in && p < unsigned(w.winPixels) ? row * rowBytes + col * unsigned(pixelBytes) : kRange;
-            };
-            const int units = w.winPixels * blocks;
-            // all loads first, or (PARTS: the sums are in registers meanwhile) four at a time
-            constexpr int kBatch = PARTS ? 4 : kTapsLoads;
-            uint8_t z[kBatch];
-#pragma unroll 1
-            for (int from = 0; from < kTapsLoads && from * kThreads < units; from += kBatch)
-            {
-#pragma unroll
-                for (int i = 0; i < kBatch; ++i)
-                {
-                    const int at = (from + i) * kThreads;
-                    if (at + wave * 64 >= units) continue;
-                    const unsigned u = at + tid, p = byBlocks(u), o = offsetOf(p);
-                    const unsigned off = o == kRange ? kRange : o + place(p, u - p * unsigned(blocks)) * kMxBytes;
-                    loadToLds(xd, off, ldsAt + kWindow + (at + wave * 64) * 16);
-                    if (!WORDS) z[i] = uint8_t(loadByte(zd, off / kMxBytes));
-                }
-                if (!WORDS)
-                {
-#pragma unroll
-                    for (int i = 0; i < kBatch; ++i)
-                    {
-                        const unsigned u = (from + i) * kThreads + tid, p = byBlocks(u);
-                        if (u < unsigned(units)) dyn[kWindow + w.scales + p * unsigned(blocks) + place(p, u - p * unsigned(blocks))] = z[i];
-                    }
-                }
-            }
-            if (WORDS)
-            {
-#pragma unroll PARTS ? 1 : kTapsLoads / 4
-                for (int i = 0; i < kTapsLoads / 4; ++i)
-                {
-                    if (i * kThreads + wave * 64 >= units / 4) continue;
-                    const unsigned u = i * kThreads + tid, p = blocks == 8 ? u >> 1 : u, o = offsetOf(p);
-                    loadWordToLds(zd, o == kRange ? kRange : o / kMxBytes + (blocks == 8 ? (u & 1) * 4 : 0), ldsAt + kWindow + w.scales + (i * kThreads + wave * 64) * 4);
-                }
-            }
-            else settle(0);
-        }
-        float* const bias = reinterpret_cast<float*>(dyn + kStage);
-        if ((!PARTS || part == 0) && tid < kBO) bias[tid] = a.bias && o0 + tid < a.O ? (float)static_cast<const T*>(a.bias)[o0 + tid] : 0.0f;
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (!PARTS || part == 0)
-        {
-            startAt<FO, FP>(acc, bias, h);
-            // the bias has been read by every wave: its place is the second chunk's
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        }
-        read(0, 0, 0);
-        readScales(0);
-        const int chunks = (total + kChunk - 1) / kChunk;
-        if (chunks > 1)
-        {
-            prepare();
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) load(i, kStage);
-            if (!WORDS) loadBytes();
-        }
-        int stage = 0;
-        for (int c = 1; c < chunks; ++c)
-        {
-            // (no branch in here: the compiler would move the products behind it)
-            read(1, stage, 1);
-            __builtin_amdgcn_sched_barrier(0);
-            SRX_MULTIPLY(0, 0)
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int j = 0; j < FP; ++j) oldX[j] = xs[0][j];
-            read(0, stage, 2);
-            __builtin_amdgcn_sched_barrier(0);
-            prepare();
-            SRX_MULTIPLY(1, 1)
-            __builtin_amdgcn_sched_barrier(0);
-            read(1, stage, 3);
-            __builtin_amdgcn_sched_barrier(0);
-            SRX_MULTIPLY(2, 0)
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = 0; i < FO; ++i) oldW[i] = ws[i];
-            stage = kStage - stage;
-            if (!WORDS) settle(stage);
-            // after this the next chunk is there, and this one is in registers in every wave: its place is free
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            ++chunk;
-            read(0, stage, 0);
-            readScales(stage);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = 0; i < FO; ++i)
-#pragma unroll
-                for (int j = 0; j < FP; ++j)
-                {
-                    SRX_STEP(3, 1, i, j, oldW, oldX)
-                    __builtin_amdgcn_sched_barrier(0);
-                    constexpr int kN = FO * FP;
-#pragma unroll
-                    for (int k = kLoads * (i * FP + j) / kN; k < kLoads * (i * FP + j + 1) / kN; ++k) load(k, kStage - stage);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            if (!WORDS) loadBytes();
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        const int left = total - chunk * kChunk;
-        SRX_MULTIPLY(0, 0)
-        if (left > 1)
-        {
-            read(1, stage, 1);
-            SRX_MULTIPLY(1, 1)
-            if (left > 2)
-            {
-                read(0, stage, 2);
-                SRX_MULTIPLY(2, 0)
-                if (left > 3)
-                {
-                    read(1, stage, 3);
-                    SRX_MULTIPLY(3, 1)
-                }
-            }
-        }
-        // every wave has read this part's window and filters (and the loads behind the last chunk have written their zeros)
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (!PARTS || ++part == w.parts) break;
-    }
-#undef SRX_MULTIPLY
-#undef SRX_STEP
-    finish<T, FO, FP>(a, acc, dyn + wave * 32 * L::kOutRow, o0, lane, [&](int j, uint8_t*& to, int& count) {
-        to = static_cast<uint8_t*>(a.out) + (((int64_t(n) * a.H + y0 + r0 + j) * a.W + x0) * a.O + o0) * int64_t(sizeof(T));
-        count = y0 + r0 + j < a.H ? min(32, a.W - x0) : 0;
-    });
-}
-
-// hipErrorInvalidConfiguration, and no launch, where the window does not fit half a CU's LDS, where the tiles at the images' edges
-// are a quarter empty, or where there are too few (96 -> 96 channels, 3x3, 200x200, 175 tiles: 9.9 instead of 11.9 us;
-// 180x180, 138: 9.6 instead of 8.3).
-template <typename T, int FO>
-hipError_t launchTaps(const ConvMxArgs& args, hipStream_t s)
-{
-    using L = TapsLds<T, FO>;
-    ConvMxArgs a = args;
-    TapsArgs w{};
-    const int winH = kWinH + a.taps / a.kw - 1;
-    if ((int64_t(winH) * a.W + a.kw + kWinW) * a.blocks * kMxBytes >= int64_t(kRange)) return hipErrorInvalidConfiguration;
-    w.tilesX = (a.W + kWinW - 1) / kWinW;
-    w.tilesY = (a.H + kWinH - 1) / kWinH;
-    a.tilesO = (a.O + L::kBO - 1) / L::kBO;
-    a.tilesP = a.pixels / (a.H * a.W) * w.tilesX * w.tilesY;
-    if (int64_t(a.tilesP) * a.tilesO < 160 || int64_t(a.tilesP) * (kWinW * kWinH * 4) > int64_t(a.pixels) * 5) return hipErrorInvalidConfiguration;
-    const bool words = scalesInWords(a);
-    w.parts = (a.blocks + kChunk - 1) / kChunk;
-    w.last = a.blocks - (w.parts - 1) * kChunk;
-    w.winW = kWinW + a.kw - 1;
-    w.winPixels = winH * w.winW;
-    const int units = w.winPixels * (w.parts > 1 ? kChunk : w.last);
-    w.scales = (units + 63) / 64 * 1024;
-    const int lds = L::bytes(w.scales + (words ? (units / 4 + 63) / 64 * 256 : units)), most = 80 << 10;
-    if (units > kTapsLoads * kThreads || lds > most) return hipErrorInvalidConfiguration;
-    w.byLast = Divider(unsigned(w.last));
-    w.byTilesX = Divider(unsigned(w.tilesX));
-    w.byTilesY = Divider(unsigned(w.tilesY));
-    w.byWinW = Divider(unsigned(w.winW));
-    a.byTilesO = Divider(unsigned(a.tilesO));
-    const int64_t grid = int64_t(a.tilesO) * ((int64_t(a.tilesP) + 7) / 8 * 8);
-    if (grid > INT32_MAX) return hipErrorInvalidConfiguration;
-    const auto launchAs = [&](auto kernel) {
-        const hipError_t e = dev::ensureDynamicLds(reinterpret_cast<const void*>(kernel), most);
-        if (e != hipSuccess) return e;
-        hipLaunchKernelGGL(kernel, gridOf(grid), dim3(kThreads), lds, s, a, w);
-        return hipGetLastError();
-    };
-    if (w.parts > 1) return words ? launchAs(ConvMxTapsKernel<T, FO, true, true>) : launchAs(ConvMxTapsKernel<T, FO, false, true>);
-    return words ? launchAs(ConvMxTapsKernel<T, FO, true, false>) : launchAs(ConvMxTapsKernel<T, FO, false, false>);
-}
-template <int FO>
-hipError_t launchTaps(bool half, const ConvMxArgs& a, hipStream_t s)
-{
-    return half ? launchTaps<f16, FO>(a, s) : launchTaps<float, FO>(a, s);
-}
-
 template <typename T, int THREADS, int BO, int BP, int FO, int FP>
 hipError_t launch(const ConvMxArgs& args, hipStream_t s)
 {
@@ -1280,7 +778,7 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
         const hipError_t e = !half ? launchWindow<float, 1>(a, s) : a.O <= 32 ? launchWindow<f16, 1>(a, s) : launchWindow<f16, 2>(a, s);
         if (e != hipErrorInvalidConfiguration) return e;
     }
-    // Several taps: the window staged once (launchTaps refuses where tiles are few or empty), with the tile that computes least
+    // Several taps: the window staged once (launchConvMxTaps refuses where tiles are few or empty), with the tile that computes least
     // beyond what is needed; a tile of 96 channels takes a twentieth longer for a channel than one of 128, one of 64 a quarter, but
     // in short reductions, where the output takes the time, the smaller ones win (32 -> 384, 3x3, 512x512: 44 instead of 49 us;
     // 32 -> 300: 43 instead of 52).  3x3, with tiles that read every pixel for every tap: 96 -> 96, 960x540: 47 instead of 75 us;
@@ -1291,10 +789,10 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
     {
         const bool brief = a.total <= 2 * kChunk;
         const int64_t by128 = padded(128) * 20, by96 = padded(96) * (brief ? 19 : 21), by64 = padded(64) * (brief ? 18 : 25);
-        const hipError_t e = a.O <= 32                          ? launchTaps<1>(half, a, s)
-                             : by128 <= by96 && by128 <= by64 ? launchTaps<4>(half, a, s)
-                             : by96 <= by64                     ? launchTaps<3>(half, a, s)
-                                                                : launchTaps<2>(half, a, s);
+        const hipError_t e = a.O <= 32                          ? launchConvMxTaps(half, 32, a, s)
+                             : by128 <= by96 && by128 <= by64 ? launchConvMxTaps(half, 128, a, s)
+                             : by96 <= by64                     ? launchConvMxTaps(half, 96, a, s)
+                                                                : launchConvMxTaps(half, 64, a, s);
         if (e != hipErrorInvalidConfiguration) return e;
     }
     // The largest tile that leaves no CU without one: 256x256 reads a quarter of what 64x64 does (2048 -> 2048 channels, 1x1,
