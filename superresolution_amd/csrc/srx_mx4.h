@@ -29,7 +29,7 @@ inline dim3 gridOf(int64_t blocks)
 {
     return blocks <= int64_t(kGridRow) ? dim3(unsigned(blocks)) : dim3(kGridRow, unsigned((blocks + kGridRow - 1) / kGridRow));
 }
-// Number of this workgroup; those behind the last one of the grid asked for leave at once.
+// Number of this workgroup; a kernel has nothing to do for those behind the last one of the grid asked for.
 __device__ __forceinline__ unsigned blockNumber() { return blockIdx.y * kGridRow + blockIdx.x; }
 
 constexpr int kMxBlock = 32;                          // values that share a scale

@@ -39,7 +39,7 @@ struct NormArgs
     int tileGroups, tiles;            // whole groups per workgroup (statistics, slabs)
     int applyChunks, applyPixels, applyTiles;
     int groupsInAll;                  // N * G
-    int blocks;                       // workgroups of this launch
+    int blocks, first;                // workgroups, number of this launch's first one
     int slabRows;                     // pixels that the threads of a slab hold at a time
     Divider byTiles, byChunks, byGroupC, byVecs;
     float epsilon;
@@ -219,8 +219,7 @@ __global__ __launch_bounds__(THREADS) void NormSlabKernel(const NormArgs a)
     __shared__ __attribute__((aligned(16))) float sPart[THREADS * kVec];
     __shared__ float sTeam[THREADS];
     __shared__ float2 sStat[THREADS * kVec];
-    const unsigned number = blockNumber();
-    if (number >= unsigned(a.blocks)) return;
+    const unsigned number = unsigned(a.first) + blockNumber();
     const int tid = threadIdx.x, n = int(a.byTiles(number)), tile = int(number) - n * a.tiles;
     const int g0 = tile * a.tileGroups, groups = min(a.tileGroups, a.G - g0);
     const int c0 = g0 * a.groupC, tileC = groups * a.groupC;
@@ -351,8 +350,7 @@ template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
 {
     __shared__ __attribute__((aligned(16))) float sMean[kTileC], sM2[kTileC];
-    const unsigned number = blockNumber();
-    if (number >= unsigned(a.blocks)) return;
+    const unsigned number = unsigned(a.first) + blockNumber();
     const int b = int(a.byTiles(number)), tile = int(number) - b * a.tiles;
     const int n = int(a.byChunks(unsigned(b))), chunk = b - n * a.chunks;
     const int g0 = tile * a.tileGroups, groups = min(a.tileGroups, a.G - g0);
@@ -528,8 +526,7 @@ __global__ __launch_bounds__(kThreads) void NormApplyKernel(const NormArgs a)
 {
     __shared__ float2 sStat[kTileC];
     // from the last part to the first: the statistics kernel read the last ones last, so they are still cached
-    const unsigned number = blockNumber();
-    if (number >= unsigned(a.blocks)) return;
+    const unsigned number = unsigned(a.first) + blockNumber();
     const int b0 = a.blocks - 1 - int(number), b = int(a.byTiles(unsigned(b0))), tile = b0 - b * a.tiles;
     const int n = int(a.byChunks(unsigned(b))), chunk = b - n * a.applyChunks;
     const int c0 = tile * kTileC, tileC = min(kTileC, a.C - c0);
@@ -807,21 +804,31 @@ size_t normWorkspace(const NormPlan& p)
     return size_t(p.images) * p.a.G * (p.a.chunks + (p.a.chunks > kJoin ? 1 : 0)) * sizeof(float2);
 }
 
+// f(grid, arguments) for all workgroups: whole rows of them (gridOf), and the rest in a launch of its own.  (One launch whose last
+// workgroups leave at once would have every one of them wait for their number: 0.4 us of kernels of 6.)
+template <typename F>
+hipError_t inGrids(NormArgs a, int64_t blocks, F&& f)
+{
+    const int64_t rows = blocks / kGridRow, rest = blocks % kGridRow;
+    a.blocks = int(blocks);
+    a.first = 0;
+    if (rows > 0) f(dim3(kGridRow, unsigned(rows)), a);
+    a.first = int(rows * kGridRow);
+    if (rest > 0) f(dim3(unsigned(rest)), a);
+    return hipGetLastError();
+}
+
 template <typename T, bool MX4>
 hipError_t launchNorm(const NormPlan& p, hipStream_t s)
 {
     const NormArgs& a = p.a;
     if (p.slabThreads)
-    {
-        NormArgs a = p.a;
-        a.blocks = int(p.images * a.tiles);
-        const dim3 grid = gridOf(a.blocks);
-        if (p.slabThreads == 256 && p.slabHeld == 1) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 256, 1>), grid, dim3(256), 0, s, a);
-        else if (p.slabThreads == 256) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 256, 4>), grid, dim3(256), 0, s, a);
-        else if (p.slabHeld <= 2) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 1024, 2>), grid, dim3(1024), 0, s, a);
-        else hipLaunchKernelGGL((NormSlabKernel<T, MX4, 1024, 4>), grid, dim3(1024), 0, s, a);
-        return hipGetLastError();
-    }
+        return inGrids(a, p.images * a.tiles, [&](dim3 grid, const NormArgs& g) {
+            if (p.slabThreads == 256 && p.slabHeld == 1) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 256, 1>), grid, dim3(256), 0, s, g);
+            else if (p.slabThreads == 256) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 256, 4>), grid, dim3(256), 0, s, g);
+            else if (p.slabHeld <= 2) hipLaunchKernelGGL((NormSlabKernel<T, MX4, 1024, 2>), grid, dim3(1024), 0, s, g);
+            else hipLaunchKernelGGL((NormSlabKernel<T, MX4, 1024, 4>), grid, dim3(1024), 0, s, g);
+        });
     const int64_t statsGrid = p.images * a.chunks * a.tiles, applyGrid = p.images * a.applyChunks * a.applyTiles;
     if (statsGrid > INT32_MAX || applyGrid > INT32_MAX || p.images * a.G > INT32_MAX) return hipErrorInvalidValue;
     const dim3 block(kThreads);
@@ -831,21 +838,21 @@ hipError_t launchNorm(const NormPlan& p, hipStream_t s)
     ap.tiles = a.applyTiles;
     ap.byTiles = Divider(unsigned(a.applyTiles));
     ap.byChunks = Divider(unsigned(a.applyChunks));
-    st.blocks = int(statsGrid);
-    ap.blocks = int(applyGrid);
     const bool whole = a.C % kVec == 0 && (a.tileGroups == a.G || (a.tileGroups * a.groupC) % kVec == 0);
-    if (whole) hipLaunchKernelGGL((NormStatsKernel<T, true>), gridOf(statsGrid), block, 0, s, st);
-    else hipLaunchKernelGGL((NormStatsKernel<T, false>), gridOf(statsGrid), block, 0, s, st);
-    hipError_t e = hipGetLastError();
+    hipError_t e = inGrids(st, statsGrid, [&](dim3 grid, const NormArgs& g) {
+        if (whole) hipLaunchKernelGGL((NormStatsKernel<T, true>), grid, block, 0, s, g);
+        else hipLaunchKernelGGL((NormStatsKernel<T, false>), grid, block, 0, s, g);
+    });
     if (e != hipSuccess) return e;
     if (a.chunks > kJoin)
     {
         hipLaunchKernelGGL(NormJoinKernel, dim3(unsigned(a.groupsInAll)), dim3(64), 0, s, a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    if (a.C % kVec == 0) hipLaunchKernelGGL((NormApplyKernel<T, MX4, true>), gridOf(applyGrid), block, 0, s, ap);
-    else hipLaunchKernelGGL((NormApplyKernel<T, MX4, false>), gridOf(applyGrid), block, 0, s, ap);
-    return hipGetLastError();
+    return inGrids(ap, applyGrid, [&](dim3 grid, const NormArgs& g) {
+        if (a.C % kVec == 0) hipLaunchKernelGGL((NormApplyKernel<T, MX4, true>), grid, block, 0, s, g);
+        else hipLaunchKernelGGL((NormApplyKernel<T, MX4, false>), grid, block, 0, s, g);
+    });
 }
 
 }  // namespace
