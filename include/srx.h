@@ -325,8 +325,9 @@ srx_status srx_layer_add(int32_t dtype, const void* a, const void* b, void* out,
  *     may overlap on different streams as long as their outputs and workspaces are different memory.
  *   - Results do not depend on what runs beside a call: no atomics, fixed orders of summation.
  *   - A call that is refused (SRX_ERR_INVALID) has launched nothing.  Sizes of zero are refused.
- *   - At most 2^20 channels and filters; in srx_layer_group_norm* N * groups is at most 2^31 - 1; in
- *     srx_layer_conv2d_mx4 N*H*W is at most 2^31 - 1 and kh * kw * ceil(C / 32) below 2^19.
+ *   - A tensor holds fewer than 2^40 values (2^38 blocks), in at most 2^20 channels or columns; at most 2^20 filters;
+ *     in srx_layer_group_norm* N * groups is at most 2^31 - 1; in srx_layer_conv2d_mx4 N*H*W is at most 2^31 - 1 and
+ *     kh * kw * ceil(C / 32) below 2^19.
  *
  * Activations: 0 = none, 1 = ReLU, 2 = SiLU, y / (1 + exp(-y)).
  *

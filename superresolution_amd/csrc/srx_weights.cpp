@@ -81,10 +81,12 @@ uint64_t tensorBytes(const uint32_t sizes[4], TensorDataType t)
     return uint64_t(sizes[0]) * sizes[1] * sizes[2] * sizes[3] * (t == TensorDataType::FLOAT16 ? 2 : 4);
 }
 
+// Sizes of a tensor of 1 .. 2^40 - 1 values.  (The product of four sizes may pass 64 bits: each is compared with what is left.)
 bool validSizes(const uint32_t sizes[4])
 {
-    return sizes && sizes[0] && sizes[1] && sizes[2] && sizes[3] &&
-           uint64_t(sizes[0]) * sizes[1] * sizes[2] * sizes[3] < (uint64_t(1) << 40);
+    uint64_t left = (uint64_t(1) << 40) - 1;
+    for (int i = 0; sizes && i < 4 && left; ++i) left = sizes[i] ? left / sizes[i] : 0;
+    return sizes && left;
 }
 
 // Channels of the normalisation and 4-bit layers: their kernels count channels and blocks in 32 bits.
