@@ -320,7 +320,27 @@ _U32x4 = C.c_uint32 * 4
 
 
 def _sizes(v):
-    return _U32x4(*map(int, v))
+    v = [*map(int, v)]
+    a = _U32x4(*v)
+    if a[:len(v)] != v:
+        _refuse("a size does not fit 32 bits")
+    return a
+
+
+# ctypes takes a number that does not fit its type for what its low bits are: the calls below refuse it instead.
+def _refuse(what):
+    raise SrxError(1, what)
+
+
+def _codes_fit(bits):
+    """Data types, activations and numbers of groups, one or-ed with another: 31 bits."""
+    if bits >> 31:
+        _refuse("a data type, activation or number of groups is out of range")
+
+
+def _counts_fit(bits):
+    if bits >> 64:
+        _refuse("a number of rows, columns or bytes is out of range")
 
 
 def layer_plan(kind, dtype, in_sizes, param, in_bytes=0, out_bytes=0):
@@ -349,6 +369,7 @@ def layer_add(dtype, a_ptr, b_ptr, out_ptr, count, stream=None):
 
 def layer_mx4_sizes(rows, columns):
     """Host-only: (code bytes, scale bytes) of rows x columns values in the 4-bit block form."""
+    _counts_fit(rows | columns)
     c, s = C.c_uint64(), C.c_uint64()
     _check(lib().srx_layer_mx4_sizes(rows, columns, C.byref(c), C.byref(s)))
     return c.value, s.value
@@ -356,16 +377,21 @@ def layer_mx4_sizes(rows, columns):
 
 def layer_quantize_mx4(dtype, in_ptr, rows, columns, codes_ptr, scales_ptr, stream=None):
     """rows x columns values (dtype 0 fp16 / 1 fp32) to the 4-bit block form, on device pointers."""
+    _codes_fit(dtype)
+    _counts_fit(rows | columns)
     _check(lib().srx_layer_quantize_mx4(dtype, in_ptr, rows, columns, codes_ptr, scales_ptr, stream))
 
 
 def layer_dequantize_mx4(dtype, codes_ptr, scales_ptr, rows, columns, out_ptr, stream=None):
     """What the 4-bit block form of rows x columns values stands for."""
+    _codes_fit(dtype)
+    _counts_fit(rows | columns)
     _check(lib().srx_layer_dequantize_mx4(dtype, codes_ptr, scales_ptr, rows, columns, out_ptr, stream))
 
 
 def layer_group_norm_workspace(dtype, sizes, groups):
     """Host-only: bytes of device workspace of layer_group_norm and layer_group_norm_mx4 for sizes {N, C, H, W}."""
+    _codes_fit(dtype | groups)
     n = C.c_size_t()
     _check(lib().srx_layer_group_norm_workspace(dtype, C.byref(_sizes(sizes)), groups, C.byref(n)))
     return n.value
@@ -374,6 +400,8 @@ def layer_group_norm_workspace(dtype, sizes, groups):
 def layer_group_norm(dtype, in_ptr, sizes, groups, scale_ptr, bias_ptr, epsilon, activation, out_ptr, workspace_ptr,
                      workspace_bytes, stream=None):
     """Group normalisation with an activation (ACT_*) of a channels-last tensor; scale and bias may be None."""
+    _codes_fit(dtype | groups | activation)
+    _counts_fit(workspace_bytes)
     _check(lib().srx_layer_group_norm(dtype, in_ptr, C.byref(_sizes(sizes)), groups, scale_ptr, bias_ptr, epsilon, activation,
                                       out_ptr, workspace_ptr, workspace_bytes, stream))
 
@@ -381,6 +409,8 @@ def layer_group_norm(dtype, in_ptr, sizes, groups, scale_ptr, bias_ptr, epsilon,
 def layer_group_norm_mx4(dtype, in_ptr, sizes, groups, scale_ptr, bias_ptr, epsilon, activation, codes_ptr, scales_ptr,
                          workspace_ptr, workspace_bytes, stream=None):
     """The same, with the result in the 4-bit block form (one row per pixel)."""
+    _codes_fit(dtype | groups | activation)
+    _counts_fit(workspace_bytes)
     _check(lib().srx_layer_group_norm_mx4(dtype, in_ptr, C.byref(_sizes(sizes)), groups, scale_ptr, bias_ptr, epsilon,
                                           activation, codes_ptr, scales_ptr, workspace_ptr, workspace_bytes, stream))
 
@@ -388,6 +418,7 @@ def layer_group_norm_mx4(dtype, in_ptr, sizes, groups, scale_ptr, bias_ptr, epsi
 def layer_conv2d_mx4(dtype, codes_ptr, scales_ptr, sizes, filter_codes_ptr, filter_scales_ptr, filter_sizes, bias_ptr,
                      activation, out_ptr, stream=None):
     """Convolution of a 4-bit tensor with a 4-bit filter (rows in the order O, kh, kw); a 1x1 filter is the matrix product."""
+    _codes_fit(dtype | activation)
     _check(lib().srx_layer_conv2d_mx4(dtype, codes_ptr, scales_ptr, C.byref(_sizes(sizes)), filter_codes_ptr, filter_scales_ptr,
                                       C.byref(_sizes(filter_sizes)), bias_ptr, activation, out_ptr, stream))
 

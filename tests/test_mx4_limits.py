@@ -35,3 +35,35 @@ def test_pixels_are_counted_past_64_bits(n, h, w):
 def test_the_largest_tensor_is_taken():
     assert S.layer_plan(2, 0, (1, 1, (1 << 20) - 1, (1 << 20) + 1), (1, 1, 1, 1))[0] == (1, 1, (1 << 20) - 1, (1 << 20) + 1)
     refused(S.layer_plan, 2, 0, (1, 1, 1 << 20, 1 << 20), (1, 1, 1, 1))
+
+
+@pytest.mark.parametrize("by", [1 << 32, -(1 << 32), 1 << 64])
+def test_numbers_past_their_type_are_refused(by):
+    """Not taken for what their low bits are."""
+    sizes = (1, 8, 4, 4)
+    for i in range(4):
+        far = tuple(v + by * (k == i) for k, v in enumerate(sizes))
+        refused(S.layer_group_norm_workspace, 0, far, 2)
+        assert "32 bits" in refused(S.layer_conv2d_mx4, 0, P, P, far, P, P, (5, 8, 3, 3), None, 0, P)
+        assert "32 bits" in refused(S.layer_conv2d_mx4, 0, P, P, sizes, P, P, far, None, 0, P)
+        assert "32 bits" in refused(S.layer_plan, 0, 0, far, (5, 8, 3, 3))
+    refused(S.layer_group_norm_workspace, 0, sizes, 2 + by)
+    refused(S.layer_group_norm_workspace, by, sizes, 2)
+    for call in (S.layer_group_norm, lambda *a: S.layer_group_norm_mx4(*a[:8], P, *a[8:])):
+        for dtype, groups, act, nbytes in ((by, 2, 0, 1 << 20), (0, 2 + by, 0, 1 << 20), (0, 2, by, 1 << 20), (0, 2, 0, -1), (0, 2, 0, (1 << 64) + (1 << 20))):
+            assert "out of range" in refused(call, dtype, P, sizes, groups, P, P, 1e-5, act, P, P, nbytes)
+    assert "out of range" in refused(S.layer_conv2d_mx4, by, P, P, sizes, P, P, (5, 8, 3, 3), None, 0, P)
+    assert "out of range" in refused(S.layer_conv2d_mx4, 0, P, P, sizes, P, P, (5, 8, 3, 3), None, by, P)
+
+
+@pytest.mark.parametrize("rows,columns", [((1 << 64) + 3, 32), (3, (1 << 64) + 32), (3 - (1 << 64), 32), (-1, 32), (3, -32)])
+def test_rows_and_columns_past_64_bits_are_refused(rows, columns):
+    refused(S.layer_mx4_sizes, rows, columns)
+    assert "out of range" in refused(S.layer_quantize_mx4, 0, P, rows, columns, P, P)
+    assert "out of range" in refused(S.layer_dequantize_mx4, 0, P, P, rows, columns, P)
+
+
+@pytest.mark.parametrize("sizes", [(1, 8, 4), (1, 8, 4, 4, 1)])
+def test_sizes_are_four(sizes):
+    with pytest.raises((S.SrxError, IndexError)):
+        S.layer_group_norm_workspace(0, sizes, 2)
