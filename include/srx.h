@@ -358,8 +358,8 @@ srx_status srx_layer_group_norm_workspace(int32_t dtype, const uint32_t sizes[4]
  *     out = act((in - mean) / sqrt(variance + epsilon) * scale[c] + bias[c]).
  * epsilon is a positive normal number; scale and bias are C values of the tensor's type, NULL stands for 1 and 0.
  * `out` may be `in` (no other operands of these layers may overlap an output).  A NaN or an infinity makes NaN of its
- * group, and so do fp32 values whose sum, or whose squared deviations' sum, passes the range of fp32.  The workspace may
- * be reused by the next call on the same stream. */
+ * group, and so do fp32 values whose squared deviations' sum passes the range of fp32; where only their sum passes it,
+ * the group may be NaN.  The workspace may be reused by the next call on the same stream. */
 srx_status srx_layer_group_norm(int32_t dtype, const void* in, const uint32_t sizes[4], uint32_t groups,
                                 const void* scale, const void* bias, float epsilon, int32_t activation, void* out,
                                 void* workspace, size_t workspace_bytes, void* stream);

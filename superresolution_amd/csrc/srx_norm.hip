@@ -98,18 +98,25 @@ __device__ __forceinline__ float sumLanes(float v, int lanes)
     return v;
 }
 
+// What a thread's sums about a value of its own are held in.  fp32 values may lie so far apart that squares of 256 times the
+// distance pass the range of fp32 while the sum of their squared deviations does not; fp16 values cannot.
+template <typename T> struct SumOf { typedef double type; };
+template <> struct SumOf<f16> { typedef float type; };
+
 // Sum of squared deviations from sums about another point: rounding may leave it below zero, a NaN stays one.
-__device__ __forceinline__ float spread(float squares, float sum, float inverseCount)
+template <typename S>
+__device__ __forceinline__ float spread(S squares, S sum, S inverseCount)
 {
-    const float m2 = squares - sum * sum * inverseCount;
-    return m2 < 0.0f ? 0.0f : m2;
+    const S m2 = squares - sum * (sum * inverseCount);
+    return m2 < S(0) ? 0.0f : float(m2);
 }
 
-// 1 / sqrt(v): the special function unit's estimate (one part in 2^22) and one Newton step.
+// 1 / sqrt(v): the special function unit's estimate (one part in 2^22) and one Newton step.  An infinity, which stands for a
+// variance past the range of fp32, gives NaN (the estimate is zero: normalised values would all be the bias).
 __device__ __forceinline__ float inverseRoot(float v)
 {
     const float r = __builtin_amdgcn_rsqf(v);
-    return v < 3.0e38f ? fmaf(0.5f * r, fmaf(-v * r, r, 1.0f), r) : r;
+    return fmaf(0.5f * r, fmaf(-v * r, r, 1.0f), r);
 }
 
 // Threads that share one group's reduction when `threads` of them reduce `groups` groups.
@@ -403,7 +410,9 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
     {
         const int m = min(kVec, tileC - col * kVec);
         const T* src = in + col * kVec;
-        float k[kVec], s[kVec], q[kVec];
+        typedef typename SumOf<T>::type Sum;
+        float k[kVec];
+        Sum s[kVec], q[kVec];
         // The odd pixels first, then whole batches, the next of which is asked for before the current one is summed up.
         constexpr int kFlight = 4;
         const int mine = row < count ? (count - row + rows - 1) / rows : 0, odd = mine % kFlight;
@@ -416,7 +425,7 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
         };
         const auto sum = [&](const Held<T>& x) {
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) { const float d = x.get(i) - k[i]; s[i] += d; q[i] = fmaf(d, d, q[i]); }
+            for (int i = 0; i < kVec; ++i) { const Sum d = x.get(i) - k[i]; s[i] += d; q[i] = __builtin_elementwise_fma(d, d, q[i]); }
         };
 #pragma unroll
         for (int u = 0; u < kFlight - 1; ++u)
@@ -428,7 +437,7 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
             for (int u = 0; u < kFlight; ++u) load(v[u], at + u * step);
         }
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) { k[i] = odd ? first[0].get(i) : (mine ? v[0].get(i) : 0.0f); s[i] = q[i] = 0.0f; }
+        for (int i = 0; i < kVec; ++i) { k[i] = odd ? first[0].get(i) : (mine ? v[0].get(i) : 0.0f); s[i] = q[i] = 0; }
 #pragma unroll
         for (int u = 0; u < kFlight - 1; ++u)
             if (u < odd) sum(first[u]);
@@ -449,11 +458,11 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
 #pragma unroll
             for (int u = 0; u < kFlight; ++u) sum(v[u]);
         }
-        const float inv = 1.0f / float(max(1, mine));
+        const Sum inv = 1.0f / float(max(1, mine));
 #pragma unroll
         for (int i = 0; i < kVec; ++i)
         {
-            sMean[(row * vecs + col) * kVec + i] = fmaf(s[i], inv, k[i]);
+            sMean[(row * vecs + col) * kVec + i] = float(__builtin_elementwise_fma(s[i], inv, Sum(k[i])));
             sM2[(row * vecs + col) * kVec + i] = spread(q[i], s[i], inv);
         }
     }

@@ -1,0 +1,81 @@
+"""Group normalisation of fp32 values at the end of their range, and of values far from the others, against the definition in
+64 bits.  Helpers and tolerances are those of test_gpu_mx4."""
+import pytest
+import torch
+
+import superresolution_amd as S
+from test_gpu_mx4 import Guarded, U, check_codes, group_norm, norm64, norm_tolerance, step, stream
+
+pytestmark = pytest.mark.gpu
+
+# n, c, h, w, groups: one workgroup holds one group, several groups; parts joined by the output kernel, by a kernel of their own
+SHAPES = [(2, 64, 8, 9, 2), (2, 96, 16, 16, 12), (2, 64, 120, 100, 2), (2, 64, 600, 500, 4)]
+WIDE = (2, 4224, 5, 3, 1)                                        # a group wider than a workgroup
+
+
+def noise(shape, seed):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed))
+
+
+@pytest.mark.parametrize("size", [3e38, 1e20, None])
+@pytest.mark.parametrize("n,c,h,w,groups", SHAPES + [WIDE])
+def test_squares_past_the_range_make_nan(size, n, c, h, w, groups):
+    """Of image 1, group 0: squares that pass the range of fp32, and squares a 64th of it whose sum passes it."""
+    k = c // groups
+    x = noise((n, h, w, c), 1)
+    sign = torch.where(torch.arange(h * w * k) % 2 == 0, 1.0, -1.0).reshape(h, w, k)
+    ref, *parts = norm64(x, groups, None, None, 1e-5, 2)
+    x[1, :, :, :k] = sign * (size or 2.0 ** 61)
+    got = group_norm(x, 1, groups, None, None, 2)
+    assert got[1, :, :, :k].isnan().all()
+    other = torch.ones(n, h, w, c, dtype=torch.bool)
+    other[1, :, :, :k] = False
+    assert ((got.double() - ref).abs() <= step(1, ref) + norm_tolerance(*parts))[other].all()
+    codes, scales = group_norm(x, 1, groups, None, None, 2, mx4=True)
+    blocks = -(-c // 32)
+    bad = torch.zeros(n, h * w, blocks, dtype=torch.bool)
+    bad[1, :, :-(-k // 32)] = True                               # blocks that hold a value of the group
+    assert torch.equal((scales.whole() == 255).reshape(bad.shape), bad)
+    assert (codes.whole().reshape(*bad.shape, 16)[bad] == 0).all()
+
+
+@pytest.mark.parametrize("n,c,h,w,groups", SHAPES + [WIDE])
+def test_squares_within_the_range_are_normalised(n, c, h, w, groups):
+    """The squared deviations' sum is a quarter of fp32's range."""
+    k = c // groups
+    x = noise((n, h, w, c), 2) * (2.0 ** 126 / (h * w * k)) ** 0.5
+    ref, *parts = norm64(x, groups, None, None, 1e-5, 0)
+    got = group_norm(x, 1, groups, None, None, 0)
+    assert ((got.double() - ref).abs() <= step(1, ref) + norm_tolerance(*parts)).all()
+    check_codes(*group_norm(x, 1, groups, None, None, 0, mx4=True), ref.reshape(-1, c), norm_tolerance(*parts).reshape(-1, c))
+
+
+@pytest.mark.parametrize("n,c,h,w,groups", SHAPES)
+def test_one_value_takes_half_the_range(n, c, h, w, groups):
+    """The first value of every group is 2^63.5 and the others are small against it: the squared deviations' sum is half the range
+    of fp32, but squares about that value pass it from the third on."""
+    x = noise((n, h, w, c), 3)
+    x[:, 0, 0, ::c // groups] = 2.0 ** 63.5
+    ref, *parts = norm64(x, groups, None, None, 1e-5, 0)
+    got = group_norm(x, 1, groups, None, None, 0)
+    assert ((got.double() - ref).abs() <= step(1, ref) + norm_tolerance(*parts)).all()
+
+
+def test_a_sum_whose_square_passes_the_range():
+    """256 values of a thread about a first one 1e17 away: the square of their sum passes the range of fp32, nothing else does."""
+    n, h, w, c, d = 1, 8192, 8192, 4, 1e17
+    x = torch.randn(n, h, w, c, device="cuda", generator=torch.Generator("cuda").manual_seed(2)) * 1e10
+    x.view(-1, c)[65536] = d                                     # the first pixel of a part
+    v = x.double().view(-1, 2, 2)
+    mean = v.mean(dim=(0, 2))
+    v = v - mean[:, None]
+    rstd = 1 / torch.sqrt((v ** 2).mean(dim=(0, 2)) + 1e-5)
+    want = (v * rstd[:, None]).view(n, h, w, c)
+    out = torch.empty_like(x)
+    need = S.layer_group_norm_workspace(1, (n, c, h, w), 2)
+    work = Guarded((need,), torch.uint8)
+    S.layer_group_norm(1, x.data_ptr(), (n, c, h, w), 2, None, None, 1e-5, 0, out.data_ptr(), work.ptr(), need, stream())
+    torch.cuda.synchronize()
+    # The two far values of each group are squared about themselves: differences are off by U d, their squares' sum by 2 U of
+    # itself (256 d^2, of a variance of d^2), which halves in the result; 80 half steps for the rest, as in norm_tolerance.
+    assert ((out.double() - want).abs() <= U * (256 * want.abs() + 80 * (want.abs() + 1))).all()
