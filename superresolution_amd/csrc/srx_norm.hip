@@ -98,6 +98,19 @@ __device__ __forceinline__ float sumLanes(float v, int lanes)
     return v;
 }
 
+// Sum over a workgroup of kThreads, in each of its threads.  `waves` holds a value of each wave, of this call alone.
+__device__ __forceinline__ double sumThreads(double v, double* waves)
+{
+#pragma unroll
+    for (int i = 32; i > 0; i >>= 1) v += __shfl_xor(v, i);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) v += waves[i];
+    return v;
+}
+
 // What a thread's sums about a value of its own are held in.  fp32 values may lie so far apart that squares of 256 times the
 // distance pass the range of fp32 while the sum of their squared deviations does not; fp16 values cannot.
 template <typename T> struct SumOf { typedef double type; };
@@ -371,8 +384,10 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
 
     if (vecs > kThreads)
     {
-        // one group wider than a workgroup: every value belongs to it
-        float k = 0.0f, s = 0.0f, q = 0.0f;
+        // One group wider than a workgroup: every value belongs to it, and a thread adds up thousands of them about its first one.
+        // In 32 bits the rounding of those sums would drown the spread where the first value is far from the others.
+        // (The sums are kept in halves, which do not wait for each other.)
+        double k = 0.0, s[2] = {0.0, 0.0}, q[2] = {0.0, 0.0};
         int have = 0;
         for (int p = 0; p < count; ++p)
             for (int col = tid; col < vecs; col += kThreads)
@@ -384,24 +399,17 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
                 have += m;
 #pragma unroll
                 for (int i = 0; i < kVec; ++i)
-                    if (i < m) { const float d = v[i] - k; s += d; q = fmaf(d, d, q); }
+                {
+                    const double d = i < m ? v[i] - k : 0.0;
+                    s[i & 1] += d;
+                    q[i & 1] = fma(d, d, q[i & 1]);
+                }
             }
-        const float cnt = float(have), total = float(count) * float(tileC);
-        const float mean = have ? k + s / cnt : 0.0f, m2 = have ? spread(q, s, 1.0f / cnt) : 0.0f;
-        sMean[tid] = cnt * mean;
-        __syncthreads();
-        float all = 0.0f;
-        for (int i = 0; i < kThreads; ++i) all += sMean[i];
-        all /= total;
-        const float d = mean - all;
-        sM2[tid] = m2 + cnt * d * d;
-        __syncthreads();
-        if (tid == 0)
-        {
-            float r = 0.0f;
-            for (int i = 0; i < kThreads; ++i) r += sM2[i];
-            out[0] = float2{all, r};
-        }
+        // (vecs > kThreads: every thread has values)
+        const double inverse = 1.0 / have, sum = s[0] + s[1], mean = k + sum * inverse;
+        const double all = sumThreads(have * k + sum, reinterpret_cast<double*>(sMean)) / (double(count) * tileC), d = mean - all;
+        const double m2 = sumThreads(double(spread(q[0] + q[1], sum, inverse)) + have * d * d, reinterpret_cast<double*>(sM2));
+        if (tid == 0) out[0] = float2{float(all), float(m2)};
         return;
     }
 
@@ -458,7 +466,7 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
 #pragma unroll
             for (int u = 0; u < kFlight; ++u) sum(v[u]);
         }
-        const Sum inv = 1.0f / float(max(1, mine));
+        const Sum inv = Sum(1) / Sum(max(1, mine));
 #pragma unroll
         for (int i = 0; i < kVec; ++i)
         {

@@ -50,7 +50,7 @@ def test_squares_within_the_range_are_normalised(n, c, h, w, groups):
     check_codes(*group_norm(x, 1, groups, None, None, 0, mx4=True), ref.reshape(-1, c), norm_tolerance(*parts).reshape(-1, c))
 
 
-@pytest.mark.parametrize("n,c,h,w,groups", SHAPES)
+@pytest.mark.parametrize("n,c,h,w,groups", SHAPES + [WIDE, (1, 1 << 18, 3, 1, 2)])
 def test_one_value_takes_half_the_range(n, c, h, w, groups):
     """The first value of every group is 2^63.5 and the others are small against it: the squared deviations' sum is half the range
     of fp32, but squares about that value pass it from the third on."""
@@ -76,6 +76,37 @@ def test_a_sum_whose_square_passes_the_range():
     work = Guarded((need,), torch.uint8)
     S.layer_group_norm(1, x.data_ptr(), (n, c, h, w), 2, None, None, 1e-5, 0, out.data_ptr(), work.ptr(), need, stream())
     torch.cuda.synchronize()
-    # The two far values of each group are squared about themselves: differences are off by U d, their squares' sum by 2 U of
-    # itself (256 d^2, of a variance of d^2), which halves in the result; 80 half steps for the rest, as in norm_tolerance.
-    assert ((out.double() - want).abs() <= U * (256 * want.abs() + 80 * (want.abs() + 1))).all()
+    # A difference of the 255 is off by U d at most, and counts with the d / 256 that it is off their mean: 2 U d^2 of the sum of
+    # squared deviations, which is d^2, and half of that in the result; 80 half steps for the rest, as in norm_tolerance.
+    assert ((out.double() - want).abs() <= U * (want.abs() + 80 * (want.abs() + 1))).all()
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("n,c,h,w", [(1, 1 << 20, 2, 1), (1, 4100, 5, 3), (2, 100003, 3, 1), (8, 2064, 64, 64)])
+def test_wide_group_first_values_far_from_the_others(dtype, n, c, h, w):
+    """A group wider than a workgroup, whose threads add up thousands of values (2^20 channels: 4096) about the first one."""
+    x = noise((n, h, w, c), 4)
+    x[:, 0, 0, :2048:8] += 300                                   # the first value of each of 256 threads
+    x = x.to(torch.float32 if dtype else torch.float16)
+    ref, *parts = norm64(x, 1, None, None, 1e-5, 0)
+    got = group_norm(x, dtype, 1, None, None, 0)
+    assert ((got.double() - ref).abs() <= step(dtype, ref) + norm_tolerance(*parts)).all()
+
+
+def test_wide_group_in_parts_of_many_values():
+    """So many images that a workgroup takes 241 pixels of one: threads add up 1928 to 3856 values, the first of which is far."""
+    n, c, h, w = 64, 2064, 64, 64
+    x = torch.randn(n, h * w, c, device="cuda", generator=torch.Generator("cuda").manual_seed(5))
+    x[:, ::241, :2048:8] += 300
+    out = torch.empty_like(x)
+    need = S.layer_group_norm_workspace(1, (n, c, h, w), 1)
+    assert need == n * -(-h * w // 241) * 8
+    work = Guarded((need,), torch.uint8)
+    S.layer_group_norm(1, x.data_ptr(), (n, c, h, w), 1, None, None, 1e-5, 0, out.data_ptr(), work.ptr(), need, stream())
+    work.whole()
+    for i in range(n):
+        v = x[i].double()
+        var, mean = torch.var_mean(v, correction=0)
+        rstd = 1 / torch.sqrt(var + 1e-5)
+        v = (v - mean) * rstd
+        assert ((out[i].double() - v).abs() <= U * (v.abs() + 80 * (float(mean.abs() * rstd) + v.abs() + 1))).all()
