@@ -794,9 +794,11 @@ NormPlan planNorm(const ML::Operator& op, bool mx4)
     if (chunks > kJoin) chunks = imageBytes <= int64_t(kJoin) * (192 << 10) ? kJoin : (imageBytes + (64 << 10) - 1) / (64 << 10);
     const int64_t most = (1024 + n * a.tiles - 1) / (n * a.tiles);
     if (chunks > most) chunks = most;
-    // No thread adds up more than 256 values of a channel (parts of 1 MB in fp16): the rounding of its sums, about a first value
-    // that may be far from the others, grows with their number.
-    const int64_t longest = kThreads * int64_t(256) / vecsFor<false>(a.tileGroups * a.groupC);
+    // No thread adds up more than 256 values of a channel (parts of 1 MB in fp16, if its rows fill the workgroup): the rounding of
+    // its sums, about a first value that may be far from the others, grows with their number.  Threads of a group wider than the
+    // workgroup add up all its channels, in 64 bits; their parts are cut to about the same size.
+    const int64_t vecs = vecsFor<false>(a.tileGroups * a.groupC);
+    const int64_t longest = vecs <= kThreads ? 256 * (kThreads / vecs) : 256 * kThreads / vecs;
     const int64_t least = longest > 1 ? (a.pixels + longest - 1) / longest : a.pixels;
     if (chunks < least) chunks = least;
     a.chunkPixels = int((a.pixels + chunks - 1) / chunks);

@@ -110,3 +110,31 @@ def test_wide_group_in_parts_of_many_values():
         rstd = 1 / torch.sqrt(var + 1e-5)
         v = (v - mean) * rstd
         assert ((out[i].double() - v).abs() <= U * (v.abs() + 80 * (float(mean.abs() * rstd) + v.abs() + 1))).all()
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_one_row_of_threads_first_values_far_from_the_others(dtype):
+    """1032 channels: 129 threads a pixel, so that one row of them adds up a part's pixels, the first of which is far."""
+    n, c, h, w, d = 64, 1032, 64, 64, 300.0
+    x = torch.randn(n, h * w, c, device="cuda", generator=torch.Generator("cuda").manual_seed(6))
+    x[:, ::256] += d
+    x = x.to(torch.float32 if dtype else torch.float16)
+    out = torch.empty_like(x)
+    need = S.layer_group_norm_workspace(dtype, (n, c, h, w), 1)
+    assert need == n * 16 * 8                                    # 16 parts of 256 pixels
+    work = Guarded((need,), torch.uint8)
+    S.layer_group_norm(dtype, x.data_ptr(), (n, c, h, w), 1, None, None, 1e-5, 0, out.data_ptr(), work.ptr(), need, stream())
+    work.whole()
+    # fp16: sums in 32 bits, as in test_group_norm_first_value_far_from_the_others, but every channel of every part has a far value
+    off = 1.5 * 256 ** 2 * U * d ** 2 / (256 + d ** 2) / 2 if dtype == 0 else 0
+    for i in range(n):
+        v = x[i].double()
+        var, mean = torch.var_mean(v, correction=0)
+        rstd = 1 / torch.sqrt(var + 1e-5)
+        v = (v - mean) * rstd
+        tol = off * v.abs() + U * (80 * (float(mean.abs() * rstd) + v.abs() + 1) + d * rstd)
+        if dtype == 0:
+            tol += v.abs() * 2.0 ** -11 + 2.0 ** -25 + 256 * U * d * rstd        # and each part's mean
+        else:
+            tol += U * v.abs()
+        assert ((out[i].double() - v).abs() <= tol).all()

@@ -67,3 +67,19 @@ def test_rows_and_columns_past_64_bits_are_refused(rows, columns):
 def test_sizes_are_four(sizes):
     with pytest.raises((S.SrxError, IndexError)):
         S.layer_group_norm_workspace(0, sizes, 2)
+
+
+@pytest.mark.parametrize("n,c,h,w,groups", [
+    (1024, 1032, 20, 25, 1), (64, 1032, 128, 128, 1), (64, 2040, 128, 128, 8), (64, 696, 200, 200, 3), (256, 2048, 64, 64, 4),
+    (64, 5000, 64, 64, 50), (1, 4, 8192, 8192, 2), (1024, 8, 256, 256, 2), (2, 520, 2048, 2048, 1)])
+def test_parts_are_short_enough_for_sums_in_32_bits(n, c, h, w, groups):
+    """The statistics of an image come in parts (a mean and a sum of squares of 4 bytes each, and once more where there are over
+    64), whose pixels 256 threads of eight channels share: no thread may add up more than 256 of them."""
+    need = S.layer_group_norm_workspace(0, (n, c, h, w), groups)
+    parts = need // (n * groups * 8)
+    assert need == parts * n * groups * 8
+    parts -= parts > 64
+    pixels = -(-h * w // parts)
+    k = c // groups
+    vecs = -(-k * min(groups, 2048 // k) // 8)                   # of a workgroup's whole groups
+    assert vecs <= 256 and -(-pixels // (256 // vecs)) <= 256
