@@ -503,7 +503,8 @@ __global__ __launch_bounds__(kThreads) void NormStatsKernel(const NormArgs a)
 }
 
 // The parts of one group of one image joined by `lanes` lanes: (mean, 1 / deviation).  PER parts of each lane are asked for
-// at once and kept; more than that only images of over 2^32 pixels have.
+// at once and kept.  A lane has more where the output kernel's lanes share over 32 groups (64 parts over four lanes and less), and
+// in NormJoinKernel from 1024 parts on (the least that images of over 2^18 pixels of 2048 channels, or 2^26 of 8, come in).
 template <int PER>
 __device__ __forceinline__ float2 joinParts(const NormArgs& a, const float2* partial, int lane, int lanes)
 {

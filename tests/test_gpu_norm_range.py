@@ -138,3 +138,36 @@ def test_one_row_of_threads_first_values_far_from_the_others(dtype):
         else:
             tol += U * v.abs()
         assert ((out[i].double() - v).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("n,c,h,w,groups", [(1, 64, 256, 190, 64), (1, 128, 128, 190, 128), (1, 512, 60, 90, 512), (2, 90, 150, 210, 45)])
+def test_many_groups_of_many_parts(dtype, n, c, h, w, groups):
+    """The output kernel joins up to 64 parts of a group by four lanes and fewer: 16 to 64 parts a lane."""
+    x = noise((n, h, w, c), 7) * torch.exp2(noise((c,), 8)) + noise((c,), 9)
+    x = x.to(torch.float32 if dtype else torch.float16)
+    parts = S.layer_group_norm_workspace(dtype, (n, c, h, w), groups) // (n * groups * 8)
+    assert parts == 64
+    ref, *rest = norm64(x, groups, None, None, 1e-5, 2)
+    got = group_norm(x, dtype, groups, None, None, 2)
+    assert ((got.double() - ref).abs() <= step(dtype, ref) + norm_tolerance(*rest)).all()
+    blocks = group_norm(x, dtype, groups, None, None, 2, mx4=True)
+    check_codes(*blocks, ref.reshape(-1, c), norm_tolerance(*rest).reshape(-1, c))
+
+
+def test_more_parts_than_a_wave_keeps():
+    """1040 parts of an image, joined by the 64 lanes of a wave."""
+    n, c, h, w, groups = 1, 1032, 520, 512, 8
+    x = torch.randn(h * w, groups, c // groups, device="cuda", generator=torch.Generator("cuda").manual_seed(8)).half()
+    x[:, 3] += torch.linspace(-3, 3, h * w, device="cuda")[:, None].half()      # parts with means of their own
+    need = S.layer_group_norm_workspace(0, (n, c, h, w), groups)
+    assert need == (1040 + 1) * groups * 8
+    out, work = torch.empty_like(x), Guarded((need,), torch.uint8)
+    S.layer_group_norm(0, x.data_ptr(), (n, c, h, w), groups, None, None, 1e-5, 0, out.data_ptr(), work.ptr(), need, stream())
+    work.whole()
+    for g in range(groups):
+        v = x[:, g].double()
+        var, mean = torch.var_mean(v, correction=0)
+        rstd = 1 / torch.sqrt(var + 1e-5)
+        v = (v - mean) * rstd
+        assert ((out[:, g].double() - v).abs() <= v.abs() * 2.0 ** -11 + 2.0 ** -25 + U * 80 * (float(mean.abs() * rstd) + v.abs() + 1)).all()
