@@ -1,6 +1,8 @@
 // What the kernels of the convolution of 4-bit operands share (internal header; srx_conv_mx4.hip has the mathematics).
 #pragma once
 
+#include <optional>
+
 #include "srx_mx4.h"
 
 namespace srx {
@@ -158,9 +160,13 @@ inline bool scalesInWords(const ConvMxArgs& a)
     return a.blocks % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.scales) | reinterpret_cast<uintptr_t>(a.wScales)) & 3) == 0;
 }
 
-// ConvMxTapsKernel with tiles of 32, 64, 96 or 128 channels.  hipErrorInvalidConfiguration, and no launch, where the window does
-// not fit half a CU's LDS, where the tiles at the images' edges are a quarter empty, or where there are too few.
-hipError_t launchConvMxTaps(bool half, int channels, const ConvMxArgs& a, hipStream_t s);
+// What became of a launch; nothing where the kernel does not suit the sizes and none was tried.  (A launch that was tried and
+// failed is an error, whatever its code: no other kernel may cover it up.)
+typedef std::optional<hipError_t> Launched;
+
+// ConvMxTapsKernel with tiles of 32, 64, 96 or 128 channels.  Nothing where the window does not fit half a CU's LDS, where the
+// tiles at the images' edges are a quarter empty, or where there are too few.
+Launched launchConvMxTaps(bool half, int channels, const ConvMxArgs& a, hipStream_t s);
 
 }  // namespace dev
 }  // namespace srx

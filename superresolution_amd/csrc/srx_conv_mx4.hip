@@ -652,8 +652,9 @@ __global__ __launch_bounds__(kThreads, 2) void ConvMxWindowKernel(const ConvMxAr
     // nothing is in flight: the last tile fetched no other
 }
 
+// Nothing where the filters or the window do not fit.
 template <typename T, int FO, int NL>
-hipError_t launchWindow(const ConvMxArgs& args, WindowArgs w, hipStream_t s)
+Launched launchWindow(const ConvMxArgs& args, WindowArgs w, hipStream_t s)
 {
     using L = WindowLds<T, FO, NL>;
     ConvMxArgs a = args;
@@ -661,7 +662,7 @@ hipError_t launchWindow(const ConvMxArgs& args, WindowArgs w, hipStream_t s)
     a.byTilesO = Divider(unsigned(a.tilesO));
     const void* kernel = reinterpret_cast<const void*>(ConvMxWindowKernel<T, FO, NL>);
     const int lds = L::bytes(w.steps), most = 160 << 10;
-    if (lds > most) return hipErrorInvalidConfiguration;
+    if (lds > most) return {};
     const hipError_t e = dev::ensureDynamicLds(kernel, most);
     if (e != hipSuccess) return e;
     // as many workgroups as the device holds at a time, in eights
@@ -673,12 +674,11 @@ hipError_t launchWindow(const ConvMxArgs& args, WindowArgs w, hipStream_t s)
     hipLaunchKernelGGL((ConvMxWindowKernel<T, FO, NL>), dim3(unsigned(slots * a.tilesO)), dim3(kThreads), lds, s, a, w);
     return hipGetLastError();
 }
-// hipErrorInvalidConfiguration, and no launch, where the filters or the window do not fit.
 template <typename T, int FO>
-hipError_t launchWindow(const ConvMxArgs& a, hipStream_t s)
+Launched launchWindow(const ConvMxArgs& a, hipStream_t s)
 {
     // (the rows of a window are eight more than the taps')
-    if (a.blocks > 2 || (int64_t(a.taps / a.kw + kWinH) * a.W + a.kw + kWinW) * a.blocks * kMxBytes >= int64_t(kRange)) return hipErrorInvalidConfiguration;
+    if (a.blocks > 2 || (int64_t(a.taps / a.kw + kWinH) * a.W + a.kw + kWinW) * a.blocks * kMxBytes >= int64_t(kRange)) return {};
     WindowArgs w{};
     const int winH = kWinH + a.taps / a.kw - 1;
     w.winW = kWinW + a.kw - 1;
@@ -694,7 +694,7 @@ hipError_t launchWindow(const ConvMxArgs& a, hipStream_t s)
     if (w.units <= 2 * kThreads) return launchWindow<T, FO, 2>(a, w, s);
     if (w.units <= 4 * kThreads) return launchWindow<T, FO, 4>(a, w, s);
     if (w.units <= 7 * kThreads) return launchWindow<T, FO, 7>(a, w, s);
-    return hipErrorInvalidConfiguration;
+    return {};
 }
 
 template <typename T, int THREADS, int BO, int BP, int FO, int FP>
@@ -775,8 +775,8 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
     // leave room for 32 channels at a time only (960x540: 33 instead of 46).
     if (a.blocks <= 2 && a.O <= 128 && (a.taps == 1 || padded(64) <= padded(96)) && a.W >= kWinW && a.H >= kWinH && tiles(64, 256) >= 768)
     {
-        const hipError_t e = !half ? launchWindow<float, 1>(a, s) : a.O <= 32 ? launchWindow<f16, 1>(a, s) : launchWindow<f16, 2>(a, s);
-        if (e != hipErrorInvalidConfiguration) return e;
+        const Launched e = !half ? launchWindow<float, 1>(a, s) : a.O <= 32 ? launchWindow<f16, 1>(a, s) : launchWindow<f16, 2>(a, s);
+        if (e) return *e;
     }
     // Several taps: the window staged once (launchConvMxTaps refuses where tiles are few or empty), with the tile that computes least
     // beyond what is needed; a tile of 96 channels takes a twentieth longer for a channel than one of 128, one of 64 a quarter, but
@@ -789,11 +789,11 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
     {
         const bool brief = a.total <= 2 * kChunk;
         const int64_t by128 = padded(128) * 20, by96 = padded(96) * (brief ? 19 : 21), by64 = padded(64) * (brief ? 18 : 25);
-        const hipError_t e = a.O <= 32                          ? launchConvMxTaps(half, 32, a, s)
-                             : by128 <= by96 && by128 <= by64 ? launchConvMxTaps(half, 128, a, s)
-                             : by96 <= by64                     ? launchConvMxTaps(half, 96, a, s)
-                                                                : launchConvMxTaps(half, 64, a, s);
-        if (e != hipErrorInvalidConfiguration) return e;
+        const Launched e = a.O <= 32                          ? launchConvMxTaps(half, 32, a, s)
+                           : by128 <= by96 && by128 <= by64 ? launchConvMxTaps(half, 128, a, s)
+                           : by96 <= by64                     ? launchConvMxTaps(half, 96, a, s)
+                                                              : launchConvMxTaps(half, 64, a, s);
+        if (e) return *e;
     }
     // The largest tile that leaves no CU without one: 256x256 reads a quarter of what 64x64 does (2048 -> 2048 channels, 1x1,
     // 16384 pixels: 54 instead of 93 us), but 64 such tiles for 2048 pixels take 19 instead of 12.

@@ -317,18 +317,18 @@ __global__ __launch_bounds__(kThreads, FO > 3 || PARTS ? 2 : FO > 2 ? 3 : 4) voi
 
 // Too few tiles: 96 -> 96 channels, 3x3, 200x200, 175 of them: 9.9 instead of 11.9 us; 180x180, 138: 9.6 instead of 8.3.
 template <typename T, int FO>
-hipError_t launchTaps(const ConvMxArgs& args, hipStream_t s)
+Launched launchTaps(const ConvMxArgs& args, hipStream_t s)
 {
     using L = TapsLds<T, FO>;
     ConvMxArgs a = args;
     TapsArgs w{};
     const int winH = kWinH + a.taps / a.kw - 1;
-    if ((int64_t(winH) * a.W + a.kw + kWinW) * a.blocks * kMxBytes >= int64_t(kRange)) return hipErrorInvalidConfiguration;
+    if ((int64_t(winH) * a.W + a.kw + kWinW) * a.blocks * kMxBytes >= int64_t(kRange)) return {};
     w.tilesX = (a.W + kWinW - 1) / kWinW;
     w.tilesY = (a.H + kWinH - 1) / kWinH;
     a.tilesO = (a.O + L::kBO - 1) / L::kBO;
     a.tilesP = a.pixels / (a.H * a.W) * w.tilesX * w.tilesY;
-    if (int64_t(a.tilesP) * a.tilesO < 160 || int64_t(a.tilesP) * (kWinW * kWinH * 4) > int64_t(a.pixels) * 5) return hipErrorInvalidConfiguration;
+    if (int64_t(a.tilesP) * a.tilesO < 160 || int64_t(a.tilesP) * (kWinW * kWinH * 4) > int64_t(a.pixels) * 5) return {};
     const bool words = scalesInWords(a);
     w.parts = (a.blocks + kChunk - 1) / kChunk;
     w.last = a.blocks - (w.parts - 1) * kChunk;
@@ -337,15 +337,15 @@ hipError_t launchTaps(const ConvMxArgs& args, hipStream_t s)
     const int units = w.winPixels * (w.parts > 1 ? kChunk : w.last);
     w.scales = (units + 63) / 64 * 1024;
     const int lds = L::bytes(w.scales + (words ? (units / 4 + 63) / 64 * 256 : units)), most = 80 << 10;
-    if (units > kTapsLoads * kThreads || lds > most) return hipErrorInvalidConfiguration;
+    if (units > kTapsLoads * kThreads || lds > most) return {};
     w.byLast = Divider(unsigned(w.last));
     w.byTilesX = Divider(unsigned(w.tilesX));
     w.byTilesY = Divider(unsigned(w.tilesY));
     w.byWinW = Divider(unsigned(w.winW));
     a.byTilesO = Divider(unsigned(a.tilesO));
     const int64_t grid = int64_t(a.tilesO) * ((int64_t(a.tilesP) + 7) / 8 * 8);
-    if (grid > INT32_MAX) return hipErrorInvalidConfiguration;
-    const auto launchAs = [&](auto kernel) {
+    if (grid > INT32_MAX) return {};
+    const auto launchAs = [&](auto kernel) -> Launched {
         const hipError_t e = dev::ensureDynamicLds(reinterpret_cast<const void*>(kernel), most);
         if (e != hipSuccess) return e;
         hipLaunchKernelGGL(kernel, gridOf(grid), dim3(kThreads), lds, s, a, w);
@@ -355,14 +355,14 @@ hipError_t launchTaps(const ConvMxArgs& args, hipStream_t s)
     return words ? launchAs(ConvMxTapsKernel<T, FO, true, false>) : launchAs(ConvMxTapsKernel<T, FO, false, false>);
 }
 template <typename T>
-hipError_t launchTaps(int channels, const ConvMxArgs& a, hipStream_t s)
+Launched launchTaps(int channels, const ConvMxArgs& a, hipStream_t s)
 {
     return channels == 128 ? launchTaps<T, 4>(a, s) : channels == 96 ? launchTaps<T, 3>(a, s) : channels == 64 ? launchTaps<T, 2>(a, s) : launchTaps<T, 1>(a, s);
 }
 
 }  // namespace
 
-hipError_t dev::launchConvMxTaps(bool half, int channels, const ConvMxArgs& a, hipStream_t s)
+Launched dev::launchConvMxTaps(bool half, int channels, const ConvMxArgs& a, hipStream_t s)
 {
     return half ? launchTaps<f16>(channels, a, s) : launchTaps<float>(channels, a, s);
 }

@@ -1,0 +1,55 @@
+"""What the normalisation and 4-bit layers launch, without a GPU: their host side linked with a runtime that launches nothing
+(mx4_launch.cpp)."""
+import os
+import subprocess
+
+import pytest
+
+from conftest import ROOT
+
+CSRC = os.path.join(ROOT, "superresolution_amd", "csrc")
+OBJECTS = [os.path.join(CSRC, "build", f + ".o") for f in ("srx_conv_mx4", "srx_conv_mx4_taps", "srx_norm", "srx_layers", "srx_weights")]
+OK, INVALID_CONFIGURATION, LAUNCH_FAILURE = 0, 9, 719
+
+
+@pytest.fixture(scope="module")
+def program(tmp_path_factory):
+    if not all(os.path.exists(o) for o in OBJECTS):
+        subprocess.check_call(["make", "-j4", "-C", CSRC])
+    out = str(tmp_path_factory.mktemp("mx4_launch") / "mx4_launch")
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I" + CSRC, "-I" + os.path.join(ROOT, "include"),
+                           "-o", out, os.path.join(ROOT, "tests", "mx4_launch.cpp")] + OBJECTS)
+
+    def run(*args):
+        lines = subprocess.check_output([out] + [str(a) for a in args], text=True, timeout=60).splitlines()
+        assert lines[-1].startswith("status ")
+        return int(lines[-1].split()[1]), lines[:-1]
+    return run
+
+
+# dtype, n, c, h, w, o, kh, kw and the kernel
+CONVS = [((0, 1, 64, 1080, 1920, 64, 3, 3), "ConvMxWindowKernel"), ((1, 1, 32, 540, 960, 64, 3, 3), "ConvMxWindowKernel"),
+         ((0, 1, 512, 256, 256, 512, 3, 3), "ConvMxTapsKernel"), ((1, 1, 96, 200, 215, 96, 3, 3), "ConvMxTapsKernel"),
+         ((0, 1, 96, 540, 960, 40, 3, 3), "ConvMxTapsKernel"), ((0, 1, 128, 540, 960, 32, 3, 3), "ConvMxTapsKernel"),
+         ((0, 1, 4096, 1, 1, 4096, 1, 1), "ConvMxRowsKernel"), ((0, 4, 256, 128, 128, 256, 1, 1), "ConvMxKernel")]
+
+
+@pytest.mark.parametrize("case,kernel", CONVS)
+def test_one_kernel_makes_the_convolution(program, case, kernel):
+    status, launched = program("conv", *case, OK)
+    assert status == OK and len(launched) == 1 and kernel in launched[0]
+
+
+@pytest.mark.parametrize("error", [INVALID_CONFIGURATION, LAUNCH_FAILURE])
+@pytest.mark.parametrize("case,kernel", CONVS)
+def test_a_failed_launch_is_not_covered_up(program, case, kernel, error):
+    """Its error is the call's: no second kernel runs over the same output."""
+    status, launched = program("conv", *case, error)
+    assert status == error and len(launched) == 1 and kernel in launched[0]
+
+
+@pytest.mark.parametrize("case", [(0, 2, 64, 8, 9, 2, 0), (1, 1, 64, 600, 500, 4, 0), (0, 1, 256, 256, 256, 32, 1)])
+def test_a_failed_normalisation_stops(program, case):
+    assert program("norm", *case, OK)[0] == OK
+    status, launched = program("norm", *case, INVALID_CONFIGURATION)
+    assert status == INVALID_CONFIGURATION and len(launched) == 1
