@@ -45,16 +45,20 @@ __device__ __forceinline__ i32x4 descriptor(const uint8_t* p, unsigned range)
     const uint64_t at = reinterpret_cast<uint64_t>(p);
     return i32x4{int(unsigned(at)), int(unsigned(at >> 32) & 0xffffu), int(range), 0x00027000};
 }
-// 16 bytes a lane from memory to LDS, lane after lane from the address `lds` on, without registers.  The compiler does
-// not count this load: whoever reads the data waits for it (vmcnt) and for the other waves (s_barrier) first.
+// 16 bytes a lane from memory to LDS, lane after lane from the address `lds` on, without registers.  The address goes by m0, an
+// output, so that the compiler does not take what it wrote there for still there (an input, which the compiler would write,
+// cost a tile kernel bound by its output 2 %).  The compiler does not count this load: whoever reads the data waits for it (vmcnt)
+// and for the other waves (s_barrier) first.
 __device__ __forceinline__ void loadToLds(i32x4 from, unsigned offset, unsigned lds)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(from) : "memory");
+    unsigned m0;
+    asm volatile("s_mov_b32 %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds" : "=&{m0}"(m0) : "s"(lds), "v"(offset), "s"(from) : "memory");
 }
 // The same with 4 bytes a lane.
 __device__ __forceinline__ void loadWordToLds(i32x4 from, unsigned offset, unsigned lds)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(from) : "memory");
+    unsigned m0;
+    asm volatile("s_mov_b32 %0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, 0 offen lds" : "=&{m0}"(m0) : "s"(lds), "v"(offset), "s"(from) : "memory");
 }
 __device__ __forceinline__ unsigned loadByte(i32x4 from, unsigned offset)
 {
