@@ -1153,7 +1153,7 @@ srx_status groupNorm(const char* who, int32_t dtype, const void* in, const uint3
     const OnDeviceOf scope(in);
     if (!scope.valid) return fail(SRX_ERR_INVALID, std::string(who) + kNotOnDevice);
     SRX_HIP(srx::LaunchGroupNorm(op, in, scale, bias, out, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales),
-                                 workspace, static_cast<hipStream_t>(stream)));
+                                 workspace, workspaceBytes, static_cast<hipStream_t>(stream)));
     return SRX_OK;
 }
 }  // namespace

@@ -734,6 +734,9 @@ hipError_t launch(bool half, const ConvMxArgs& a, hipStream_t s)
 hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uint8_t* scales, const uint8_t* filterCodes,
                          const uint8_t* filterScales, const void* bias, void* out, hipStream_t s)
 {
+    if (op.kind != ML::Operator::Kind::CONVOLUTION_MX4 || !codes || !scales || !filterCodes || !filterScales || !out ||
+        ((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(filterCodes)) & 15))
+        return hipErrorInvalidValue;
     ConvMxArgs a{};
     a.codes = codes;
     a.scales = scales;

@@ -119,7 +119,8 @@ hipError_t LaunchConv(const ConvLaunch& l, int numCUs, hipStream_t s);
 
 // Generic layers (srx_layers.hip): run an operator made by ML::Util::Create*Layer on dense device
 // tensors.  CONVOLUTION: (input, filter, bias or nullptr, output); UPSAMPLE_2D: (input, -, -, output);
-// ELEMENT_WISE_ADD: (a, b, -, output), output may alias a or b.
+// ELEMENT_WISE_ADD: (a, b, -, output), output may alias a or b.  GROUP_NORM and CONVOLUTION_MX4 have other operands and are
+// refused here: LaunchGroupNorm and LaunchConvMx4 run them.
 hipError_t DispatchOperator(const ML::Operator& op, const void* input, const void* filterOrB, const void* bias,
                             void* output, hipStream_t s);
 // CSImageToTensor / PSTensorToImage for a {batch, 3, height, width} tensor of any data type and layout.
@@ -128,12 +129,14 @@ hipError_t LaunchImageToTensor(const Image& src, void* tensor, ML::TensorDataTyp
 hipError_t LaunchTensorToImage(const void* tensor, const Image& dst, ML::TensorDataType t, ML::TensorLayout layout,
                                int width, int height, int batch, hipStream_t s);
 
-// Group normalisation (srx_norm.hip): out (or codes and scales, the 4-bit block form) from dense channels-last tensors.
-// scale and bias may be null; the workspace holds GroupNormWorkspace(op) bytes.
+// The layers below run on the current device.  Operators of another kind, missing pointers, codes that are not at a multiple of
+// 16 bytes and workspaces too small are refused with hipErrorInvalidValue, before anything is launched.
+// Group normalisation (srx_norm.hip): out, or codes and scales (the 4-bit block form; out is null), from dense channels-last
+// tensors.  scale and bias may be null; the workspace (a multiple of 8) holds GroupNormWorkspace(op) bytes.
 size_t GroupNormWorkspace(const ML::Operator& op);
-hipError_t LaunchGroupNorm(const ML::Operator& op, const void* in, const void* scale, const void* bias, void* out,
-                           uint8_t* codes, uint8_t* scales, void* workspace, hipStream_t s);
-// Rows of `columns` values to and from the 4-bit block form (srx_norm.hip).
+hipError_t LaunchGroupNorm(const ML::Operator& op, const void* in, const void* scale, const void* bias, void* out, uint8_t* codes,
+                           uint8_t* scales, void* workspace, size_t workspaceBytes, hipStream_t s);
+// Rows of `columns` values (at most 2^20) to and from the 4-bit block form (srx_norm.hip).
 hipError_t LaunchQuantizeMx4(ML::TensorDataType t, const void* in, int64_t rows, int64_t columns, uint8_t* codes,
                              uint8_t* scales, hipStream_t s);
 hipError_t LaunchDequantizeMx4(ML::TensorDataType t, const uint8_t* codes, const uint8_t* scales, int64_t rows,

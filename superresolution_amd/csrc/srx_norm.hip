@@ -879,14 +879,19 @@ hipError_t launchNorm(const NormPlan& p, hipStream_t s)
 
 size_t GroupNormWorkspace(const ML::Operator& op)
 {
+    if (op.kind != ML::Operator::Kind::GROUP_NORM) return 0;
     const size_t plain = normWorkspace(planNorm(op, false)), mx4 = normWorkspace(planNorm(op, true));
     return plain > mx4 ? plain : mx4;
 }
 
 hipError_t LaunchGroupNorm(const ML::Operator& op, const void* in, const void* scale, const void* bias, void* out,
-                           uint8_t* codes, uint8_t* scales, void* workspace, hipStream_t s)
+                           uint8_t* codes, uint8_t* scales, void* workspace, size_t workspaceBytes, hipStream_t s)
 {
+    if (op.kind != ML::Operator::Kind::GROUP_NORM || !in || !codes != !scales || !out == !codes || (reinterpret_cast<uintptr_t>(codes) & 15))
+        return hipErrorInvalidValue;
     NormPlan p = planNorm(op, codes != nullptr);
+    const size_t need = normWorkspace(p);
+    if (need && (!workspace || workspaceBytes < need || (reinterpret_cast<uintptr_t>(workspace) & 7))) return hipErrorInvalidValue;
     NormArgs& a = p.a;
     a.in = in;
     a.scale = scale;
@@ -904,6 +909,7 @@ hipError_t LaunchGroupNorm(const ML::Operator& op, const void* in, const void* s
 namespace {
 bool planMx(int64_t rows, int64_t columns, int bytes, MxArgs& a, dim3& grid)
 {
+    if (rows < 1 || columns < 1 || columns > 1 << 20 || rows >= int64_t(1) << 40) return false;
     a.columns = columns;
     a.values = rows * columns;
     a.rowUnits = unsigned(4 * mxBlocks(columns));
@@ -921,6 +927,7 @@ hipError_t LaunchQuantizeMx4(ML::TensorDataType t, const void* in, int64_t rows,
 {
     MxArgs a{};
     dim3 grid;
+    if (!in || !codes || !scales || (reinterpret_cast<uintptr_t>(codes) & 15)) return hipErrorInvalidValue;
     if (!planMx(rows, columns, t == ML::TensorDataType::FLOAT16 ? 2 : 4, a, grid)) return hipErrorInvalidValue;
     a.in = in;
     a.codes = codes;
@@ -935,6 +942,7 @@ hipError_t LaunchDequantizeMx4(ML::TensorDataType t, const uint8_t* codes, const
 {
     MxArgs a{};
     dim3 grid;
+    if (!codes || !scales || !out || (reinterpret_cast<uintptr_t>(codes) & 15)) return hipErrorInvalidValue;
     if (!planMx(rows, columns, t == ML::TensorDataType::FLOAT16 ? 2 : 4, a, grid)) return hipErrorInvalidValue;
     a.codesIn = codes;
     a.scalesIn = scales;

@@ -185,15 +185,17 @@ bool Util::CreateConvolutionMx4Layer(const uint32_t inputSizes[4], const uint32_
 {
     uint64_t ib = 0, ob = 0;
     uint32_t os[4];
+    Operator op;
     if (m_layout != TensorLayout::NHWC || activation > uint32_t(Activation::SILU)) return false;
-    if (!CreateConvolutionLayer(inputSizes, filterSizes, false, ib, ob, os, opOut)) return false;
+    if (!CreateConvolutionLayer(inputSizes, filterSizes, false, ib, ob, os, op)) return false;
     if (filterSizes[2] > 7 || filterSizes[3] > 7 || inputSizes[1] > kMaxChannels || filterSizes[0] > kMaxChannels) return false;
     if (uint64_t(inputSizes[0]) * inputSizes[2] * inputSizes[3] > uint64_t(INT32_MAX)) return false;
     if (!validSizes(os)) return false;
     // the filters of a tile lie within 2^31 bytes of each other
     if (uint64_t(filterSizes[2]) * filterSizes[3] * ((inputSizes[1] + 31) / 32) >= (1u << 19)) return false;
-    opOut.kind = Operator::Kind::CONVOLUTION_MX4;
-    opOut.activation = Activation(activation);
+    op.kind = Operator::Kind::CONVOLUTION_MX4;
+    op.activation = Activation(activation);
+    opOut = op;                                                         // (untouched where the sizes are refused)
     return true;
 }
 

@@ -53,3 +53,7 @@ def test_a_failed_normalisation_stops(program, case):
     assert program("norm", *case, OK)[0] == OK
     status, launched = program("norm", *case, INVALID_CONFIGURATION)
     assert status == INVALID_CONFIGURATION and len(launched) == 1
+
+
+def test_what_the_launchers_refuse(program):
+    assert program("refusals") == (0, [])
