@@ -1,6 +1,7 @@
 """ctypes binding of libsrx.so (include/srx.h)."""
 import ctypes as C
 import os
+import struct
 import subprocess
 import weakref
 
@@ -119,10 +120,10 @@ def load_library(path):
     L.srx_layer_mx4_sizes.argtypes = [u64, u64, C.POINTER(u64), C.POINTER(u64)]
     L.srx_layer_quantize_mx4.argtypes = [i32, vp, u64, u64, vp, vp, vp]
     L.srx_layer_dequantize_mx4.argtypes = [i32, vp, vp, u64, u64, vp, vp]
-    L.srx_layer_group_norm_workspace.argtypes = [i32, u32x4, u32, C.POINTER(sz)]
-    L.srx_layer_group_norm.argtypes = [i32, vp, u32x4, u32, vp, vp, f32, i32, vp, vp, sz, vp]
-    L.srx_layer_group_norm_mx4.argtypes = [i32, vp, u32x4, u32, vp, vp, f32, i32, vp, vp, vp, sz, vp]
-    L.srx_layer_conv2d_mx4.argtypes = [i32, vp, vp, u32x4, vp, vp, u32x4, vp, i32, vp, vp]
+    L.srx_layer_group_norm_workspace.argtypes = [i32, vp, u32, C.POINTER(sz)]
+    L.srx_layer_group_norm.argtypes = [i32, vp, vp, u32, vp, vp, f32, i32, vp, vp, sz, vp]
+    L.srx_layer_group_norm_mx4.argtypes = [i32, vp, vp, u32, vp, vp, f32, i32, vp, vp, vp, sz, vp]
+    L.srx_layer_conv2d_mx4.argtypes = [i32, vp, vp, vp, vp, vp, vp, vp, i32, vp, vp]
     for name in SYMBOLS:
         if name not in ("srx_stage_name", "srx_last_error", "srx_frames_per_launch", "srx_pipe_slots", "srx_static_scratch_bytes"):
             getattr(L, name).restype = i32
@@ -332,6 +333,20 @@ def _refuse(what):
     raise SrxError(1, what)
 
 
+_pack4 = struct.Struct("4I").pack
+
+
+def _four(v):
+    """Four sizes as the bytes of a uint32_t[4] (1 us less than a ctypes array)."""
+    try:
+        return _pack4(*v)
+    except struct.error:
+        try:
+            return _pack4(*map(int, v))
+        except struct.error:
+            _refuse("sizes are four numbers of 32 bits")
+
+
 def _codes_fit(bits):
     """Data types, activations and numbers of groups, one or-ed with another: 31 bits."""
     if bits >> 31:
@@ -393,7 +408,7 @@ def layer_group_norm_workspace(dtype, sizes, groups):
     """Host-only: bytes of device workspace of layer_group_norm and layer_group_norm_mx4 for sizes {N, C, H, W}."""
     _codes_fit(dtype | groups)
     n = C.c_size_t()
-    _check(lib().srx_layer_group_norm_workspace(dtype, C.byref(_sizes(sizes)), groups, C.byref(n)))
+    _check(lib().srx_layer_group_norm_workspace(dtype, _four(sizes), groups, C.byref(n)))
     return n.value
 
 
@@ -402,7 +417,7 @@ def layer_group_norm(dtype, in_ptr, sizes, groups, scale_ptr, bias_ptr, epsilon,
     """Group normalisation with an activation (ACT_*) of a channels-last tensor; scale and bias may be None."""
     _codes_fit(dtype | groups | activation)
     _counts_fit(workspace_bytes)
-    _check(lib().srx_layer_group_norm(dtype, in_ptr, C.byref(_sizes(sizes)), groups, scale_ptr, bias_ptr, epsilon, activation,
+    _check(lib().srx_layer_group_norm(dtype, in_ptr, _four(sizes), groups, scale_ptr, bias_ptr, epsilon, activation,
                                       out_ptr, workspace_ptr, workspace_bytes, stream))
 
 
@@ -411,7 +426,7 @@ def layer_group_norm_mx4(dtype, in_ptr, sizes, groups, scale_ptr, bias_ptr, epsi
     """The same, with the result in the 4-bit block form (one row per pixel)."""
     _codes_fit(dtype | groups | activation)
     _counts_fit(workspace_bytes)
-    _check(lib().srx_layer_group_norm_mx4(dtype, in_ptr, C.byref(_sizes(sizes)), groups, scale_ptr, bias_ptr, epsilon,
+    _check(lib().srx_layer_group_norm_mx4(dtype, in_ptr, _four(sizes), groups, scale_ptr, bias_ptr, epsilon,
                                           activation, codes_ptr, scales_ptr, workspace_ptr, workspace_bytes, stream))
 
 
@@ -419,8 +434,8 @@ def layer_conv2d_mx4(dtype, codes_ptr, scales_ptr, sizes, filter_codes_ptr, filt
                      activation, out_ptr, stream=None):
     """Convolution of a 4-bit tensor with a 4-bit filter (rows in the order O, kh, kw); a 1x1 filter is the matrix product."""
     _codes_fit(dtype | activation)
-    _check(lib().srx_layer_conv2d_mx4(dtype, codes_ptr, scales_ptr, C.byref(_sizes(sizes)), filter_codes_ptr, filter_scales_ptr,
-                                      C.byref(_sizes(filter_sizes)), bias_ptr, activation, out_ptr, stream))
+    _check(lib().srx_layer_conv2d_mx4(dtype, codes_ptr, scales_ptr, _four(sizes), filter_codes_ptr, filter_scales_ptr,
+                                      _four(filter_sizes), bias_ptr, activation, out_ptr, stream))
 
 
 def fold_weights(layer, weights_path=None):
