@@ -7,21 +7,23 @@
 // instruction multiplies two blocks: lanes 0-31 hold one of them for 32 rows (or columns), lanes 32-63 the other, 16
 // bytes and one scale byte each, so that the two blocks may come from different taps.  fp32 accumulation.
 //
-// Four kernels, chosen by LaunchConvMx4 (ConvMxTapsKernel is in srx_conv_mx4_taps.hip); times of the kernels themselves, fp16
-// results (they differ by 5 % between devices, and by as much between operands of all bit patterns and those of a normalised
-// layer: the power limit):
-//   ConvMxRowsKernel    few pixels; bound by the latency of one trip to memory and of the join.  One row times 4096 x 4096: 6.0 us
-//                       (8.9 MB of filter: 1.5 TB/s).
+// Four kernels, chosen by LaunchConvMx4 (ConvMxTapsKernel is in srx_conv_mx4_taps.hip).  Times here and beside the rules are of the
+// kernels themselves, back to back, with fp16 results and operands quantised from normal values; devices differ by 5 - 7 %, and
+// operands of all bit patterns cost the wide layers 5 % more (the power limit).
+//   ConvMxRowsKernel    few pixels; bound by the latency of one trip to memory and of the join, and up to 15 pixels by the 64 that
+//                       its tile has room for where there are many channels.  One row times 4096 x 4096: 5.3 us (8.9 MB of filter:
+//                       1.7 TB/s; 1.9 us at what reads alone reach); 16 rows 6.3, 64 rows 8.8.
 //   ConvMxWindowKernel  up to 64 channels on large images; bound by the output's bytes.  64 -> 64 channels, 3x3, 1920x1080:
-//                       74 us (336 MB: 4.5 TB/s; 2.1 PFLOP/s).
-//   ConvMxTapsKernel    several taps.  512 -> 512 channels, 3x3, 256x256: 76 - 81 us, 3.8 - 4.0 PFLOP/s; 256 -> 256: 26, 3.0; 96 -> 96,
-//                       960x540: 47 us (126 MB: 2.7 TB/s; 1.8 PFLOP/s), bound by the start and end of its tiles as much as by the
+//                       75 - 79 us (336 MB: 4.3 - 4.5 TB/s; 2.0 PFLOP/s).
+//   ConvMxTapsKernel    several taps.  512 -> 512 channels, 3x3, 256x256: 74 us, 4.2 PFLOP/s; 256 -> 256: 25, 3.1; 96 -> 96,
+//                       960x540: 42 us (126 MB: 3.0 TB/s; 2.0 PFLOP/s), bound by the start and end of its tiles as much as by the
 //                       products.
-//   ConvMxKernel        everything else.  2048 -> 2048 channels, 1x1, 16384 pixels: 55 us, 2.5 PFLOP/s; 512 -> 512, 65536 pixels:
-//                       24 us (103 MB: 4.3 TB/s).
+//   ConvMxKernel        everything else.  2048 -> 2048 channels, 1x1, 16384 pixels: 48 us, 2.8 PFLOP/s: one workgroup fits a CU, so
+//                       nothing runs beside a tile's first load, its turn through LDS and its stores; 512 -> 512, 65536 pixels:
+//                       23 us (103 MB: 4.5 TB/s).
 // The matrix units alone reach 6.2 PFLOP/s on operands of all bit patterns held in registers (at the power limit; 7.7 on
-// constants), 5.5 where every operand is read from LDS.  Of 102 us that ConvMxKernel takes for 512 -> 512, 3x3, its loads from memory
-// cost 36 and its reads from LDS 15: L2, LDS and power together bound the wide layers.
+// constants), 5.5 where every operand is read from LDS.  Of the 102 us that ConvMxKernel took for 512 -> 512, 3x3, on operands of all
+// bit patterns, its loads from memory cost 36 and its reads from LDS 15: L2, LDS and power together bound the wide layers.
 #include "srx_conv_mx4.h"
 
 namespace srx {
@@ -61,9 +63,9 @@ __global__ __launch_bounds__(THREADS, 2) void ConvMxKernel(const ConvMxArgs a)
     float* const sBias = reinterpret_cast<float*>(dyn);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l = lane & 31;
     // Workgroups are dealt round-robin over the 8 XCDs.  Where there are enough pixel tiles, all channel tiles of the same
-    // pixels go to one XCD and share its L2 (512 -> 512 channels, 3x3, 256x256: 95 instead of 98 us; 128 -> 512, 1x1: 18.3
-    // and 18.6); pixels are dealt out singly (one long run of them for each XCD: 95, and 12.2 instead of 11.8 for 256 ->
-    // 256, 1x1).
+    // pixels go to one XCD and share its L2 (1x1, 2048 -> 2048 channels, 16384 pixels: 48 instead of 51 us; 512 -> 512, 65536
+    // pixels: 22.5 instead of 24.3; 128 -> 512: 18.5 and 18.7); pixels are dealt out singly (one long run of them for each XCD:
+    // 12.2 instead of 11.8 for 256 -> 256).
     const unsigned number = blockNumber();
     unsigned tileO, tileP;
     if (a.tilesP >= 64)
@@ -765,17 +767,18 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
 
     // Few pixels: the shared reduction (ConvMxRowsKernel), as wide as 256 workgroups allow, while what its workgroups read
     // (their number times 1 + FP rows of 16) takes less time than the chunks of a tile take one after the other.
-    // 4096 -> 4096 channels, 1x1: 5.3 (1 pixel), 8.9 (64) us instead of 9.4, 9.6 with tiles; 31 instead of 10.3 for 256
-    // pixels.  256 -> 256 channels, 3x3, 16x16: 4.0 instead of 6.6; 1024 -> 1024, 3x3, 8x8: 8.0 instead of 18.
+    // 4096 -> 4096 channels, 1x1: 5.3 (1 pixel), 6.3 (16), 8.8 (64) us instead of 9.5, 9.7, 9.7 with tiles; 31 instead of 10.3
+    // for 256 pixels.  256 -> 256 channels, 3x3, 16x16: 4.0 instead of 6.7; 1024 -> 1024, 3x3, 8x8: 8.0 instead of 18.
+    // (256: the CUs of the device, here and in the thresholds below, which are those of the measured crossings.)
     const int rows = tiles(16, 64) >= 256 ? 4 : tiles(16, 32) >= 256 ? 2 : 1;
     if (tiles(16, 16 * rows) * (1 + rows) < 1560 && tapsInRange(a))
         return rows == 4 ? launchRows<4>(half, a, s) : rows == 2 ? launchRows<2>(half, a, s) : launchRows<1>(half, a, s);
     const auto padded = [&](int64_t o) { return (a.O + o - 1) / o * o; };
-    // Up to 64 channels on large images: the window kernel.  64 -> 64 channels, 3x3: 90 instead of 162 us for 1920x1080
-    // (codes of all bit patterns; 74 - 78 for those of a normalised layer), 15 instead of 22 for 640x360 (900 tiles), 7.3
-    // and 7.4 for 320x180 (240); 1x1, 1920x1080: 65 instead of 88.  32 -> 128, 3x3, 512x512: 18 instead of 26; with more
-    // channel tiles the window is read as often as the tiles read it (64 -> 256, 3x3, 256x256: 14.7 and 15.9).  fp32 results
-    // leave room for 32 channels at a time only (960x540: 33 instead of 46).
+    // Up to 64 channels on large images: the window kernel.  64 -> 64 channels, 3x3: 79 us for 1920x1080 instead of 104 with
+    // ConvMxTapsKernel, 14.5 and 14.0 for 640x360 (900 tiles); 1x1, 1920x1080: 63 instead of 88 with tiles.  32 -> 32, 3x3, 512x512:
+    // 8.4 instead of 9.5, 32 -> 128: 18.4 instead of 19.5; with more channel tiles the window is read as often as the tiles read
+    // it (64 -> 256, 3x3, 256x256: 14.7 and 15.9).  fp32 results leave room for 32 channels at a time only (960x540: 31 instead of
+    // 33).
     if (a.blocks <= 2 && a.O <= 128 && (a.taps == 1 || padded(64) <= padded(96)) && a.W >= kWinW && a.H >= kWinH && tiles(64, 256) >= 768)
     {
         const Launched e = !half ? launchWindow<float, 1>(a, s) : a.O <= 32 ? launchWindow<f16, 1>(a, s) : launchWindow<f16, 2>(a, s);
@@ -784,10 +787,10 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
     // Several taps: the window staged once (launchConvMxTaps refuses where tiles are few or empty), with the tile that computes least
     // beyond what is needed; a tile of 96 channels takes a twentieth longer for a channel than one of 128, one of 64 a quarter, but
     // in short reductions, where the output takes the time, the smaller ones win (32 -> 384, 3x3, 512x512: 44 instead of 49 us;
-    // 32 -> 300: 43 instead of 52).  3x3, with tiles that read every pixel for every tap: 96 -> 96, 960x540: 47 instead of 75 us;
-    // 128 -> 128, 512x512: 33 instead of 42; 96 -> 64: 19 instead of 27; 96 -> 32: 14 instead of 20.8; 160 -> 160, 256x256: 19.8
-    // instead of 22.7; 384 -> 384: 55 instead of 70; 512 -> 512: 88 instead of 94; 64 -> 96, 512x512: 21 instead of 25 with the
-    // window kernel.
+    // 32 -> 300: 43 instead of 52).  3x3, instead of tiles that read every pixel for every tap: 96 -> 96, 960x540: 42 instead of 74
+    // us; 128 -> 128, 512x512: 30 instead of 38; 96 -> 64: 17 instead of 26; 96 -> 32: 13.4 instead of 19; 160 -> 160, 256x256: 18
+    // instead of 21; 256 -> 256: 25 instead of 28; 384 -> 384: 50 instead of 66; 512 -> 512: 74 instead of 80; 64 -> 96, 512x512:
+    // 21 instead of 25 with the window kernel.
     if (a.taps > 1)
     {
         const bool brief = a.total <= 2 * kChunk;
@@ -798,11 +801,11 @@ hipError_t LaunchConvMx4(const ML::Operator& op, const uint8_t* codes, const uin
                                                               : launchConvMxTaps(half, 64, a, s);
         if (e) return *e;
     }
-    // The largest tile that leaves no CU without one: 256x256 reads a quarter of what 64x64 does (2048 -> 2048 channels, 1x1,
-    // 16384 pixels: 54 instead of 93 us), but 64 such tiles for 2048 pixels take 19 instead of 12.
+    // The largest tile that leaves no CU without one: 256x256 reads half of what 128x128 does (2048 -> 2048 channels, 1x1,
+    // 16384 pixels: 50 instead of 62 us), but 64 such tiles for 2048 pixels take 19 instead of 12.
     // 128x128: 13.0 instead of 15.3 us with 128x64 for 1024 -> 96, 1x1, 65536 pixels; 9.5 instead of 8.0 for half as many (256
     // tiles).  32x128: 27.5 instead of 29.4 with 64x64 for 1024 -> 32, 1x1, 262144 pixels; 42 instead of 54 for 288 -> 32, 3x3.
-    // Channels that only fill up a tile count: 1024 -> 160, 1x1, 65536 pixels in 256: 18.7 instead of 22 us, but 8 -> 416, 1x7, one
+    // Channels that only fill up a tile count: 1024 -> 160, 1x1, 65536 pixels in 256: 18.4 instead of 21 us, but 8 -> 416, 1x7, one
     // row of 100500 pixels in 512: 34 instead of 24 (nothing but the output takes time there).
     const bool deep = a.total > 2 * kChunk;
     if (a.O > 128 && tiles(256, 256) >= 256 && padded(256) * 10 <= padded(64) * (deep ? 14 : 10)) return launch<512, 256, 256, 4, 2>(half, a, s);

@@ -106,8 +106,8 @@ void clockProbeReport(ClockProbe* probe, const char* name, int blocks, hipStream
 int diagEnvInt(const char* name, int fallback);
 #endif  // SRX_DIAG
 
-// Raise a kernel's dynamic shared memory limit, once per (device, kernel).  Thread-safe.  Called at set-up
-// (PrepareFusedKernels, from srx_create), not on a launch.
+// Raise a kernel's dynamic shared memory limit, once per (device, kernel).  Thread-safe.  Called at set-up for the fused
+// kernels (PrepareFusedKernels, from srx_create), not on a launch; by the layers, which have no set-up, on every launch.
 hipError_t ensureDynamicLds(const void* kernel, int bytes);
 
 inline TensorD toDevice(const Tensor& t) { return TensorD{reinterpret_cast<f16*>(t.base), t.pitch, long(t.frame)}; }

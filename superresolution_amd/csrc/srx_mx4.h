@@ -10,7 +10,8 @@
 namespace srx {
 namespace dev {
 
-// Division of numbers below 2^31 by a constant d: (mulhi(n, mul) + n) >> shift.
+// Division of numbers below 2^31 by a constant d: (mulhi(n, mul) + n) >> shift, division by an invariant integer through
+// multiplication (Granlund and Montgomery, 1994).
 struct Divider
 {
     unsigned mul = 0, shift = 0, d = 1;

@@ -6,13 +6,16 @@
 //     y = act((x - mean) / sqrt(var + epsilon) * scale[c] + bias[c])
 // Statistics are kept as (mean, M2 = sum of squared deviations) of a part of the data and joined by
 //     M2 = sum M2_i + sum n_i (mean_i - mean)^2,
-// so nothing cancels when the mean is large against the deviation.  Everything is fp32, rounded once when stored.
+// so nothing cancels when the mean is large against the deviation.  Everything is fp32, rounded once when stored, but for the
+// statistics' sums of fp32 tensors and of groups wider than a workgroup, which are fp64 (NormStatsKernel).
 //
 // Times of the kernels themselves, and what bounds them (a large copy reaches 4.9 TB/s here, reads alone 6.4, writes 6.8):
 //   NormSlabKernel       512 channels of 16x16 pixels, fp16, SiLU: 5.0 us; one trip to memory, two joins in LDS.
-//   NormStatsKernel      64 channels of 1920x1080, fp16: 50 us, 5.3 TB/s of reads.
-//   NormApplyKernel      the same: 87 us, 6.1 TB/s of reads (half of them still cached) and writes.  256 channels of 256x256 to
-//                        4 bits: 9.0 + 13.5 us, 3.7 and 3.2 TB/s from the last-level cache; half of it is a launch's start and end.
+//   NormStatsKernel      64 channels of 1920x1080, fp16: 50 us, 5.3 TB/s of reads; fp32: 103 us, 5.2.  4096 channels of 64x64
+//                        pixels in one group, fp16: 13.5 us, 2.5 TB/s (one load in flight a thread).
+//   NormApplyKernel      the same: 89 us, 6.0 TB/s of reads (half of them still cached) and writes; fp32: 229.  256 channels of
+//                        256x256 to 4 bits: 9.5 + 13.8 us, 3.5 TB/s and 3.1 from the last-level cache; the output's 18 vector
+//                        instructions a value with SiLU take 71 % of the cycles that its CUs are busy.
 //   QuantizeKernel, DequantizeKernel   133 M values in fp16: 62 us (5.4 TB/s) and 48 us (6.9 TB/s): memory.
 #include "srx_mx4.h"
 
