@@ -356,7 +356,8 @@ __global__ __launch_bounds__(THREADS) void NormSlabKernel(const NormArgs a)
             }
         }
     total(s, [&](int g, float sum) { sStat[g].y = inverseRoot(fmaf(sum, inv, a.epsilon)); });
-    if (row >= rows) return;
+    // (in the last tile, whose threads may be more than its blocks', the others would write into the next pixel)
+    if (row >= rows || col >= vecsFor<MX4>(tileC)) return;
     f.prepare(a, sStat, g0, m, c);
     const Target<T> to(a, int64_t(n) * pixels + row, c, rows);
     forActivation(a.activation, [&](auto act) {

@@ -171,3 +171,18 @@ def test_more_parts_than_a_wave_keeps():
         rstd = 1 / torch.sqrt(var + 1e-5)
         v = (v - mean) * rstd
         assert ((out[:, g].double() - v).abs() <= v.abs() * 2.0 ** -11 + 2.0 ** -25 + U * 80 * (float(mean.abs() * rstd) + v.abs() + 1)).all()
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("n,c,h,w,groups", [(1, 399, 4, 9, 133), (2, 144, 8, 8, 3), (3, 120, 5, 5, 5), (1, 205, 9, 9, 41), (2, 112, 16, 16, 7), (3, 33, 5, 5, 33)])
+def test_last_tile_of_groups_narrower_than_the_others(dtype, n, c, h, w, groups):
+    """Images held in registers, whose groups come in tiles of whole blocks and a rest: nothing is written behind the rest's blocks,
+    where the next pixel's are."""
+    x = noise((n, h, w, c), 10).to(torch.float32 if dtype else torch.float16)
+    assert S.layer_group_norm_workspace(dtype, (n, c, h, w), groups) == 0
+    for act in range(3):
+        ref, *rest = norm64(x, groups, None, None, 1e-5, act)
+        blocks = group_norm(x, dtype, groups, None, None, act, mx4=True)
+        check_codes(*blocks, ref.reshape(-1, c), norm_tolerance(*rest).reshape(-1, c))
+        got = group_norm(x, dtype, groups, None, None, act)
+        assert ((got.double() - ref).abs() <= step(dtype, ref) + norm_tolerance(*rest)).all()
